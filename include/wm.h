@@ -443,6 +443,64 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
                                int P, int want_msle, float msle_eps, double *sums, float *Yhat,
                                void *workspace, size_t workspace_bytes, void *stream);
 
+/* ------------------------------------------------------------------ layers of experts --- */
+
+/* Element types of the entry points below; WM_F32 is the type of everything above. */
+#define WM_F32 0
+#define WM_F64 1
+#define WM_BF16 2
+#define WM_F16 3
+
+/* Dense layers of G experts in one launch: the rows of x (M, K) are sorted by expert, expert g owns
+ * rows offsets[g] .. offsets[g+1] - 1 (offsets: G + 1 int64 in DEVICE memory, never read by the host) and
+ * the weights W[g] (N, K), bias b[g] (N).  The reference trains such a family one member at a time: one
+ * linear map per WRF variable (multipleRegression.py:28-45,533-550).  x, W, b and y are all of `dtype`
+ * (WM_F32, WM_BF16 or WM_F16); sums are held in float32.
+ *   fwd       y[r] = act(W[g] x[r] + b[g]); b may be NULL; relu != 0 applies max(., 0)
+ *   bwd_data  gx[r] = W[g]^T gy[r], zeroed where mask_below <= 0 when mask_below != NULL (the post-ReLU
+ *             activation that fed this layer, shaped like gx); gy is the gradient of the pre-activation
+ *   bwd_wb    gW[g] = sum_r gy[r] x[r]^T, gb[g] = sum_r gy[r] (gb may be NULL); zeros for an expert
+ *             without rows; large sums are split over rows and joined in a fixed order through `workspace`
+ * Rows that no expert owns (before offsets[0], behind offsets[G]) get zeros in y and gx and add nothing to gW and
+ * gb.  Any values of offsets are safe: those outside 0 .. M count as the nearest inside, one below its
+ * predecessor counts as that.  Results are bitwise reproducible.  float32 products are formed from three
+ * bf16 pieces of each factor, with float32 accuracy; infinities and NaN come out as in float32 arithmetic.
+ * N, K <= 2^20, M <= 2^30, G <= 2^16. */
+int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, const int64_t *offsets,
+                         int G, int M, int N, int K, int dtype, int relu, void *stream);
+int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx,
+                              const int64_t *offsets, int G, int M, int N, int K, int dtype,
+                              void *stream);
+size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K);
+int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, void *workspace,
+                            size_t workspace_bytes, const int64_t *offsets, int G, int M, int N, int K,
+                            int dtype, void *stream);
+
+/* Dropout whose mask is a function of (seed, element) and never stored; no counterpart in the reference.
+ *   y[i] = (residual ? residual[i] : 0) + (u(e) >= t ? x[i] / (1 - t / 2^32) : 0)
+ * with t = p 2^32 rounded, e = offset + *offset_dev + i (offset_dev: an int64 in device memory or NULL, for
+ * a captured graph whose replays draw anew) and u(e) 32 bits: with z = the framework's hash of (seed, e / 4)
+ * -- the one of wm_synth_uniform_f32 -- bits 16 (e % 4) .. + 15 of z above the same bits of the hash of
+ * (seed, z).  The backward pass is the same call on the gradient, without residual.  A dropped element is an exact 0
+ * whatever x holds; p = 1 drops all.  n elements of `dtype`; y may be x or residual. */
+int wm_dropout(const void *x, const void *residual, void *y, int64_t n, int dtype, double p,
+               uint64_t seed, uint64_t offset, const int64_t *offset_dev, void *stream);
+
+/* 8-bit codes with a scale per row: scale[m] = max_k |x[m][k]| / 127 in float32, q[m][k] = x[m][k] / scale[m]
+ * (float32) rounded to even, within +-127.  A row of zeros: scale 0, codes 0; a row with an infinity or a
+ * NaN: scale NaN, codes 0.  x is (M, K) of `dtype`, q (M, K) int8.  Also packs weights: a scale per
+ * output channel of W (N, K).
+ * wm_dense_i8: y[m][n] = act((sum_k q[m][k] W[n][k]) scale[m] wscale[n] + b[n]) with x quantised by the call --
+ * what serves a trained Dense layer (convolution.py:175-176, model.predict) from weights of a byte each.
+ * W (G, N, K) int8, wscale and b (G, N) float32 (b may be NULL), y (M, N) of `dtype`; offsets as in
+ * wm_dense_grouped_fwd, or NULL with G = 1: all rows use the one W.  The sums are exact integers (K <= 2^17).
+ * The workspace (16-byte aligned) holds the codes and scales of x. */
+int wm_quantize_rows_i8(const void *x, int M, int K, int dtype, int8_t *q, float *scale, void *stream);
+size_t wm_dense_i8_workspace_bytes(int M, int K);
+int wm_dense_i8(const void *x, const int8_t *W, const float *wscale, const float *b, void *y,
+                const int64_t *offsets, int G, int M, int N, int K, int dtype, int relu,
+                void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------------ exchange step ------- */
 
 /* The one collective of the data-parallel path (SURVEY.md 8b ABI block, 8e) for hosts without
@@ -459,8 +517,6 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
  *                      asynchronous on `stream`; one call per step on the whole buffer;
  *   wm_comm_size       ranks of the live communicator, 0 if none;  wm_comm_destroy  frees it. */
 #define WM_COMM_ID_BYTES 128
-#define WM_F32 0
-#define WM_F64 1
 int wm_comm_unique_id(void *id128);
 int wm_comm_init(int rank, int nranks, const void *unique_id);
 int wm_comm_size(void);

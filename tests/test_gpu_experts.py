@@ -1,0 +1,489 @@
+"""GPU: the layers of experts -- grouped Dense products, dropout from the counter-based generator, the 8-bit
+integer product -- against plain float64 implementations on the CPU, and ExpertStack, which runs them together.
+
+Tolerances, fixed before the first run.  u = 2^-24.  A sum of n float32 additions is off by at most
+5 sqrt(n) u S (S = sum of the |products|) but for one element in 10^5 (the probabilistic bound, lambda = 5); a
+matrix instruction's additions and, for float32, the six piece products make n <= 1.5 K + 16.  float32's split leaves out
+products below 3 2^-26 S.  The result is then rounded to its type: finfo.eps / 2 of it.  float32 results are also held to the
+norm bound sqrt(n) u, which a missing piece product (2^-17 and up) cannot meet."""
+import numpy as np
+import pytest
+import torch
+
+from weather_model_amd import synth
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rows(seed, shape, dtype, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def close(got, ref, S, n, what, norm=True):
+    """got (device) against ref (float64) whose terms have absolute sum S over n additions each."""
+    got_t, ref = got.detach().cpu(), torch.as_tensor(ref)
+    assert got_t.shape == ref.shape, what
+    h = half_step(got_t.dtype)
+    acc = (5 * (1.5 * n + 16) ** 0.5 * U + 3 * 2.0 ** -26) * torch.as_tensor(S, dtype=torch.float64)
+    tiny = torch.finfo(got_t.dtype).tiny
+    bad = (got_t.double() - ref).abs() > (1 + h) * acc + h * ref.abs() + tiny
+    assert not bool(bad.any()), (what, int(bad.sum()), float((got_t.double() - ref).abs().max()))
+    if norm and got_t.dtype == torch.float32 and float(ref.norm()) > 0:
+        assert float((got_t.double() - ref).norm() / ref.norm()) <= (1.5 * n + 16) ** 0.5 * U, what
+
+
+def offsets_of(sizes, before=0):
+    return torch.tensor(np.cumsum([before] + list(sizes)), dtype=torch.int64, device="cuda")
+
+
+def grouped_ref(x, w, b, sizes, before, relu):
+    """(y, S) in float64 on the CPU"""
+    y = torch.zeros((x.shape[0], w.shape[1]), dtype=torch.float64)
+    S = torch.zeros_like(y)
+    at = before
+    for g, n in enumerate(sizes):
+        p = slice(at, at + n)
+        y[p] = x[p].double() @ w[g].double().t()
+        S[p] = x[p].double().abs() @ w[g].double().abs().t()
+        if b is not None:
+            y[p] += b[g].double()
+            S[p] += b[g].double().abs()
+        at += n
+    return (y.clamp(min=0) if relu else y), S
+
+
+SHAPES = [
+    # sizes, N, K, rows before, rows behind
+    ([1], 4, 4, 0, 0),
+    ([1], 8000, 640, 0, 0),
+    ([5, 0, 3, 130], 37, 19, 0, 0),
+    ([0, 0, 0], 16, 16, 3, 2),                     # nobody has rows
+    ([128, 256, 1], 128, 64, 0, 0),
+    ([129, 127, 0, 383], 216, 432, 2, 5),          # singleRegression's map
+    ([300] + [0] * 63 + [40], 65, 129, 0, 1),      # more than one wave of groups
+    (list(range(80)), 33, 40, 1, 0),
+    ([700, 900], 300, 520, 0, 0),
+    ([17, 2], 1, 1, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_grouped_forward(case, dtype):
+    from weather_model_amd import ops
+    sizes, N, K, before, behind = SHAPES[case]
+    M = before + sum(sizes) + behind
+    x, w, b = rows(case, (M, K), dtype), rows(case + 50, (len(sizes), N, K), dtype, K ** -0.5), rows(case + 90, (len(sizes), N), dtype, 0.3)
+    off = offsets_of(sizes, before)
+    for bias, relu in ((None, False), (b, True)):
+        y = ops.dense_grouped_forward(x.cuda(), w.cuda(), off, None if bias is None else bias.cuda(), relu=relu)
+        ref, S = grouped_ref(x, w, bias, sizes, before, relu)
+        close(y, ref, S, K, (case, relu))
+        inside = torch.zeros(M, dtype=torch.bool)
+        inside[before:before + sum(sizes)] = True
+        assert not bool(y.cpu()[~inside].any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(SHAPES)))
+def test_grouped_backward(case, dtype):
+    from weather_model_amd import ops
+    sizes, N, K, before, behind = SHAPES[case]
+    M, G = before + sum(sizes) + behind, len(sizes)
+    x, w, gy = rows(case + 7, (M, K), dtype), rows(case + 57, (G, N, K), dtype, K ** -0.5), rows(case + 97, (M, N), dtype)
+    off = offsets_of(sizes, before)
+    gx, gw, gb = ops.dense_grouped_backward(x.cuda(), w.cuda(), off, gy.cuda(), mask_below=x.cuda())
+    gx0, none, none2 = ops.dense_grouped_backward(x.cuda(), w.cuda(), off, gy.cuda(), need_gw=False)
+    assert none is None and none2 is None
+    rx, Sx = grouped_ref(gy, w.transpose(1, 2), None, sizes, before, False)
+    close(gx0, rx, Sx, N, (case, "gx"))
+    keep = (x > 0).double()
+    close(gx, rx * keep, Sx * keep, N, (case, "gx masked"))
+    at = before
+    for g, n in enumerate(sizes):
+        p = slice(at, at + n)
+        a, c = gy[p].double(), x[p].double()
+        close(gw[g], a.t() @ c, a.abs().t() @ c.abs(), n, (case, g, "gw"))
+        close(gb[g], a.sum(0), a.abs().sum(0), n, (case, g, "gb"), norm=False)
+        at += n
+
+
+def test_grouped_weight_gradient_split_over_rows():
+    """Few small weights and many rows: the rows are split over workgroups and joined in a fixed order."""
+    from weather_model_amd import _lib, ops
+    sizes, N, K = [9000, 0, 5001], 24, 70
+    assert _lib.lib().wm_dense_grouped_bwd_wb_workspace_bytes(3, sum(sizes), N, K) > 0
+    for dtype in TYPES:
+        x, gy = rows(1, (sum(sizes), K), dtype), rows(2, (sum(sizes), N), dtype)
+        w = torch.zeros((3, N, K), dtype=dtype, device="cuda")
+        off = offsets_of(sizes)
+        runs = [ops.dense_grouped_backward(x.cuda(), w, off, gy.cuda(), need_gx=False) for _ in range(2)]
+        assert torch.equal(runs[0][1], runs[1][1]) and torch.equal(runs[0][2], runs[1][2])
+        at = 0
+        for g, n in enumerate(sizes):
+            a, c = gy[at:at + n].double(), x[at:at + n].double()
+            close(runs[0][1][g], a.t() @ c, a.abs().t() @ c.abs(), n, g)
+            close(runs[0][2][g], a.sum(0), a.abs().sum(0), n, g, norm=False)
+            at += n
+
+
+def test_grouped_offsets_of_any_value_are_safe():
+    from weather_model_amd import ops
+    x, w = rows(1, (20, 8), torch.float32), rows(2, (4, 6, 8), torch.float32)
+    for off, sizes, before in (([-5, 3, 2, 99, 7], [3, 0, 17, 0], 0), ([4, 4, 1, 6, 6], [0, 0, 2, 0], 4),
+                               ([2 ** 40, 0, 0, 0, 0], [0, 0, 0, 0], 20)):
+        y = ops.dense_grouped_forward(x.cuda(), w.cuda(), torch.tensor(off, device="cuda"))
+        ref, S = grouped_ref(x, w, None, sizes, before, False)
+        close(y, ref, S, 8, off)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_infinities_and_nan_stay_in_their_rows(dtype):
+    """An infinity or a NaN in a row, in a weight, in a row of no expert, next to zeros; float32 values that round up
+    to infinity in bf16: the results are those of the arithmetic itself."""
+    from weather_model_amd import ops
+    inf, nan = float("inf"), float("nan")
+    x, w = rows(1, (70, 48), dtype), rows(2, (2, 40, 48), dtype, 48 ** -0.5)
+    x[3, 5], x[4, 6], x[5, 7], x[69, 0], x[8, :] = inf, -inf, nan, nan, 0
+    w[1, 2, 5] = inf
+    if dtype == torch.float32:
+        x[9, 1], w[0, 7, 1] = 3.4e38, 0.5
+    sizes = [30, 39]
+    gy = rows(3, (70, 40), dtype)
+    gy[6, 1], gy[69, 2] = inf, nan
+    y = ops.dense_grouped_forward(x.cuda(), w.cuda(), offsets_of(sizes))
+    gx, gw, gb = ops.dense_grouped_backward(x.cuda(), w.cuda(), offsets_of(sizes), gy.cuda())
+    xd, wd, gd = (t.double() for t in (x, w, gy))
+    ry = torch.cat([xd[:30] @ wd[0].t(), xd[30:69] @ wd[1].t(), torch.zeros(1, 40, dtype=torch.float64)])
+    rx = torch.cat([gd[:30] @ wd[0], gd[30:69] @ wd[1], torch.zeros(1, 48, dtype=torch.float64)])
+    rw = torch.stack([gd[:30].t() @ xd[:30], gd[30:69].t() @ xd[30:69]])
+    rb = torch.stack([gd[:30].sum(0), gd[30:69].sum(0)])
+    for name, got, ref in (("y", y, ry), ("gx", gx, rx), ("gw", gw, rw), ("gb", gb, rb)):
+        got = got.cpu().double()
+        ref = torch.where(ref.abs() > torch.finfo(dtype).max, ref.sign() * inf, ref)
+        assert torch.equal(got.isnan(), ref.isnan()), name
+        assert torch.equal(got.isposinf(), ref.isposinf()) and torch.equal(got.isneginf(), ref.isneginf()), name
+        fine = ref.isfinite()
+        scale = 1.0 if float(ref[fine].abs().max()) < 1e6 else float(ref[fine].abs().max())
+        assert float((got - ref)[fine].abs().max()) <= (half_step(dtype) * 32 + 64 * U) * scale, name
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** 60, 2.0 ** -120])
+def test_grouped_float32_at_far_scales(scale):
+    """The split keeps float32 accuracy from far below to far above 1 (2^-120: the third piece is subnormal in bf16,
+    2^-133 is its last step: absolute error 2^-134 of each factor)."""
+    from weather_model_amd import ops
+    x, w = rows(1, (40, 64), torch.float32), rows(2, (1, 24, 64), torch.float32, 0.125)
+    y = ops.dense_grouped_forward((x * scale).cuda(), w.cuda(), offsets_of([40]))
+    ref, S = grouped_ref(x.double() * scale, w, None, [40], 0, False)
+    d = (y.cpu().double() - ref).abs()
+    assert bool((d <= (5 * 112 ** 0.5 * U + 3 * 2.0 ** -26) * S + 64 * 2.0 ** -133).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_takes_views_streams_and_unaligned_storage(dtype):
+    """Strided views, storage that begins at an odd element, a side stream."""
+    from weather_model_amd import ops
+    sizes, N, K = [70, 60], 50, 33
+    x, w, b = rows(1, (130, K), dtype), rows(2, (2, N, K), dtype, 0.2), rows(3, (2, N), dtype)
+    ref, S = grouped_ref(x, w, b, sizes, 0, False)
+    wide = torch.zeros((130, 2 * K), dtype=dtype)
+    wide[:, ::2] = x
+    flat = torch.zeros((x.numel() + 1,), dtype=dtype, device="cuda")
+    flat[1:] = x.cuda().reshape(-1)
+    wflat = torch.zeros((w.numel() + 1,), dtype=dtype, device="cuda")
+    wflat[1:] = w.cuda().reshape(-1)
+    wv = wflat[1:].view(w.shape)
+    off = offsets_of(sizes)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ys = ops.dense_grouped_forward(x.cuda(), w.cuda().transpose(1, 2).contiguous().transpose(1, 2), off, b.cuda())
+    torch.cuda.current_stream().wait_stream(side)
+    for y in (ys, ops.dense_grouped_forward(wide.cuda()[:, ::2], wv, off, b.cuda()),
+              ops.dense_grouped_forward(flat[1:].view(130, K), wv, off, b.cuda())):
+        close(y, ref, S, K, dtype)
+    gy = rows(4, (130, N), dtype)
+    gflat = torch.zeros((gy.numel() + 1,), dtype=dtype, device="cuda")
+    gflat[1:] = gy.cuda().reshape(-1)
+    got = ops.dense_grouped_backward(flat[1:].view(130, K), wv, off, gflat[1:].view(130, N))
+    want = ops.dense_grouped_backward(x.cuda(), w.cuda(), off, gy.cuda())
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)
+
+
+def test_grouped_autograd_against_differences():
+    """Gradients of a scalar of y against central differences of the float64 formula (step 1e-4: its own
+    error is 1e-8 of the third derivative, zero for these products, plus 1e-12)."""
+    from weather_model_amd import ops
+    sizes, N, K = [4, 0, 9], 6, 5
+    x, w, b, c = rows(1, (13, K), torch.float32), rows(2, (3, N, K), torch.float32), rows(3, (3, N), torch.float32), rows(4, (13, N), torch.float32)
+    leaves = [t.clone().cuda().requires_grad_() for t in (x, w, b)]
+    y = ops.dense_grouped(leaves[0], leaves[1], offsets_of(sizes), leaves[2], relu=True)
+    (y * c.cuda()).sum().backward()
+
+    def loss(xd, wd, bd):
+        return float((grouped_ref(xd, wd, bd, sizes, 0, True)[0] * c.double()).sum())
+    base = [t.double() for t in (x, w, b)]
+    gen = torch.Generator().manual_seed(9)
+    for k, leaf in enumerate(leaves):
+        for _ in range(12):
+            e = torch.zeros(base[k].numel(), dtype=torch.float64)
+            at = int(torch.randint(base[k].numel(), (1,), generator=gen))
+            e[at] = 1e-4
+            d = (loss(*[t + e.view(t.shape) if j == k else t for j, t in enumerate(base)])
+                 - loss(*[t - e.view(t.shape) if j == k else t for j, t in enumerate(base)])) / 2e-4
+            assert abs(float(leaf.grad.reshape(-1)[at]) - d) <= 1e-5 * max(1.0, abs(d)), (k, at)
+
+
+# ------------------------------------------------------------------ dropout
+
+def kept(n, p, seed, offset):
+    """The documented draw in numpy: 16 bits of the hash of (seed, e / 4) above 16 of the hash of that."""
+    e = np.arange(n, dtype=np.uint64) + np.uint64(offset)
+    z = synth.hash64(seed, e >> np.uint64(2))
+    at = (e & np.uint64(3)) * np.uint64(16)
+    u = ((z >> at) & np.uint64(0xFFFF)) << np.uint64(16) | ((synth.hash64(seed, z) >> at) & np.uint64(0xFFFF))
+    return torch.from_numpy(u >= np.uint64(round(p * 2 ** 32)))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,p,offset", [(1, 0.5, 0), (7, 0.3, 0), (4099, 0.1, 0), (4099, 0.1, 1), (100003, 0.9, 2), (65536, 0.5, 3),
+                                        (262145, 2.0 ** -16, 8), (262144, 1e-9, 5), (50000, 1.0, 0), (50001, 0.0, 0),
+                                        (30000, 0.25, 2 ** 33 + 5), (30000, 0.25, 2 ** 62 + 6)])
+def test_dropout_matches_the_documented_draw(n, p, offset, dtype):
+    from weather_model_amd import ops
+    x, r = rows(n, (n,), dtype), rows(n + 1, (n,), dtype)
+    keep = kept(n, p, 77, offset)
+    scale = 0.0 if p == 1.0 else 1.0 / (1.0 - round(p * 2 ** 32) / 2 ** 32)
+    ref = torch.where(keep, x.double() * scale, 0.0)
+    for res in (None, r):
+        y = ops.dropout_forward(x.cuda(), p, 77, offset=offset, residual=None if res is None else res.cuda()).cpu()
+        want = ref if res is None else ref + res.double()
+        # the scale and the product are rounded in float32 (2 u), the sum (u), the result to its type
+        tol = 4 * U * (ref.abs() + (0 if res is None else res.double().abs())) + half_step(dtype) * want.abs() + torch.finfo(dtype).tiny
+        assert bool(((y.double() - want).abs() <= tol).all())
+        if res is None:
+            assert torch.equal(y == 0, (~keep) | (x == 0)) or dtype == torch.float16
+    dev = ops.dropout_forward(x.cuda(), p, 77, offset=torch.tensor([offset], device="cuda")).cpu()
+    assert torch.equal(dev, ops.dropout_forward(x.cuda(), p, 77, offset=offset).cpu())
+    g = ops.dropout_backward(r.cuda(), p, 77, offset=offset).cpu()
+    assert torch.equal(g == 0, (~keep) | (r == 0)) or dtype == torch.float16
+
+
+def test_dropout_drops_infinities_works_in_place_and_in_pieces():
+    from weather_model_amd import ops
+    n, p = 10007, 0.4
+    x = torch.full((n,), float("nan"), device="cuda")
+    keep = kept(n, p, 5, 0)
+    y = ops.dropout_forward(x, p, 5).cpu()
+    assert torch.equal(y.isnan(), keep) and not bool(y[~keep].any())
+    z = rows(1, (n,), torch.bfloat16).cuda()
+    whole = ops.dropout_forward(z, p, 5, offset=11)
+    parts = torch.cat([ops.dropout_forward(z[a:b], p, 5, offset=11 + a) for a, b in ((0, 1), (1, 4098), (4098, n))])
+    assert torch.equal(whole, parts)
+    ops.dropout_forward(z, p, 5, offset=11, out=z)
+    assert torch.equal(z, whole)
+    share = float(kept(1 << 20, 0.1, 3, 0).double().mean())
+    assert abs(share - 0.9) < 5 * (0.09 / 2 ** 20) ** 0.5
+
+
+def test_dropout_autograd_and_graph_replays_with_a_device_offset():
+    from weather_model_amd import ops
+    x, r = rows(1, (64, 130), torch.float32).cuda().requires_grad_(), rows(2, (64, 130), torch.float32).cuda().requires_grad_()
+    gy = rows(3, (64, 130), torch.float32).cuda()
+    ops.dropout(x, 0.3, 9, 40, residual=r).backward(gy)
+    assert torch.equal(r.grad, gy)
+    assert torch.equal(x.grad, ops.dropout_backward(gy, 0.3, 9, 40))
+    counter = torch.zeros((1,), dtype=torch.int64, device="cuda")
+    src, dst = rows(4, (5001,), torch.float32).cuda(), torch.empty((5001,), device="cuda")
+    ops.dropout_forward(src, 0.5, 2, offset=counter, out=dst)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.dropout_forward(src, 0.5, 2, offset=counter, out=dst)
+        counter.add_(5001)
+    for k in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dst, ops.dropout_forward(src, 0.5, 2, offset=5001 * k)), k
+    lost = ops.dropout(x, 0.3, 9, counter)
+    counter.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lost.sum().backward()
+
+
+# ------------------------------------------------------------------ 8 bits
+
+def codes_ref(x):
+    """(codes float64, scale float64) by the definition: float32 scale, float32 quotient rounded to even"""
+    top = x.double().abs().amax(1)
+    scale = (top / 127).float().double()
+    q = (x.double() / torch.where(scale > 0, scale, 1.0)[:, None]).float().double().round().clamp(-127, 127)
+    return q * (scale > 0)[:, None], scale
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 7), (5, 16), (2, 640), (33, 1283), (4, 8192), (1, 20011), (70, 63)])
+def test_quantize_rows(M, K, dtype):
+    from weather_model_amd import ops
+    x = rows(M + K, (M, K), dtype) * torch.logspace(-3, 2, M)[:, None].to(dtype)
+    if M > 2:
+        x[1] = 0
+        x[2, K // 2:] = -x[2].abs().max()
+    q, s = ops.quantize_rows(x.cuda())
+    rq, rs = codes_ref(x)
+    assert torch.equal(s.cpu().double(), rs)
+    assert torch.equal(q.cpu().double(), rq)
+
+
+def test_quantize_ties_extremes_and_bad_rows():
+    from weather_model_amd import ops
+    x = torch.zeros((6, 130))
+    x[0, 0], x[0, 1:7] = 127.0, torch.tensor([0.5, 1.5, 2.5, -0.5, -1.5, 126.5])          # ties go to even
+    x[1, 0], x[1, 1] = 1e-45, 3e-45                                                       # the scale underflows to zero
+    x[2, 5], x[2, 6] = 2.6e-43, -1.4e-45                                                  # a subnormal scale
+    x[3, 9], x[4, 129], x[5, 3] = float("inf"), float("nan"), 3e38
+    q, s = ops.quantize_rows(x.cuda())
+    q, s = q.cpu(), s.cpu()
+    assert q[0, :7].tolist() == [127, 0, 2, 2, 0, -2, 126]
+    rq, rs = codes_ref(x[[0, 1, 2, 5]])
+    assert torch.equal(q[[0, 1, 2, 5]].double(), rq) and torch.equal(s[[0, 1, 2, 5]].double(), rs)
+    assert bool(s[3:5].isnan().all()) and not bool(q[3:5].any())
+    w, t = ops.quantize_rows(rows(3, (40, 130), torch.float32).cuda())
+    y = ops.dense_i8(x.cuda(), w, t).cpu()
+    assert bool(y[3:5].isnan().all()) and not bool(y[:3].isnan().any()) and not bool(y[5].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8000, 640), (3, 37, 19), (16, 64, 128), (17, 130, 257), (128, 128, 64), (200, 301, 515),
+                                   (130, 260, 2049), (48, 129, 33), (300, 50, 127)])
+def test_dense_i8(M, N, K, dtype):
+    from weather_model_amd import ops
+    x, b = rows(M, (M, K), dtype), rows(N, (N,), torch.float32)
+    q, t = ops.quantize_rows(rows(K, (N, K), torch.float32, K ** -0.5).cuda())
+    xq, xs = codes_ref(x)
+    exact = (xq @ q.cpu().double().t()) * xs[:, None] * t.cpu().double()
+    for bias, relu in ((None, False), (b, True)):
+        y = ops.dense_i8(x.cuda(), q, t, None if bias is None else bias.cuda(), relu=relu).cpu()
+        ref = exact if bias is None else exact + bias.double()
+        ref = ref.clamp(min=0) if relu else ref
+        # the integer, two scalings and the sum are rounded once each in float32
+        tol = 4 * U * (exact.abs() + (0 if bias is None else bias.double().abs())) + half_step(dtype) * ref.abs() + torch.finfo(dtype).tiny
+        assert bool(((y.double() - ref).abs() <= tol * (1 + 2.0 ** -8)).all())
+
+
+def test_dense_i8_grouped_extreme_codes_and_unaligned_weights():
+    from weather_model_amd import ops
+    sizes, N, K = [0, 50, 1, 0, 140], 45, 203
+    M = sum(sizes) + 4
+    x, b = rows(1, (M, K), torch.bfloat16), rows(2, (5, N), torch.float32)
+    flat = torch.randint(-128, 128, (5 * N * K + 1,), generator=torch.Generator().manual_seed(3)).to(torch.int8).cuda()
+    q = flat[1:].view(5, N, K)                                # storage begins at an odd byte; -128 among the codes
+    t = rows(4, (5, N), torch.float32).abs().cuda()
+    y = ops.dense_i8(x.cuda(), q, t, b.cuda(), offsets=offsets_of(sizes)).cpu().double()
+    xq, xs = codes_ref(x)
+    at = 0
+    for g, n in enumerate(sizes):
+        p = slice(at, at + n)
+        e = (xq[p] @ q[g].cpu().double().t()) * xs[p][:, None] * t[g].cpu().double()
+        ref = e + b[g].double()
+        assert bool(((y[p] - ref).abs() <= 4 * U * (e.abs() + b[g].double().abs()) + 2.0 ** -8 * ref.abs()).all()), g
+        at += n
+    assert not bool(y[at:].any())
+    # every product at its largest, over the longest sum that is allowed
+    K = 1 << 17
+    big = torch.full((2, K), -128, dtype=torch.int8, device="cuda")
+    y = ops.dense_i8(torch.ones((1, K), device="cuda"), big, torch.ones((2,), device="cuda"))
+    assert torch.equal(y.cpu(), torch.full((1, 2), float(np.float32(-127.0 * 128 * K) * (np.float32(1) / np.float32(127)))))
+
+
+# ------------------------------------------------------------------ together
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_expert_stack_trains_and_serves(dtype):
+    """Three layers of four experts with dropout: activations and all gradients against the same chain in float64 on
+    the layer's own inputs, a graph of the step replayed, then served in 8 bits within the codes' resolution."""
+    from weather_model_amd.experts import ExpertStack
+    sizes, widths, p = [40, 0, 133, 20], [20, 48, 33, 10], 0.25
+    M, G = sum(sizes) + 3, len(sizes)
+    x = rows(1, (M, widths[0]), dtype)
+    ws = [rows(10 + l, (G, n, k), dtype, k ** -0.5) for l, (k, n) in enumerate(zip(widths, widths[1:]))]
+    bs = [rows(20 + l, (G, n), dtype, 0.1) for l, n in enumerate(widths[1:])]
+    gout = rows(30, (M, widths[-1]), dtype)
+    off = offsets_of(sizes)
+    st = ExpertStack([w.cuda() for w in ws], [b.cuda() for b in bs], p=p, seed=4)
+    st.forward(x.cuda(), off, train=True)
+    flat = st.backward(gout.cuda()).clone()
+    h = [t.cpu() for t in st.h]
+    scale = 1.0 / (1.0 - p)
+    masks, drawn = [], 0
+    for l in range(3):
+        ref, S = grouped_ref(h[l], ws[l], bs[l], sizes, 0, l < 2)
+        if l < 2:
+            keep = kept(ref.numel(), p, 4, drawn).view(ref.shape)
+            drawn += ref.numel()
+            ref, S = torch.where(keep, ref * scale, 0.0), S * scale
+            masks.append((h[l + 1] > 0).double() * scale)
+            # two roundings to the type: the product's and dropout's
+            d = (h[l + 1].double() - ref).abs()
+            assert bool((d <= 2.1 * half_step(dtype) * ref.abs() + 6 * 100 ** 0.5 * U * S + torch.finfo(dtype).tiny).all()), l
+            assert not bool(h[l + 1][~keep].any())
+        else:
+            close(st.h[3], ref, S, widths[l], l)
+    # the chain of gradients rounds to the type at every layer: at most (2 per layer) half steps of |.| propagated
+    g, err = gout.double(), torch.zeros_like(gout, dtype=torch.float64)
+    for l in range(2, -1, -1):
+        at = 0
+        ng, nerr = torch.zeros_like(h[l], dtype=torch.float64), torch.zeros_like(h[l], dtype=torch.float64)
+        for e, n in enumerate(sizes):
+            q = slice(at, at + n)
+            a, c, w = g[q], h[l][q].double(), ws[l][e].double()
+            u = 6 * (1.5 * max(n, widths[l + 1]) + 16) ** 0.5 * U
+            tol = err[q].t() @ c.abs() + (a.abs() + err[q]).t() @ c.abs() * u + half_step(dtype) * (a.t() @ c).abs()
+            assert bool(((st.gw[l][e].cpu().double() - a.t() @ c).abs() <= 1.01 * tol + torch.finfo(dtype).tiny).all()), (l, e)
+            tol = err[q].sum(0) + a.abs().sum(0) * u + half_step(dtype) * a.sum(0).abs()
+            assert bool(((st.gb[l][e].cpu().double() - a.sum(0)).abs() <= 1.01 * tol + torch.finfo(dtype).tiny).all()), (l, e)
+            if l:
+                ng[q] = a @ w * masks[l - 1][q]
+                nerr[q] = (err[q] @ w.abs() + u * (a.abs() @ w.abs())) * masks[l - 1][q] + 2.1 * half_step(dtype) * ng[q].abs()
+            at += n
+        g, err = ng, 1.01 * nerr
+    # the same step captured and replayed: same draws from the same counter
+    st.drawn = 0
+    sx, sg = x.cuda(), gout.cuda()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        st.step_grads(sx, off, sg)
+    for _ in range(3):
+        st.flat_grads.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(st.flat_grads, flat)
+    # served: every code is within half a step of its value
+    y8 = st.quantize().predict(x.cuda(), off).cpu().double()
+    a, err = x.double(), torch.zeros_like(x, dtype=torch.float64)
+    for l in range(3):
+        z, S = grouped_ref(a, ws[l], bs[l], sizes, 0, False)
+        z8, e8 = torch.zeros_like(z), torch.zeros_like(z)
+        at = 0
+        for e, n in enumerate(sizes):
+            q = slice(at, at + n)
+            dx = err[q] + (a[q].abs() + err[q]).amax(1, keepdim=True) / 254 * 1.001
+            dw = ws[l][e].double().abs().amax(1, keepdim=True) / 254 * 1.001
+            w = ws[l][e].double().abs()
+            e8[q] = dx @ (w + dw).t() + a[q].abs() @ dw.expand_as(w).t()
+            at += n
+        z = z.clamp(min=0) if l < 2 else z
+        e8 = e8 + half_step(dtype) * (z.abs() + e8) + 8 * U * (S + e8) + torch.finfo(dtype).tiny
+        a, err = z, e8
+    assert bool(((y8 - a).abs() <= 1.01 * err).all())
+    assert float((y8 - a).norm() / a.norm()) < 0.05

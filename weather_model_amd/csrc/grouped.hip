@@ -1,0 +1,310 @@
+// grouped.hip -- Dense layers of several experts at once: rows sorted by expert, expert g owning rows
+// offsets[g] .. offsets[g+1] - 1 of x (M, K) and its own weights W[g] (N, K) and bias b[g] (N).
+//   forward   y[r][n]     = act(b[g][n] + sum_k x[r][k] W[g][n][k])
+//   backward  gx[r][k]    = mask(sum_n gy[r][n] W[g][n][k])
+//             gW[g][n][k] = sum_{r of g} gy[r][n] x[r][k],   gb[g][n] = sum_{r of g} gy[r][n]
+// The number of rows of an expert is only known on the device, so a launch has as many workgroups as any
+// partition of M rows can need tiles, and each finds its tile from the offsets (tile_gemm.h).
+#include "tile_gemm.h"
+
+namespace {
+
+using namespace tile;
+
+template <class T> __device__ __forceinline__ f32x4 load4_f32(const T *p)
+{
+    return __builtin_convertvector(*reinterpret_cast<const typename Vec4<T>::type *>(p), f32x4);
+}
+
+// ---- rows: out (M, NO) = x (M, C) times W[g], forward (W[g] is (NO, C), its c along memory) or backward
+// (W[g] is (C, NO)).  bias and relu are the forward's, mask the backward's.
+template <class T, int BM, int BN, bool BACKWARD>
+__global__ __launch_bounds__(THREADS) void grouped_rows_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
+                                                               const typename T::elem *__restrict__ bias,
+                                                               const typename T::elem *__restrict__ mask,
+                                                               typename T::elem *__restrict__ out, const long long *__restrict__ offsets,
+                                                               int G, int M, int NO, int C, int relu, int band)
+{
+    typedef typename T::elem E;
+    __shared__ __attribute__((aligned(16))) char lds[lds_bytes_one<T, BM, BN>()];
+    int rt, ct;
+    if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (NO + BN - 1) / BN, band, rt, ct)) return;
+    const Segment s = row_tile(offsets, G, M, BM, rt);
+    const int n0 = ct * BN, cols = min(BN, NO - n0);
+    if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
+        for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) out[(long long)(s.row0 + e / cols) * NO + n0 + e % cols] = (E)0.0f;
+        return;
+    }
+    const E *wg = W + (long long)s.g * NO * C;
+    const E *xr = x + (long long)s.row0 * C;
+    typedef typename std::conditional<BACKWARD, Strided<T, BN>, Contiguous<T, BN>>::type LA;
+    LA a;
+    Contiguous<T, BM> b;
+    const E *wt = BACKWARD ? wg + n0 : wg + (long long)n0 * C;
+    a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
+    b.init(xr, C, s.rows, C, x + (long long)M * C);
+    constexpr int MI = BM / 32, NI = BN / 32;
+    typename T::acc acc[MI][NI];
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) acc[m][n] = typename T::acc{0, 0, 0, 0};
+    product<T, BM, BN>(a, b, C, lds, acc);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int ni0 = (wave & 1) * (BN / 2) + 4 * (lane >> 4), mi0 = (wave >> 1) * (BM / 2) + (lane & 15);
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+        const int r = mi0 + 16 * m;
+        if (r >= s.rows) continue;
+        const long long row = (long long)(s.row0 + r) * NO + n0;
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int i = ni0 + 16 * n;
+            if (i >= cols) continue;
+            const int have = min(4, cols - i);
+            f32x4 v = acc[m][n];
+            if constexpr (T::PLANES == 3) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (v[k] != v[k] && k < have)
+                        v[k] = BACKWARD ? dot_again(wt + i + k, NO, xr + (long long)r * C, 1, C)
+                                        : dot_again(wt + (long long)(i + k) * C, 1, xr + (long long)r * C, 1, C);
+            }
+            if (have == 4) {
+                if (!BACKWARD && bias) v += load4_f32(bias + (long long)s.g * NO + n0 + i);
+                if (!BACKWARD && relu) v = (f32x4){relu_of(v[0]), relu_of(v[1]), relu_of(v[2]), relu_of(v[3])};
+                if (BACKWARD && mask) {
+                    const f32x4 k = load4_f32(mask + row + i);
+                    v = (f32x4){k[0] > 0 ? v[0] : 0, k[1] > 0 ? v[1] : 0, k[2] > 0 ? v[2] : 0, k[3] > 0 ? v[3] : 0};
+                }
+                store4(out + row + i, v);
+            } else {
+                for (int k = 0; k < have; ++k) {
+                    float o = v[k];
+                    if (!BACKWARD && bias) o += to_float(bias[(long long)s.g * NO + n0 + i + k]);
+                    if (!BACKWARD && relu) o = relu_of(o);
+                    if (BACKWARD && mask) o = to_float(mask[row + i + k]) > 0 ? o : 0.0f;
+                    out[row + i + k] = from_float<E>(o);
+                }
+            }
+        }
+    }
+}
+
+// ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
+// with S > 1 the shares go to `partial` (S, G, N, K) and grouped_weights_sum_kernel adds them in order.
+template <class T, int BM, int BN>
+__global__ __launch_bounds__(THREADS) void grouped_weights_kernel(const typename T::elem *__restrict__ gy, const typename T::elem *__restrict__ x,
+                                                                  typename T::elem *__restrict__ gW, float *__restrict__ partial,
+                                                                  const long long *__restrict__ offsets, int G, int M, int N, int K, int S)
+{
+    typedef typename T::elem E;
+    __shared__ __attribute__((aligned(16))) char lds[lds_bytes_one<T, BM, BN>()];
+    // i (contiguous in the output) is k, j is n
+    const int kt = (K + BN - 1) / BN, nt = (N + BM - 1) / BM;
+    int id = blockIdx.x;
+    const int k0 = id % kt * BN;
+    id /= kt;
+    const int n0 = id % nt * BM;
+    id /= nt;
+    const int g = id % G, split = id / G;
+    int row0, rows;
+    group_rows(offsets, G, M, g, row0, rows);
+    constexpr int STEP = T::BKC * 8;
+    const int share = ((rows + S - 1) / S + STEP - 1) / STEP * STEP;
+    row0 += min(rows, split * share);
+    rows = min(share, max(0, rows - split * share));
+    constexpr int MI = BM / 32, NI = BN / 32;
+    typename T::acc acc[MI][NI];
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < NI; ++n) acc[m][n] = typename T::acc{0, 0, 0, 0};
+    const int ks = min(BN, K - k0), ns = min(BM, N - n0);
+    const E *xt = x + (long long)row0 * K + k0, *yt = gy + (long long)row0 * N + n0;
+    if (rows > 0) {
+        Strided<T, BN> a;
+        Strided<T, BM> b;
+        a.init(xt, K, ks, rows, x + (long long)M * K);
+        b.init(yt, N, ns, rows, gy + (long long)M * N);
+        product<T, BM, BN>(a, b, rows, lds, acc);
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int ni0 = (wave & 1) * (BN / 2) + 4 * (lane >> 4), mi0 = (wave >> 1) * (BM / 2) + (lane & 15);
+    const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
+#pragma unroll
+    for (int m = 0; m < MI; ++m) {
+        const int j = mi0 + 16 * m;
+        if (j >= ns) continue;
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int i = ni0 + 16 * n;
+            if (i >= ks) continue;
+            const int have = min(4, ks - i);
+            f32x4 v = acc[m][n];
+            if constexpr (T::PLANES == 3) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (v[k] != v[k] && k < have) v[k] = dot_again(xt + i + k, K, yt + j, N, rows);
+            }
+            const long long e = at + (long long)j * K + i;
+            if (partial) {
+                if (have == 4) store4(partial + e, v);
+                else
+                    for (int k = 0; k < have; ++k) partial[e + k] = v[k];
+            } else {
+                if (have == 4) store4(gW + e, v);
+                else
+                    for (int k = 0; k < have; ++k) gW[e + k] = from_float<E>(v[k]);
+            }
+        }
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const float *__restrict__ partial, E *__restrict__ gW, long long count, int S)
+{
+    for (long long e = (long long)blockIdx.x * THREADS + threadIdx.x; e < count; e += (long long)gridDim.x * THREADS) {
+        float s = partial[e];
+        for (int p = 1; p < S; ++p) s += partial[p * count + e];
+        gW[e] = from_float<E>(s);
+    }
+}
+
+// ---- bias: gb[g][n], a workgroup per 64 columns of an expert; four waves take every fourth row
+template <class E>
+__global__ __launch_bounds__(THREADS) void grouped_bias_kernel(const E *__restrict__ gy, E *__restrict__ gb, const long long *__restrict__ offsets,
+                                                               int G, int M, int N)
+{
+    __shared__ float part[4][64];
+    const int g = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
+    int row0, rows;
+    group_rows(offsets, G, M, g, row0, rows);
+    float s = 0.0f;
+    if (n < N)
+        for (int r = wave; r < rows; r += 4) s += to_float(gy[(long long)(row0 + r) * N + n]);
+    part[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && n < N) gb[(long long)g * N + n] = from_float<E>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+}
+
+int check(const char *who, int M, int N, int K, int G, int dtype)
+{
+    WM_REQUIRE(M >= 0 && N > 0 && K > 0 && G > 0, WM_ERR_INVALID, "%s: bad sizes M=%d N=%d K=%d groups=%d", who, M, N, K, G);
+    WM_REQUIRE(N <= 1 << 20 && K <= 1 << 20 && G <= 1 << 16 && M <= 1 << 30, WM_ERR_UNSUPPORTED,
+               "%s: M=%d N=%d K=%d groups=%d is beyond 2^30 rows, 2^20 columns or 2^16 groups", who, M, N, K, G);
+    WM_REQUIRE(dtype == WM_F32 || dtype == WM_BF16 || dtype == WM_F16, WM_ERR_INVALID, "%s: bad dtype %d", who, dtype);
+    WM_REQUIRE(wm_num_cus() > 0, WM_ERR_NO_DEVICE, "%s: no HIP device", who);
+    return WM_OK;
+}
+
+int blocks_ok(const char *who, long long blocks)
+{
+    WM_REQUIRE(blocks <= (1ll << 32) / THREADS - 1, WM_ERR_UNSUPPORTED, "%s: %lld tiles are too many for one launch", who, blocks);
+    return WM_OK;
+}
+
+template <class T, int BM, int BN, bool BACKWARD>
+int rows_launch(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
+                int C, int relu, hipStream_t st)
+{
+    typedef typename T::elem E;
+    const long long blocks = row_tiles_most(G, M, BM) * ((NO + BN - 1) / BN);
+    if (int rc = blocks_ok("wm_dense_grouped", blocks)) return rc;
+    hipLaunchKernelGGL((grouped_rows_kernel<T, BM, BN, BACKWARD>), dim3((unsigned)blocks), dim3(THREADS), 0, st, (const E *)x, (const E *)W,
+                       (const E *)bias, (const E *)mask, (E *)out, (const long long *)offsets, G, M, NO, C, relu, 8);
+    WM_LAUNCH_CHECK("grouped_rows_kernel");
+    return WM_OK;
+}
+
+template <bool BACKWARD>
+int rows_any(int dtype, const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
+             int C, int relu, hipStream_t st)
+{
+    switch (dtype) {
+    case WM_F32: return rows_launch<F32, 128, 128, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    case WM_BF16: return rows_launch<BF16, 128, 128, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    default: return rows_launch<F16, 128, 128, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    }
+}
+
+constexpr int WB_TILE = 128;
+
+int weight_splits(int M, int N, int K, int G)
+{
+    // enough workgroups for two rounds of 256 CUs, at least 256 rows of an average expert each
+    const long long tiles = (long long)G * ((N + WB_TILE - 1) / WB_TILE) * ((K + WB_TILE - 1) / WB_TILE);
+    const long long want = (512 + tiles - 1) / tiles, most = M / ((long long)G * 256);
+    const long long s = want < most ? want : most;
+    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+}
+
+template <class T>
+int weights_launch(const void *x, const void *gy, void *gW, void *gb, void *workspace, const int64_t *offsets, int G, int M, int N, int K,
+                   hipStream_t st)
+{
+    typedef typename T::elem E;
+    const int S = weight_splits(M, N, K, G);
+    const long long blocks = (long long)S * G * ((N + WB_TILE - 1) / WB_TILE) * ((K + WB_TILE - 1) / WB_TILE);
+    if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
+    hipLaunchKernelGGL((grouped_weights_kernel<T, WB_TILE, WB_TILE>), dim3((unsigned)blocks), dim3(THREADS), 0, st, (const E *)gy, (const E *)x,
+                       (E *)gW, S > 1 ? (float *)workspace : nullptr, (const long long *)offsets, G, M, N, K, S);
+    WM_LAUNCH_CHECK("grouped_weights_kernel");
+    if (S > 1) {
+        const long long count = (long long)G * N * K;
+        long long grid = (count + THREADS - 1) / THREADS;
+        if (grid > 4096) grid = 4096;
+        hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid), dim3(THREADS), 0, st, (const float *)workspace, (E *)gW, count, S);
+        WM_LAUNCH_CHECK("grouped_weights_sum_kernel");
+    }
+    if (gb) {
+        hipLaunchKernelGGL(grouped_bias_kernel<E>, dim3((N + 63) / 64, G), dim3(THREADS), 0, st, (const E *)gy, (E *)gb,
+                           (const long long *)offsets, G, M, N);
+        WM_LAUNCH_CHECK("grouped_bias_kernel");
+    }
+    return WM_OK;
+}
+
+}  // namespace
+
+extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
+                                    int dtype, int relu, void *stream)
+{
+    if (int rc = check("wm_dense_grouped_fwd", M, N, K, G, dtype)) return rc;
+    if (M == 0) return WM_OK;
+    WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
+    return rows_any<false>(dtype, x, W, b, nullptr, y, offsets, G, M, N, K, relu, (hipStream_t)stream);
+}
+
+extern "C" int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx, const int64_t *offsets, int G, int M,
+                                         int N, int K, int dtype, void *stream)
+{
+    if (int rc = check("wm_dense_grouped_bwd_data", M, N, K, G, dtype)) return rc;
+    if (M == 0) return WM_OK;
+    WM_REQUIRE(gy && W && gx && offsets, WM_ERR_INVALID, "wm_dense_grouped_bwd_data: null pointer");
+    return rows_any<true>(dtype, gy, W, nullptr, mask_below, gx, offsets, G, M, K, N, 0, (hipStream_t)stream);
+}
+
+extern "C" size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K)
+{
+    if (M < 0 || N <= 0 || K <= 0 || G <= 0) return 0;
+    const int S = weight_splits(M, N, K, G);
+    return S > 1 ? wm_align_up((size_t)S * G * N * K * sizeof(float), 256) : 0;
+}
+
+extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, void *workspace, size_t workspace_bytes,
+                                       const int64_t *offsets, int G, int M, int N, int K, int dtype, void *stream)
+{
+    if (int rc = check("wm_dense_grouped_bwd_wb", M, N, K, G, dtype)) return rc;
+    WM_REQUIRE((x && gy || M == 0) && gW && offsets, WM_ERR_INVALID, "wm_dense_grouped_bwd_wb: null pointer");
+    const size_t need = wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K);
+    WM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), WM_ERR_WORKSPACE,
+               "wm_dense_grouped_bwd_wb: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+    case WM_F32: return weights_launch<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    case WM_BF16: return weights_launch<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    default: return weights_launch<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    }
+}

@@ -2,18 +2,11 @@
 // The reference reads WRF NetCDF files (multipleRegression.py:167-187); the benchmark shapes of
 // BASELINE.json are synthetic, and config 5 (2.56 TB) only exists as a generator.
 #include "common.h"
+#include "hash64.h"
 
 namespace {
 
 constexpr int BLOCK = 256;
-
-__device__ __forceinline__ uint64_t hash64(uint64_t seed, uint64_t idx)
-{
-    uint64_t z = idx + ((seed + 1) & 0xFFFFFFFFull) * 0x9E3779B97F4A7C15ull;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    return z ^ (z >> 31);
-}
 
 __device__ __forceinline__ float u01(uint64_t z) { return (float)(z >> 40) * 0x1.0p-24f; }
 

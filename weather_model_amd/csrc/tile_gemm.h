@@ -1,0 +1,430 @@
+// tile_gemm.h -- the tiled matrix product under the grouped Dense layers (grouped.hip) and the 8-bit
+// integer product (int8.hip): operand loaders, the LDS layout, the MFMA core and the map from a
+// workgroup to its tile of a ragged batch.
+//
+// A tile is C[i][j] = sum_c A[i][c] B[j][c], BN values of i (the output's contiguous side) by BM of j (its
+// rows).  D of an MFMA has four consecutive i of one j in a lane, which makes a store one vector.
+// LDS holds both operands as [row][c], `BKC` chunks of 16 bytes a row, whatever their layout in memory:
+//   contiguous  c runs along memory: a chunk is one 16-byte load (two for float32)
+//   strided     i (or j) runs along memory: a thread loads 8 c of a few rows and transposes in registers
+// and the chunk at position q of row r lies in slot q ^ swz(r), so that the 16 rows of an MFMA operand, the
+// 8 rows a loader's wave writes, and the 8-row steps of a transposed write all spread over the banks.
+//
+// float32 is split into three bf16 pieces, x = h + m + l (each the nearest to what is left: 24 bits), and a
+// product is the six piece products that are not below 2^-24 of it: hh, hm, mh, hl, lh, mm, each exact in the
+// float32 accumulator.  That is float32 accuracy (what is left out is 3 2^-26 of |a||b| at most) at 2500 / 6
+// TFLOP/s of matrix rate where the float32 MFMA has 157.  An infinity, a NaN or a value that rounds up to
+// infinity in bf16 makes a NaN of its products; such elements of C are then summed again in float32 (dot_again).
+#pragma once
+
+#include <type_traits>
+
+#include "half_types.h"
+
+namespace tile {
+
+constexpr int THREADS = 256;                 // four waves, 2 x 2 over the tile
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(1)));
+typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
+typedef f32x4 f32x4b __attribute__((aligned(16)));
+
+// ---- element types
+struct BF16 {
+    typedef bf16_t elem;
+    typedef f32x4 acc;
+    static constexpr int PLANES = 1, BKC = 8, ECH = 8;      // pieces, chunks a row, elements a chunk
+    static __device__ __forceinline__ acc mma(u32x4 a, u32x4 b, acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+struct F16 {
+    typedef f16_t elem;
+    typedef f32x4 acc;
+    static constexpr int PLANES = 1, BKC = 8, ECH = 8;
+    static __device__ __forceinline__ acc mma(u32x4 a, u32x4 b, acc c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+struct F32 {
+    typedef float elem;
+    typedef f32x4 acc;
+    static constexpr int PLANES = 3, BKC = 4, ECH = 8;
+    static __device__ __forceinline__ acc mma(u32x4 a, u32x4 b, acc c) { return BF16::mma(a, b, c); }
+};
+struct I8 {
+    typedef int8_t elem;
+    typedef i32x4 acc;
+    static constexpr int PLANES = 1, BKC = 8, ECH = 16;
+    static __device__ __forceinline__ acc mma(u32x4 a, u32x4 b, acc c)
+    {
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+    }
+};
+
+// max(v, 0) that keeps a NaN
+__device__ __forceinline__ float relu_of(float v) { return v < 0.0f ? 0.0f : v; }
+
+template <int BKC> __device__ __forceinline__ int swz(int row)
+{
+    return BKC == 8 ? (row ^ (row >> 3)) & 7 : ((row >> 1) ^ (row >> 3)) & 3;
+}
+// byte address of chunk q of a row
+template <int BKC> __device__ __forceinline__ int lds_at(int row, int q) { return row * (16 * BKC) + ((q ^ swz<BKC>(row)) << 4); }
+
+// ---- global loads
+// 16 bytes at p of which `avail` elements count; the rest read as zero.  Nothing at or beyond `end` is read.
+template <class E> __device__ __forceinline__ u32x4 load16_guarded(const E *p, const E *end, int avail)
+{
+    constexpr int N = 16 / sizeof(E);
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (avail <= 0) return v;
+    if (end - p >= N) {
+        v = *reinterpret_cast<const u32x4u *>(p);
+        if (avail < N) {
+            const int bytes = avail * (int)sizeof(E);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int keep = bytes - 4 * d;
+                v[d] = keep >= 4 ? v[d] : keep <= 0 ? 0u : v[d] & ((1u << (8 * keep)) - 1u);
+            }
+        }
+        return v;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (e < avail && p + e < end) {
+            uint32_t bits;
+            if constexpr (sizeof(E) == 4) bits = __builtin_bit_cast(uint32_t, p[e]);
+            else if constexpr (sizeof(E) == 2) bits = __builtin_bit_cast(uint16_t, p[e]);
+            else bits = (uint8_t)p[e];
+            v[e * (int)sizeof(E) / 4] |= bits << (8 * (e * (int)sizeof(E) % 4));
+        }
+    return v;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef bf16_t b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, b2));
+}
+// the three pieces of a pair of float32 values, packed
+__device__ __forceinline__ void split2(float a, float b, uint32_t out[3])
+{
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+        out[p] = pack_bf16(a, b);
+        if (p < 2) {
+            a -= __builtin_bit_cast(float, out[p] << 16);
+            b -= __builtin_bit_cast(float, out[p] & 0xFFFF0000u);
+        }
+    }
+}
+
+// ---- an operand with c along memory: rows of `ld` elements, ROWS of them a tile
+template <class T, int ROWS> struct Contiguous {
+    typedef typename T::elem E;
+    static constexpr int BKC = T::BKC, STEP = BKC * T::ECH, PER = ROWS * BKC / THREADS, LOADS = T::PLANES == 3 ? 2 : 1;
+    static_assert(PER >= 1, "tile too small for the workgroup");
+    u32x4 reg[PER][LOADS];
+    const E *base, *end;                     // (row 0 of the tile, c = 0) and the end of the tensor
+    uint32_t off[PER];                       // element offset of this thread's rows, chunk included
+    int q, count;                            // count: values of c there are
+
+    // rows_left >= 1: rows from row0 on that exist; later ones repeat the last
+    __device__ __forceinline__ void init(const E *tensor_row0, long long ld, int rows_left, int c_count, const E *tensor_end)
+    {
+        base = tensor_row0;
+        end = tensor_end;
+        count = c_count;
+        q = threadIdx.x % BKC;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = threadIdx.x / BKC + j * (THREADS / BKC);
+            off[j] = (uint32_t)((long long)min(r, rows_left - 1) * ld) + (uint32_t)(q * T::ECH);
+        }
+    }
+    __device__ __forceinline__ void load(int c0)
+    {
+        const E *at = base + c0;
+        if (c0 + STEP <= count) {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+#pragma unroll
+                for (int h = 0; h < LOADS; ++h) reg[j][h] = *reinterpret_cast<const u32x4u *>(at + off[j] + h * 4);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+#pragma unroll
+                for (int h = 0; h < LOADS; ++h)
+                    reg[j][h] = load16_guarded<E>(at + off[j] + h * 4, end, count - c0 - q * T::ECH - h * 4);
+        }
+    }
+    __device__ __forceinline__ void store(char *lds)
+    {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int r = threadIdx.x / BKC + j * (THREADS / BKC);
+            if constexpr (T::PLANES == 1) {
+                *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = reg[j][0];
+            } else {
+                u32x4 piece[3];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    uint32_t o[3];
+                    const f32x4 f = __builtin_bit_cast(f32x4, reg[j][d / 2]);
+                    split2(f[2 * (d & 1)], f[2 * (d & 1) + 1], o);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) piece[p][d] = o[p];
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<u32x4 *>(lds + p * (ROWS * BKC * 16) + lds_at<BKC>(r, q)) = piece[p];
+            }
+        }
+    }
+};
+
+// ---- an operand with the tile's rows along memory: element (row r, c) at base + c * ld + r
+template <class T, int ROWS> struct Strided {
+    typedef typename T::elem E;
+    static constexpr int BKC = T::BKC, STEP = BKC * 8, BLOCKS = THREADS / BKC, W = ROWS / BLOCKS;   // W rows x 8 c a thread
+    static_assert(W >= 1 && T::ECH == 8, "tile too small for the workgroup");
+    typedef E vec __attribute__((ext_vector_type(W), aligned(sizeof(E))));
+    vec reg[8];
+    const E *base, *end;
+    long long ld;
+    int r0, q, count;
+    bool whole;                              // all ROWS rows exist (workgroup-uniform)
+
+    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *tensor_end)
+    {
+        base = tensor_row0;
+        end = tensor_end;
+        ld = ld_;
+        count = c_count;
+        r0 = (threadIdx.x % BLOCKS) * W;
+        q = threadIdx.x / BLOCKS;
+        whole = rows_left >= ROWS;
+        if (r0 >= rows_left) r0 = 0;         // rows that do not exist: any that do (their results are not stored)
+    }
+    __device__ __forceinline__ void load(int c0)
+    {
+        const E *at = base + (long long)c0 * ld;
+        if (whole && c0 + STEP <= count) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                reg[e] = *reinterpret_cast<const vec *>(at + (uint32_t)((q * 8 + e) * (int)ld + r0));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool there = c0 + q * 8 + e < count;      // else: zero
+                const E *p = there ? at + (uint32_t)((q * 8 + e) * (int)ld + r0) : base;
+                vec v;
+                if (end - p >= W) {
+                    v = *reinterpret_cast<const vec *>(p);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < W; ++i) v[i] = p + i < end ? p[i] : (E)0;
+                }
+#pragma unroll
+                for (int i = 0; i < W; ++i) reg[e][i] = there ? v[i] : (E)0;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char *lds)
+    {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const int r = (threadIdx.x % BLOCKS) * W + i;
+            if constexpr (T::PLANES == 1) {
+                typedef E e8 __attribute__((ext_vector_type(8)));
+                e8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = reg[e][i];
+                *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = __builtin_bit_cast(u32x4, v);
+            } else {
+                u32x4 piece[3];
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    uint32_t o[3];
+                    split2((float)reg[2 * d][i], (float)reg[2 * d + 1][i], o);
+#pragma unroll
+                    for (int p = 0; p < 3; ++p) piece[p][d] = o[p];
+                }
+#pragma unroll
+                for (int p = 0; p < 3; ++p)
+                    *reinterpret_cast<u32x4 *>(lds + p * (ROWS * BKC * 16) + lds_at<BKC>(r, q)) = piece[p];
+            }
+        }
+    }
+};
+
+template <class T, int BM, int BN> constexpr int lds_bytes_one() { return (BM + BN) * T::BKC * 16 * T::PLANES; }
+
+// ---- the core: acc[mi][ni] += A B^T over c = 0 .. count; A gives i (BN), B gives j (BM)
+template <class T, int BM, int BN, class LA, class LB>
+__device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename T::acc (&acc)[BM / 32][BN / 32])
+{
+    constexpr int MI = BM / 32, NI = BN / 32, BKC = T::BKC, STEP = LA::STEP, P = T::PLANES;
+    constexpr int A_PLANE = BN * BKC * 16, B_PLANE = BM * BKC * 16;
+    static_assert(LA::STEP == LB::STEP, "one step for both operands");
+    char *la = lds, *lb = lds + A_PLANE * P;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i0 = (wave & 1) * (BN / 2) + (lane & 15), j0 = (wave >> 1) * (BM / 2) + (lane & 15), g = lane >> 4;
+    a.load(0);
+    b.load(0);
+    for (int c0 = 0; c0 < count; c0 += STEP) {
+        a.store(la);
+        b.store(lb);
+        __syncthreads();
+        if (c0 + STEP < count) {
+            a.load(c0 + STEP);
+            b.load(c0 + STEP);
+        }
+#pragma unroll
+        for (int s = 0; s < BKC / 4; ++s) {
+            u32x4 fa[P][NI], fb[P][MI];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int n = 0; n < NI; ++n) fa[p][n] = *reinterpret_cast<const u32x4 *>(la + p * A_PLANE + lds_at<BKC>(i0 + 16 * n, 4 * s + g));
+#pragma unroll
+                for (int m = 0; m < MI; ++m) fb[p][m] = *reinterpret_cast<const u32x4 *>(lb + p * B_PLANE + lds_at<BKC>(j0 + 16 * m, 4 * s + g));
+            }
+#pragma unroll
+            for (int m = 0; m < MI; ++m)
+#pragma unroll
+                for (int n = 0; n < NI; ++n) {
+                    if constexpr (P == 1) {
+                        acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
+                    } else {                 // smallest first
+                        acc[m][n] = T::mma(fa[1][n], fb[1][m], acc[m][n]);
+                        acc[m][n] = T::mma(fa[2][n], fb[0][m], acc[m][n]);
+                        acc[m][n] = T::mma(fa[0][n], fb[2][m], acc[m][n]);
+                        acc[m][n] = T::mma(fa[1][n], fb[0][m], acc[m][n]);
+                        acc[m][n] = T::mma(fa[0][n], fb[1][m], acc[m][n]);
+                        acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
+                    }
+                }
+        }
+        __syncthreads();
+    }
+}
+
+// C[i][j] once more in float32, for elements that the split made a NaN of
+__device__ __forceinline__ float dot_again(const float *a, long long sa, const float *b, long long sb, int count)
+{
+    float s = 0.0f;
+    for (int c = 0; c < count; ++c) s = fmaf(a[c * sa], b[c * sb], s);
+    return s;
+}
+
+// ---- ragged rows: group g owns rows offsets[g] .. offsets[g+1] - 1 of M.  Offsets outside 0 .. M are read as
+// the nearest inside, one below an earlier one as that one, so any values give a partition of the rows.
+// Rows that no group owns are the segments -1 (before offsets[0]) and G (behind offsets[G]).
+struct Segment {
+    int g, row0, rows;                       // rows of this tile, rows < 0: no such tile
+};
+
+// Bounds of 64 segments s0 .. s0 + 63 in the lanes (segment s is group s - 1); `carry` is the bound before s0.
+__device__ __forceinline__ void segment_bounds(const long long *offsets, int G, int M, int s0, int carry, int &lo, int &hi)
+{
+    const int s = s0 + (int)(threadIdx.x & 63);
+    // the bound at the END of segment s: offsets[s] for s <= G, M behind
+    long long v = s <= G ? (offsets ? offsets[s] : (s ? M : 0)) : M;
+    int e = v < 0 ? 0 : v > M ? M : (int)v;
+    e = max(e, carry);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(e, o, 64);
+        if ((int)(threadIdx.x & 63) >= o) e = max(e, up);
+    }
+    hi = e;
+    lo = __shfl_up(e, 1, 64);
+    if ((threadIdx.x & 63) == 0) lo = carry;
+}
+
+__device__ __forceinline__ int wave_scan(int v)          // inclusive
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(v, o, 64);
+        if ((int)(threadIdx.x & 63) >= o) v += up;
+    }
+    return v;
+}
+
+__device__ __forceinline__ int row_tiles(const long long *offsets, int G, int M, int BM)
+{
+    int total = 0, carry = 0;
+    for (int s0 = 0; s0 < G + 2; s0 += 64) {
+        int lo, hi;
+        segment_bounds(offsets, G, M, s0, carry, lo, hi);
+        total += __shfl(wave_scan((hi - lo + BM - 1) / BM), 63, 64);
+        carry = __shfl(hi, 63, 64);
+    }
+    return total;
+}
+
+// the t-th tile of BM rows
+__device__ __forceinline__ Segment row_tile(const long long *offsets, int G, int M, int BM, int t)
+{
+    int before = 0, carry = 0;
+    for (int s0 = 0; s0 < G + 2; s0 += 64) {
+        int lo, hi;
+        segment_bounds(offsets, G, M, s0, carry, lo, hi);
+        const int n = (hi - lo + BM - 1) / BM, upto = before + wave_scan(n);
+        const uint64_t holds = __ballot(t < upto);
+        if (holds) {
+            const int l = __builtin_ctzll(holds);
+            const int first = __shfl(upto - n, l, 64), rlo = __shfl(lo, l, 64), rhi = __shfl(hi, l, 64);
+            const int row0 = rlo + (t - first) * BM;
+            return {s0 + l - 1, row0, min(rhi - row0, BM)};
+        }
+        before = __shfl(upto, 63, 64);
+        carry = __shfl(hi, 63, 64);
+    }
+    return {0, 0, -1};
+}
+
+// rows of group g (workgroup-uniform)
+__device__ __forceinline__ void group_rows(const long long *offsets, int G, int M, int g, int &row0, int &rows)
+{
+    int carry = 0;
+    for (int s0 = 0; s0 < G + 2; s0 += 64) {
+        int lo, hi;
+        segment_bounds(offsets, G, M, s0, carry, lo, hi);
+        if (g + 1 < s0 + 64) {
+            row0 = __builtin_amdgcn_readfirstlane(__shfl(lo, g + 1 - s0, 64));
+            rows = __builtin_amdgcn_readfirstlane(__shfl(hi, g + 1 - s0, 64)) - row0;
+            return;
+        }
+        carry = __shfl(hi, 63, 64);
+    }
+    row0 = rows = 0;
+}
+
+inline long long row_tiles_most(int G, int M, int BM) { return (M + (long long)(G + 2) * (BM - 1)) / BM; }
+
+// Workgroups go round the eight XCDs in turn: logical tiles are dealt out so that an XCD works on a run of
+// them, and a run keeps to `band` row tiles and walks the columns, so that its operands stay in its L2.
+__device__ __forceinline__ bool tile_of_block(int block, int row_tiles, int col_tiles, int band, int &rt, int &ct)
+{
+    const int total = row_tiles * col_tiles;
+    if (block >= total) return false;
+    const int per = total / 8, extra = total % 8, xcd = block % 8, k = block / 8;
+    const int id = xcd * per + min(xcd, extra) + k;
+    const int b = id / (band * col_tiles), in = id - b * band * col_tiles, height = min(band, row_tiles - b * band);
+    rt = b * band + in % height;
+    ct = in / height;
+    return true;
+}
+
+}  // namespace tile

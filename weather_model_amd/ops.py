@@ -950,6 +950,263 @@ def mse_metrics(pred, y, broadcast, eps=1e-7, want_grad=True):
     return out3, grad
 
 
+# --------------------------------------------------------------------------- layers of experts
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}      # WM_F32, WM_BF16, WM_F16
+
+
+def _req_any(t, name, like=None):
+    """``_req`` for the operators that also take bfloat16 and float16; ``like`` fixes type and device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must live on the GPU (weather_model_amd has no CPU fallback)")
+    if t.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError(f"{name} must be {like.dtype} like the rows, got {t.dtype}")
+        _same_device(t, name, like)
+    return t.contiguous()
+
+
+def _same_device(t, name, like):
+    if t.device != like.device:
+        raise ValueError(f"{name} lives on {t.device}, the rows on {like.device}")
+    return t
+
+
+def _out_any(out, shape, like, name):
+    if out is None:
+        return torch.empty(shape, device=like.device, dtype=like.dtype)
+    if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device or \
+            not out.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {like.dtype} {tuple(shape)} tensor on {like.device}")
+    return out
+
+
+def _call(device, fn, *args):
+    """``fn(*args, stream)`` on the current stream of ``device``, which is made current for the call."""
+    if torch.cuda.current_device() == device.index:
+        _lib.check(fn(*args, _stream()))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, _stream()))
+
+
+def _grouped_args(x, weight, offsets):
+    x = _req_any(x, "input")
+    weight = _req_any(weight, "weight", x)
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
+        raise ValueError(f"dense_grouped expects (M, K) and (G, N, K), got {tuple(x.shape)}, "
+                         f"{tuple(weight.shape)}")
+    return x, weight, _group_offsets(offsets, weight.shape[0], x)
+
+
+def _group_offsets(offsets, groups, x):
+    offsets = _same_device(_req(offsets, "offsets", torch.int64), "offsets", x)
+    if tuple(offsets.shape) != (groups + 1,):
+        raise ValueError(f"offsets must be ({groups + 1},) for {groups} groups, got {tuple(offsets.shape)}")
+    return offsets
+
+
+def group_offsets(counts):
+    """Row offsets (G + 1,) int64 from the number of rows of each group (G,), on their device."""
+    out = torch.zeros((counts.numel() + 1,), device=counts.device, dtype=torch.int64)
+    torch.cumsum(counts, 0, out=out[1:])
+    return out
+
+
+def dense_grouped_forward(x, weight, offsets, bias=None, relu=False, out=None):
+    """Dense layers of G experts in one launch (``wm_dense_grouped_fwd``): row r of x (M, K), owned by
+    the expert g with offsets[g] <= r < offsets[g + 1], becomes act(weight[g] @ x[r] + bias[g]).
+    weight (G, N, K), bias (G, N), offsets (G + 1,) int64 on the GPU -- the host never reads them.  float32,
+    bfloat16 or float16 (all alike); sums in float32.  Rows of no expert become zeros."""
+    x, weight, offsets = _grouped_args(x, weight, offsets)
+    M, K = x.shape
+    G, N, _ = weight.shape
+    if bias is not None:
+        bias = _req_any(bias, "bias", x)
+        if tuple(bias.shape) != (G, N):
+            raise ValueError(f"bias must be {(G, N)}, got {tuple(bias.shape)}")
+    y = _out_any(out, (M, N), x, "out")
+    _call(x.device, _lib.lib().wm_dense_grouped_fwd, x.data_ptr(), weight.data_ptr(),
+          0 if bias is None else bias.data_ptr(), y.data_ptr(), offsets.data_ptr(), G, M, N, K,
+          _DTYPES[x.dtype], 1 if relu else 0)
+    return y
+
+
+def dense_grouped_backward(x, weight, offsets, gy, mask_below=None, need_gx=True, need_gw=True,
+                           need_bias=True, out_w=None, out_b=None):
+    """(gx, gW, gb) of ``dense_grouped_forward`` given the gradient gy of its PRE-activation output, each
+    None where not asked for (gb is formed with gW); ``mask_below`` (the post-ReLU activation that is this
+    layer's input) zeroes gx where it is not positive.  Experts without rows get zeros."""
+    x, weight, offsets = _grouped_args(x, weight, offsets)
+    M, K = x.shape
+    G, N, _ = weight.shape
+    gy = _req_any(gy, "grad_output", x)
+    if tuple(gy.shape) != (M, N):
+        raise ValueError(f"grad_output must be {(M, N)}, got {tuple(gy.shape)}")
+    L, dt = _lib.lib(), _DTYPES[x.dtype]
+    gx = gw = gb = None
+    if need_gx:
+        if mask_below is not None:
+            mask_below = _req_any(mask_below, "mask", x)
+            if tuple(mask_below.shape) != (M, K):
+                raise ValueError(f"mask must be {(M, K)}, got {tuple(mask_below.shape)}")
+        gx = torch.empty((M, K), device=x.device, dtype=x.dtype)
+        _call(x.device, L.wm_dense_grouped_bwd_data, gy.data_ptr(), weight.data_ptr(),
+              0 if mask_below is None else mask_below.data_ptr(), gx.data_ptr(), offsets.data_ptr(), G, M,
+              N, K, dt)
+    if need_gw:
+        gw = _out_any(out_w, (G, N, K), x, "out_w")
+        gb = _out_any(out_b, (G, N), x, "out_b") if need_bias else None
+        need = L.wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K)
+        ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
+        _call(x.device, L.wm_dense_grouped_bwd_wb, x.data_ptr(), gy.data_ptr(), gw.data_ptr(),
+              0 if gb is None else gb.data_ptr(), 0 if ws is None else ws.data_ptr(), need,
+              offsets.data_ptr(), G, M, N, K, dt)
+    return gx, gw, gb
+
+
+class DenseGroupedFunction(torch.autograd.Function):
+    """``dense_grouped_forward`` under autograd; ``relu_input`` and ``relu_bwd_fused`` as in
+    ``DenseFunction``."""
+
+    @staticmethod
+    def forward(ctx, x, weight, offsets, bias, relu, relu_input, relu_bwd_fused):
+        y = dense_grouped_forward(x, weight, offsets, bias, relu)
+        own_mask = relu and not relu_bwd_fused
+        ctx.save_for_backward(x, weight, offsets, y if own_mask else None)
+        ctx.own_mask, ctx.relu_input, ctx.has_bias = own_mask, relu_input, bias is not None
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        x, weight, offsets, y = ctx.saved_tensors
+        if ctx.own_mask:
+            gy = torch.where(y > 0, gy, 0.0)          # stand-alone mask (no fusing consumer), any type
+        need_b = ctx.has_bias and ctx.needs_input_grad[3]
+        gx, gw, gb = dense_grouped_backward(x, weight, offsets, gy, x if ctx.relu_input else None,
+                                            need_gx=ctx.needs_input_grad[0],
+                                            need_gw=ctx.needs_input_grad[1] or need_b, need_bias=need_b)
+        return gx, gw if ctx.needs_input_grad[1] else None, None, gb, None, None, None
+
+
+def dense_grouped(x, weight, offsets, bias=None, relu=False, relu_input=False, relu_bwd_fused=False):
+    """act(weight[g] @ x[r] + bias[g]) for the rows r of each expert g, with gradients."""
+    return DenseGroupedFunction.apply(x, weight, offsets, bias, relu, relu_input, relu_bwd_fused)
+
+
+def _dropout_args(p, seed, offset, x):
+    p, seed = float(p), int(seed)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability must be within 0 .. 1, got {p}")
+    if not 0 <= seed < 1 << 32:
+        raise ValueError(f"seed must be within 0 .. 2^32 - 1, got {seed}")
+    if isinstance(offset, torch.Tensor):
+        if offset.dtype != torch.int64 or offset.numel() != 1 or not offset.is_cuda:
+            raise TypeError("a device offset must be one int64 on the GPU")
+        return p, seed, 0, _same_device(offset, "offset", x).data_ptr()
+    offset = int(offset)
+    if not 0 <= offset < 1 << 63:
+        raise ValueError(f"offset must be within 0 .. 2^63 - 1, got {offset}")
+    return p, seed, offset, 0
+
+
+def dropout_forward(x, p, seed, offset=0, residual=None, out=None):
+    """residual + x / (1 - p) where element ``offset + i`` of the stream ``seed`` is kept, residual alone
+    where it is dropped (``wm_dropout``).  The mask is a function of (seed, offset + i) and is stored
+    nowhere: the backward pass draws it again.  ``offset`` is an integer or one int64 on the GPU (read by
+    the kernel, so that replays of a captured graph can move on); advance it by x.numel() from call to
+    call.  float32, bfloat16 or float16; p is held to 2^-32; ``out`` may be x or residual."""
+    x = _req_any(x, "input")
+    p, seed, off, off_dev = _dropout_args(p, seed, offset, x)
+    if residual is not None:
+        residual = _req_any(residual, "residual", x)
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
+    y = _out_any(out, x.shape, x, "out")
+    _call(x.device, _lib.lib().wm_dropout, x.data_ptr(), 0 if residual is None else residual.data_ptr(),
+          y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, seed, off, off_dev)
+    return y
+
+
+def dropout_backward(gy, p, seed, offset=0, out=None):
+    """Gradient of ``dropout_forward`` with respect to x (that of the residual is gy itself)."""
+    return dropout_forward(gy, p, seed, offset, None, out)
+
+
+class DropoutFunction(torch.autograd.Function):
+    """``dropout_forward`` under autograd: saves nothing but a device offset."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        on_device = isinstance(offset, torch.Tensor)
+        ctx.save_for_backward(offset if on_device else None)
+        ctx.p, ctx.seed, ctx.offset = p, seed, None if on_device else offset
+        return dropout_forward(x, p, seed, offset, residual)
+
+    @staticmethod
+    def backward(ctx, gy):
+        offset, = ctx.saved_tensors
+        gx = dropout_backward(gy, ctx.p, ctx.seed, ctx.offset if offset is None else offset) \
+            if ctx.needs_input_grad[0] else None
+        return gx, (gy if ctx.needs_input_grad[1] else None), None, None, None
+
+
+def dropout(x, p, seed, offset=0, residual=None):
+    """``dropout_forward`` with gradients.  A device ``offset`` may be advanced after the backward pass, not
+    between the two (autograd notices and refuses)."""
+    return DropoutFunction.apply(x, residual, p, seed, offset)
+
+
+def quantize_rows(x):
+    """8-bit codes of x (M, K) with a float32 scale per row (``wm_quantize_rows_i8``): scale = max|row| / 127,
+    codes = row / scale rounded to even.  Also packs a Dense weight (N, K): one scale per output channel."""
+    x = _req_any(x, "input")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"quantize_rows expects (M, K) with K > 0, got {tuple(x.shape)}")
+    M, K = x.shape
+    q = torch.empty((M, K), device=x.device, dtype=torch.int8)
+    scale = torch.empty((M,), device=x.device, dtype=torch.float32)
+    _call(x.device, _lib.lib().wm_quantize_rows_i8, x.data_ptr(), M, K, _DTYPES[x.dtype], q.data_ptr(),
+          scale.data_ptr())
+    return q, scale
+
+
+def dense_i8(x, weight, scale, bias=None, relu=False, offsets=None, out=None):
+    """act(x @ W.T + bias) in 8-bit integers (``wm_dense_i8``): x (M, K) float32, bfloat16 or float16 is
+    quantised by row, weight (N, K) int8 holds codes with ``scale`` (N,) per channel (``quantize_rows`` makes
+    both), bias (N,) float32.  Exact integer sums, output in the type of x.  With ``offsets`` (G + 1,) the
+    rows are grouped as in ``dense_grouped_forward``: weight (G, N, K), scale and bias (G, N)."""
+    x = _req_any(x, "input")
+    weight = _same_device(_req(weight, "weight", torch.int8), "weight", x)
+    scale = _same_device(_req(scale, "scale"), "scale", x)
+    lead = 2 if offsets is None else 3
+    if x.dim() != 2 or weight.dim() != lead or x.shape[1] != weight.shape[-1]:
+        raise ValueError(f"dense_i8 expects (M, K) and {'(N, K)' if lead == 2 else '(G, N, K)'}, got "
+                         f"{tuple(x.shape)}, {tuple(weight.shape)}")
+    if scale.shape != weight.shape[:-1]:
+        raise ValueError(f"scale must be {tuple(weight.shape[:-1])}, got {tuple(scale.shape)}")
+    M, K = x.shape
+    G, N = (1, weight.shape[0]) if offsets is None else weight.shape[:2]
+    if offsets is not None:
+        offsets = _group_offsets(offsets, G, x)
+    if bias is not None:
+        bias = _same_device(_req(bias, "bias"), "bias", x)
+        if bias.shape != scale.shape:
+            raise ValueError(f"bias must be {tuple(scale.shape)}, got {tuple(bias.shape)}")
+    y = _out_any(out, (M, N), x, "out")
+    L = _lib.lib()
+    need = L.wm_dense_i8_workspace_bytes(M, K)
+    ws = torch.empty((need,), device=x.device, dtype=torch.uint8)
+    _call(x.device, L.wm_dense_i8, x.data_ptr(), weight.data_ptr(), scale.data_ptr(),
+          0 if bias is None else bias.data_ptr(), y.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
+          G, M, N, K, _DTYPES[x.dtype], 1 if relu else 0, ws.data_ptr(), need)
+    return y
+
+
 # --------------------------------------------------------------------------- synthetic data
 
 def synth_uniform(shape, seed, lo=0.0, hi=1.0, offset=0, device="cuda"):
