@@ -30,7 +30,7 @@ __global__ __launch_bounds__(THREADS) void grouped_rows_kernel(const typename T:
     int rt, ct;
     if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (NO + BN - 1) / BN, band, rt, ct)) return;
     const Segment s = row_tile(offsets, G, M, BM, rt);
-    const int n0 = ct * BN, cols = min(BN, NO - n0);
+    const int n0 = min(ct * BN, max(0, NO - BN)), cols = min(BN, NO);       // the last tile moves back over its neighbour
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) out[(long long)(s.row0 + e / cols) * NO + n0 + e % cols] = (E)0.0f;
         return;
@@ -104,9 +104,9 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_kernel(const typename
     // i (contiguous in the output) is k, j is n
     const int kt = (K + BN - 1) / BN, nt = (N + BM - 1) / BM;
     int id = blockIdx.x;
-    const int k0 = id % kt * BN;
+    const int k0 = min(id % kt * BN, max(0, K - BN));       // last tiles move back over their neighbours
     id /= kt;
-    const int n0 = id % nt * BM;
+    const int n0 = min(id % nt * BM, max(0, N - BM));
     id /= nt;
     const int g = id % G, split = id / G;
     int row0, rows;
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_kernel(const typename
     for (int m = 0; m < MI; ++m)
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[m][n] = typename T::acc{0, 0, 0, 0};
-    const int ks = min(BN, K - k0), ns = min(BM, N - n0);
+    const int ks = min(BN, K), ns = min(BM, N);
     const E *xt = x + (long long)row0 * K + k0, *yt = gy + (long long)row0 * N + n0;
     if (rows > 0) {
         Strided<T, BN> a;

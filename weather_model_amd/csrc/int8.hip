@@ -55,7 +55,7 @@ __global__ __launch_bounds__(THREADS) void dense_i8_kernel(const int8_t *__restr
     int rt, ct;
     if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (N + BN - 1) / BN, band, rt, ct)) return;
     const Segment s = row_tile(offsets, G, M, BM, rt);
-    const int n0 = ct * BN, cols = min(BN, N - n0);
+    const int n0 = min(ct * BN, max(0, N - BN)), cols = min(BN, N);         // the last tile moves back over its neighbour
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) y[(long long)(s.row0 + e / cols) * N + n0 + e % cols] = (E)0.0f;
         return;

@@ -27,6 +27,7 @@ constexpr int THREADS = 256;                 // four waves, 2 x 2 over the tile
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32u __attribute__((aligned(1)));
 typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(1)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16_t f16x8 __attribute__((ext_vector_type(8)));
@@ -150,21 +151,23 @@ template <class T, int ROWS> struct Contiguous {
             off[j] = (uint32_t)((long long)min(r, rows_left - 1) * ld) + (uint32_t)(q * T::ECH);
         }
     }
+    static constexpr bool slow = false;      // every whole step can take load()
     __device__ __forceinline__ void load(int c0)
     {
         const E *at = base + c0;
-        if (c0 + STEP <= count) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
+        for (int j = 0; j < PER; ++j)
 #pragma unroll
-                for (int h = 0; h < LOADS; ++h) reg[j][h] = *reinterpret_cast<const u32x4u *>(at + off[j] + h * 4);
-        } else {
+            for (int h = 0; h < LOADS; ++h) reg[j][h] = *reinterpret_cast<const u32x4u *>(at + off[j] + h * 4);
+    }
+    __device__ __forceinline__ void load_guarded(int c0)
+    {
+        const E *at = base + c0;
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
+        for (int j = 0; j < PER; ++j)
 #pragma unroll
-                for (int h = 0; h < LOADS; ++h)
-                    reg[j][h] = load16_guarded<E>(at + off[j] + h * 4, end, count - c0 - q * T::ECH - h * 4);
-        }
+            for (int h = 0; h < LOADS; ++h)
+                reg[j][h] = load16_guarded<E>(at + off[j] + h * 4, end, count - c0 - q * T::ECH - h * 4);
     }
     __device__ __forceinline__ void store(char *lds)
     {
@@ -195,66 +198,78 @@ template <class T, int ROWS> struct Contiguous {
 template <class T, int ROWS> struct Strided {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * 8, BLOCKS = THREADS / BKC, W = ROWS / BLOCKS;   // W rows x 8 c a thread
-    static_assert(W >= 1 && T::ECH == 8, "tile too small for the workgroup");
-    typedef E vec __attribute__((ext_vector_type(W), aligned(sizeof(E))));
-    vec reg[8];
-    const E *base, *end;
+    static constexpr int WORDS = W * sizeof(E) / 4, PER_WORD = 4 / sizeof(E);
+    static_assert(WORDS >= 1 && T::ECH == 8, "tile too small for the workgroup");
+    typedef uint32_t words __attribute__((ext_vector_type(WORDS), aligned(sizeof(E))));
+    uint32_t reg[8][WORDS];
+    const E *base;
     long long ld;
     int r0, q, count;
-    bool whole;                              // all ROWS rows exist (workgroup-uniform)
+    int most;                                // rows that exist, at least 1
+    bool slow;                               // fewer rows than a thread's vector: load() does not fit (workgroup-uniform)
 
-    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *tensor_end)
+    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *)
     {
         base = tensor_row0;
-        end = tensor_end;
         ld = ld_;
         count = c_count;
-        r0 = (threadIdx.x % BLOCKS) * W;
         q = threadIdx.x / BLOCKS;
-        whole = rows_left >= ROWS;
-        if (r0 >= rows_left) r0 = 0;         // rows that do not exist: any that do (their results are not stored)
+        most = rows_left;
+        slow = rows_left < W;
+        // a vector that would leave the rows moves back into them: two threads then write the same values to the
+        // same place, and rows that do not exist keep whatever LDS held (their results are not stored)
+        r0 = slow ? 0 : min((int)(threadIdx.x % BLOCKS) * W, rows_left - W);
     }
     __device__ __forceinline__ void load(int c0)
     {
         const E *at = base + (long long)c0 * ld;
-        if (whole && c0 + STEP <= count) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                reg[e] = *reinterpret_cast<const vec *>(at + (uint32_t)((q * 8 + e) * (int)ld + r0));
-        } else {
+        for (int e = 0; e < 8; ++e) {
+            const E *p = at + (uint32_t)((q * 8 + e) * (int)ld + r0);
+            if constexpr (WORDS == 1) {
+                reg[e][0] = *reinterpret_cast<const u32u *>(p);
+            } else {
+                const words v = *reinterpret_cast<const words *>(p);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const bool there = c0 + q * 8 + e < count;      // else: zero
-                const E *p = there ? at + (uint32_t)((q * 8 + e) * (int)ld + r0) : base;
-                vec v;
-                if (end - p >= W) {
-                    v = *reinterpret_cast<const vec *>(p);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < W; ++i) v[i] = p + i < end ? p[i] : (E)0;
-                }
-#pragma unroll
-                for (int i = 0; i < W; ++i) reg[e][i] = there ? v[i] : (E)0;
+                for (int w = 0; w < WORDS; ++w) reg[e][w] = v[w];
             }
         }
+    }
+    __device__ __forceinline__ void load_guarded(int c0)
+    {
+        const E *at = base + (long long)c0 * ld;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                uint32_t v = 0;
+#pragma unroll
+                for (int i = 0; i < PER_WORD; ++i)
+                    if (c0 + q * 8 + e < count && r0 + w * PER_WORD + i < most) {
+                        const E *p = at + (uint32_t)((q * 8 + e) * (int)ld + r0 + w * PER_WORD + i);
+                        if constexpr (PER_WORD == 1) v = __builtin_bit_cast(uint32_t, *p);
+                        else v |= (uint32_t)__builtin_bit_cast(uint16_t, *p) << (16 * i);
+                    }
+                reg[e][w] = v;
+            }
     }
     __device__ __forceinline__ void store(char *lds)
     {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            const int r = (threadIdx.x % BLOCKS) * W + i;
+            const int r = r0 + i;
             if constexpr (T::PLANES == 1) {
-                typedef E e8 __attribute__((ext_vector_type(8)));
-                e8 v;
+                u32x4 v;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = reg[e][i];
-                *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = __builtin_bit_cast(u32x4, v);
+                for (int d = 0; d < 4; ++d)
+                    v[d] = __builtin_amdgcn_perm(reg[2 * d + 1][i / 2], reg[2 * d][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = v;
             } else {
                 u32x4 piece[3];
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     uint32_t o[3];
-                    split2((float)reg[2 * d][i], (float)reg[2 * d + 1][i], o);
+                    split2(__builtin_bit_cast(float, reg[2 * d][i]), __builtin_bit_cast(float, reg[2 * d + 1][i]), o);
 #pragma unroll
                     for (int p = 0; p < 3; ++p) piece[p][d] = o[p];
                 }
@@ -269,51 +284,72 @@ template <class T, int ROWS> struct Strided {
 template <class T, int BM, int BN> constexpr int lds_bytes_one() { return (BM + BN) * T::BKC * 16 * T::PLANES; }
 
 // ---- the core: acc[mi][ni] += A B^T over c = 0 .. count; A gives i (BN), B gives j (BM)
+template <class T, int BM, int BN>
+__device__ __forceinline__ void multiply(const char *la, const char *lb, typename T::acc (&acc)[BM / 32][BN / 32])
+{
+    constexpr int MI = BM / 32, NI = BN / 32, BKC = T::BKC, P = T::PLANES;
+    constexpr int A_PLANE = BN * BKC * 16, B_PLANE = BM * BKC * 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i0 = (wave & 1) * (BN / 2) + (lane & 15), j0 = (wave >> 1) * (BM / 2) + (lane & 15), g = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < BKC / 4; ++s) {
+        u32x4 fa[P][NI], fb[P][MI];
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (int n = 0; n < NI; ++n) fa[p][n] = *reinterpret_cast<const u32x4 *>(la + p * A_PLANE + lds_at<BKC>(i0 + 16 * n, 4 * s + g));
+#pragma unroll
+            for (int m = 0; m < MI; ++m) fb[p][m] = *reinterpret_cast<const u32x4 *>(lb + p * B_PLANE + lds_at<BKC>(j0 + 16 * m, 4 * s + g));
+        }
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+            for (int n = 0; n < NI; ++n) {
+                if constexpr (P == 1) {
+                    acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
+                } else {                     // smallest first
+                    acc[m][n] = T::mma(fa[1][n], fb[1][m], acc[m][n]);
+                    acc[m][n] = T::mma(fa[2][n], fb[0][m], acc[m][n]);
+                    acc[m][n] = T::mma(fa[0][n], fb[2][m], acc[m][n]);
+                    acc[m][n] = T::mma(fa[1][n], fb[0][m], acc[m][n]);
+                    acc[m][n] = T::mma(fa[0][n], fb[1][m], acc[m][n]);
+                    acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
+                }
+            }
+    }
+}
+
+// Whole steps: the next step's loads are in flight while this one is multiplied (the last step loads itself once
+// more instead of branching: a branch around the loads makes the compiler wait for them at its end).  What is left
+// of the last step goes through the guarded loads, which put zeros behind the end on both sides.
 template <class T, int BM, int BN, class LA, class LB>
 __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename T::acc (&acc)[BM / 32][BN / 32])
 {
-    constexpr int MI = BM / 32, NI = BN / 32, BKC = T::BKC, STEP = LA::STEP, P = T::PLANES;
-    constexpr int A_PLANE = BN * BKC * 16, B_PLANE = BM * BKC * 16;
+    constexpr int STEP = LA::STEP;
     static_assert(LA::STEP == LB::STEP, "one step for both operands");
-    char *la = lds, *lb = lds + A_PLANE * P;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = (wave & 1) * (BN / 2) + (lane & 15), j0 = (wave >> 1) * (BM / 2) + (lane & 15), g = lane >> 4;
-    a.load(0);
-    b.load(0);
-    for (int c0 = 0; c0 < count; c0 += STEP) {
+    char *la = lds, *lb = lds + BN * T::BKC * 16 * T::PLANES;
+    const int full = a.slow || b.slow ? 0 : count / STEP * STEP;
+    if (full > 0) {
+        a.load(0);
+        b.load(0);
+        for (int c0 = STEP; c0 <= full; c0 += STEP) {
+            a.store(la);
+            b.store(lb);
+            __syncthreads();
+            const int next = min(c0, full - STEP);
+            a.load(next);
+            b.load(next);
+            multiply<T, BM, BN>(la, lb, acc);
+            __syncthreads();
+        }
+    }
+    for (int c0 = full; c0 < count; c0 += STEP) {
+        a.load_guarded(c0);
+        b.load_guarded(c0);
         a.store(la);
         b.store(lb);
         __syncthreads();
-        if (c0 + STEP < count) {
-            a.load(c0 + STEP);
-            b.load(c0 + STEP);
-        }
-#pragma unroll
-        for (int s = 0; s < BKC / 4; ++s) {
-            u32x4 fa[P][NI], fb[P][MI];
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-#pragma unroll
-                for (int n = 0; n < NI; ++n) fa[p][n] = *reinterpret_cast<const u32x4 *>(la + p * A_PLANE + lds_at<BKC>(i0 + 16 * n, 4 * s + g));
-#pragma unroll
-                for (int m = 0; m < MI; ++m) fb[p][m] = *reinterpret_cast<const u32x4 *>(lb + p * B_PLANE + lds_at<BKC>(j0 + 16 * m, 4 * s + g));
-            }
-#pragma unroll
-            for (int m = 0; m < MI; ++m)
-#pragma unroll
-                for (int n = 0; n < NI; ++n) {
-                    if constexpr (P == 1) {
-                        acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
-                    } else {                 // smallest first
-                        acc[m][n] = T::mma(fa[1][n], fb[1][m], acc[m][n]);
-                        acc[m][n] = T::mma(fa[2][n], fb[0][m], acc[m][n]);
-                        acc[m][n] = T::mma(fa[0][n], fb[2][m], acc[m][n]);
-                        acc[m][n] = T::mma(fa[1][n], fb[0][m], acc[m][n]);
-                        acc[m][n] = T::mma(fa[0][n], fb[1][m], acc[m][n]);
-                        acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
-                    }
-                }
-        }
+        multiply<T, BM, BN>(la, lb, acc);
         __syncthreads();
     }
 }
