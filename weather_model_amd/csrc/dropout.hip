@@ -12,45 +12,88 @@
 
 namespace {
 
-constexpr int BLOCK = 256;
+constexpr int BLOCK = 256, UNROLL = 2;
 
-// bit j of the result: element e0 + j (j < 4) is dropped
-__device__ __forceinline__ unsigned dropped4(uint64_t seed, uint64_t e0, unsigned sub, uint32_t upper, uint32_t lower)
+// four draws of elements e0 .. e0 + 3, e0 = 4 g + sub: 16 bits each
+__device__ __forceinline__ uint64_t draws4(uint64_t seed, uint64_t g, unsigned sub)
 {
-    const uint64_t g = e0 >> 2;
     uint64_t w = hash64(seed, g);
-    if (sub) w = (w >> (16 * sub)) | (hash64(seed, g + 1) << (64 - 16 * sub));
-    unsigned drop = 0, tie = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t d = (uint32_t)(w >> (16 * j)) & 0xFFFFu;
-        drop |= (d < upper ? 1u : 0u) << j;
-        tie |= (d == upper ? 1u : 0u) << j;
-    }
-    if (tie != 0 && lower != 0)
-        for (int j = 0; j < 4; ++j)
-            if (tie >> j & 1) {
-                const uint64_t e = e0 + j;
-                const uint64_t z = hash64(seed, hash64(seed, e >> 2));
-                if (((uint32_t)(z >> (16 * (e & 3))) & 0xFFFFu) < lower) drop |= 1u << j;
-            }
-    return drop;
+    if (sub) w = (w >> (16 * sub)) | (hash64(seed, g + 1) << (64 - 16 * sub));      // sub is the same for all lanes
+    return w;
 }
 
-template <class T>
-__global__ __launch_bounds__(BLOCK) void dropout_kernel(const T *__restrict__ x, const T *__restrict__ res, T *__restrict__ y,
+// drop[j] for elements e0 .. e0 + V - 1
+template <int V>
+__device__ __forceinline__ void draw(uint64_t seed, uint64_t e0, unsigned sub, uint32_t upper, uint32_t lower, bool (&drop)[V])
+{
+    bool tie = false;
+#pragma unroll
+    for (int h = 0; h < V / 4; ++h) {
+        const uint64_t w = draws4(seed, (e0 >> 2) + h, sub);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t d = (uint32_t)(w >> (16 * j)) & 0xFFFFu;
+            drop[4 * h + j] = d < upper;
+            tie |= d == upper;
+        }
+    }
+    if (lower != 0 && tie) {                     // one vector of 8 in 8192
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint64_t e = e0 + j, z = hash64(seed, e >> 2);
+            if (((uint32_t)(z >> (16 * (e & 3))) & 0xFFFFu) == upper)
+                drop[j] = ((uint32_t)(hash64(seed, z) >> (16 * (e & 3))) & 0xFFFFu) < lower;
+        }
+    }
+}
+
+// A thread takes UNROLL vectors of 16 bytes, BLOCK vectors apart: their loads go out before the first hash.
+template <class T, bool RES>
+__global__ __launch_bounds__(BLOCK) void dropout_kernel(const T *x, const T *res, T *y,
                                                         long long n, uint64_t seed, uint64_t offset,
                                                         const long long *__restrict__ offset_dev, uint32_t upper,
                                                         uint32_t lower, float scale)
 {
+    constexpr int V = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
     const uint64_t base = offset + (offset_dev ? (uint64_t)*offset_dev : 0);
     const unsigned sub = (unsigned)(base & 3);
-    for (long long i = ((long long)blockIdx.x * BLOCK + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * BLOCK * 4) {
-        const unsigned drop = dropped4(seed, base + (uint64_t)i, sub, upper, lower);
-        for (int j = 0; j < 4 && i + j < n; ++j) {
-            float v = drop >> j & 1 ? 0.0f : to_float(x[i + j]) * scale;
-            if (res) v += to_float(res[i + j]);
-            y[i + j] = from_float<T>(v);
+    constexpr long long SPAN = (long long)BLOCK * V * UNROLL;
+    for (long long b = blockIdx.x * SPAN; b < n; b += gridDim.x * SPAN) {
+        const long long i0 = b + threadIdx.x * V;
+        if (b + SPAN <= n) {
+            vec in[UNROLL], r[UNROLL];
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                in[u] = *reinterpret_cast<const vec *>(x + i0 + u * BLOCK * V);
+                if (RES) r[u] = *reinterpret_cast<const vec *>(res + i0 + u * BLOCK * V);
+            }
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u) {
+                const long long i = i0 + u * BLOCK * V;
+                bool drop[V];
+                draw<V>(seed, base + (uint64_t)i, sub, upper, lower, drop);
+                vec o;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    float v = drop[j] ? 0.0f : to_float((T)in[u][j]) * scale;
+                    if (RES) v += to_float((T)r[u][j]);
+                    o[j] = from_float<T>(v);
+                }
+                *reinterpret_cast<vec *>(y + i) = o;
+            }
+        } else {
+            for (long long i = i0; i < n; i += BLOCK * V) {
+                bool drop[V];
+                draw<V>(seed, base + (uint64_t)i, sub, upper, lower, drop);
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (i + j < n) {
+                        float v = drop[j] ? 0.0f : to_float(x[i + j]) * scale;
+                        if (RES) v += to_float(res[i + j]);
+                        y[i + j] = from_float<T>(v);
+                    }
+            }
         }
     }
 }
@@ -60,10 +103,16 @@ int launch(const void *x, const void *res, void *y, long long n, uint64_t seed, 
            uint64_t thr, hipStream_t st)
 {
     const float scale = thr >> 32 ? 0.0f : (float)(0x1p32 / (0x1p32 - (double)thr));
-    long long blocks = (n + 4 * BLOCK - 1) / (4 * BLOCK);
+    constexpr long long SPAN = (long long)BLOCK * (16 / sizeof(T)) * UNROLL;
+    long long blocks = (n + SPAN - 1) / SPAN;
     if (blocks > 1 << 20) blocks = 1 << 20;
-    hipLaunchKernelGGL(dropout_kernel<T>, dim3((unsigned)blocks), dim3(BLOCK), 0, st, (const T *)x, (const T *)res, (T *)y, n,
-                       seed, offset, offset_dev, (uint32_t)(thr >> 16), (uint32_t)(thr & 0xFFFF), scale);
+    const uint32_t upper = (uint32_t)(thr >> 16), lower = (uint32_t)(thr & 0xFFFF);
+    if (res)
+        hipLaunchKernelGGL((dropout_kernel<T, true>), dim3((unsigned)blocks), dim3(BLOCK), 0, st, (const T *)x, (const T *)res, (T *)y, n, seed,
+                           offset, offset_dev, upper, lower, scale);
+    else
+        hipLaunchKernelGGL((dropout_kernel<T, false>), dim3((unsigned)blocks), dim3(BLOCK), 0, st, (const T *)x, (const T *)nullptr, (T *)y, n,
+                           seed, offset, offset_dev, upper, lower, scale);
     WM_LAUNCH_CHECK("dropout_kernel");
     return WM_OK;
 }

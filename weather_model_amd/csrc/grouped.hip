@@ -11,6 +11,8 @@ namespace {
 
 using namespace tile;
 
+constexpr int THREADS = 256;                 // of the kernels without tiles
+
 template <class T> __device__ __forceinline__ f32x4 load4_f32(const T *p)
 {
     return __builtin_convertvector(*reinterpret_cast<const typename Vec4<T>::type *>(p), f32x4);
@@ -18,15 +20,15 @@ template <class T> __device__ __forceinline__ f32x4 load4_f32(const T *p)
 
 // ---- rows: out (M, NO) = x (M, C) times W[g], forward (W[g] is (NO, C), its c along memory) or backward
 // (W[g] is (C, NO)).  bias and relu are the forward's, mask the backward's.
-template <class T, int BM, int BN, bool BACKWARD>
-__global__ __launch_bounds__(THREADS) void grouped_rows_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
-                                                               const typename T::elem *__restrict__ bias,
-                                                               const typename T::elem *__restrict__ mask,
-                                                               typename T::elem *__restrict__ out, const long long *__restrict__ offsets,
-                                                               int G, int M, int NO, int C, int relu, int band)
+template <class S, bool BACKWARD, class E = typename S::T::elem>
+__global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
+                                                                  const E *__restrict__ mask, E *__restrict__ out,
+                                                                  const long long *__restrict__ offsets, int G, int M, int NO, int C, int relu,
+                                                                  int band)
 {
-    typedef typename T::elem E;
-    __shared__ __attribute__((aligned(16))) char lds[lds_bytes_one<T, BM, BN>()];
+    typedef typename S::T T;
+    constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     int rt, ct;
     if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (NO + BN - 1) / BN, band, rt, ct)) return;
     const Segment s = row_tile(offsets, G, M, BM, rt);
@@ -37,22 +39,16 @@ __global__ __launch_bounds__(THREADS) void grouped_rows_kernel(const typename T:
     }
     const E *wg = W + (long long)s.g * NO * C;
     const E *xr = x + (long long)s.row0 * C;
-    typedef typename std::conditional<BACKWARD, Strided<T, BN>, Contiguous<T, BN>>::type LA;
-    LA a;
-    Contiguous<T, BM> b;
+    typename std::conditional<BACKWARD, Strided<T, BN, THREADS>, Contiguous<T, BN, THREADS>>::type a;
+    Contiguous<T, BM, THREADS> b;
     const E *wt = BACKWARD ? wg + n0 : wg + (long long)n0 * C;
     a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
     b.init(xr, C, s.rows, C, x + (long long)M * C);
-    constexpr int MI = BM / 32, NI = BN / 32;
-    typename T::acc acc[MI][NI];
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NI; ++n) acc[m][n] = typename T::acc{0, 0, 0, 0};
-    product<T, BM, BN>(a, b, C, lds, acc);
+    constexpr int MI = S::MI, NI = S::NI;
+    typename S::Acc acc = {};
+    product<S>(a, b, C, lds, acc);
 
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int ni0 = (wave & 1) * (BN / 2) + 4 * (lane >> 4), mi0 = (wave >> 1) * (BM / 2) + (lane & 15);
+    const int ni0 = S::col(), mi0 = S::row();
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
         const int r = mi0 + 16 * m;
@@ -94,13 +90,14 @@ __global__ __launch_bounds__(THREADS) void grouped_rows_kernel(const typename T:
 
 // ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
 // with S > 1 the shares go to `partial` (S, G, N, K) and grouped_weights_sum_kernel adds them in order.
-template <class T, int BM, int BN>
-__global__ __launch_bounds__(THREADS) void grouped_weights_kernel(const typename T::elem *__restrict__ gy, const typename T::elem *__restrict__ x,
-                                                                  typename T::elem *__restrict__ gW, float *__restrict__ partial,
-                                                                  const long long *__restrict__ offsets, int G, int M, int N, int K, int S)
+template <class S, class E = typename S::T::elem>
+__global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
+                                                                     float *__restrict__ partial, const long long *__restrict__ offsets, int G,
+                                                                     int M, int N, int K, int splits)
 {
-    typedef typename T::elem E;
-    __shared__ __attribute__((aligned(16))) char lds[lds_bytes_one<T, BM, BN>()];
+    typedef typename S::T T;
+    constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     // i (contiguous in the output) is k, j is n
     const int kt = (K + BN - 1) / BN, nt = (N + BM - 1) / BM;
     int id = blockIdx.x;
@@ -112,26 +109,21 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_kernel(const typename
     int row0, rows;
     group_rows(offsets, G, M, g, row0, rows);
     constexpr int STEP = T::BKC * 8;
-    const int share = ((rows + S - 1) / S + STEP - 1) / STEP * STEP;
+    const int share = ((rows + splits - 1) / splits + STEP - 1) / STEP * STEP;
     row0 += min(rows, split * share);
     rows = min(share, max(0, rows - split * share));
-    constexpr int MI = BM / 32, NI = BN / 32;
-    typename T::acc acc[MI][NI];
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NI; ++n) acc[m][n] = typename T::acc{0, 0, 0, 0};
+    constexpr int MI = S::MI, NI = S::NI;
+    typename S::Acc acc = {};
     const int ks = min(BN, K), ns = min(BM, N);
     const E *xt = x + (long long)row0 * K + k0, *yt = gy + (long long)row0 * N + n0;
     if (rows > 0) {
-        Strided<T, BN> a;
-        Strided<T, BM> b;
+        Strided<T, BN, THREADS> a;
+        Strided<T, BM, THREADS> b;
         a.init(xt, K, ks, rows, x + (long long)M * K);
         b.init(yt, N, ns, rows, gy + (long long)M * N);
-        product<T, BM, BN>(a, b, rows, lds, acc);
+        product<S>(a, b, rows, lds, acc);
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int ni0 = (wave & 1) * (BN / 2) + 4 * (lane >> 4), mi0 = (wave >> 1) * (BM / 2) + (lane & 15);
+    const int ni0 = S::col(), mi0 = S::row();
     const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
@@ -201,21 +193,40 @@ int check(const char *who, int M, int N, int K, int G, int dtype)
 
 int blocks_ok(const char *who, long long blocks)
 {
-    WM_REQUIRE(blocks <= (1ll << 32) / THREADS - 1, WM_ERR_UNSUPPORTED, "%s: %lld tiles are too many for one launch", who, blocks);
+    WM_REQUIRE(blocks <= (1ll << 32) / 512 - 1, WM_ERR_UNSUPPORTED, "%s: %lld tiles are too many for one launch", who, blocks);
     return WM_OK;
 }
 
-template <class T, int BM, int BN, bool BACKWARD>
+template <class S, bool BACKWARD>
 int rows_launch(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                 int C, int relu, hipStream_t st)
 {
-    typedef typename T::elem E;
-    const long long blocks = row_tiles_most(G, M, BM) * ((NO + BN - 1) / BN);
+    typedef typename S::T::elem E;
+    const long long blocks = row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN);
     if (int rc = blocks_ok("wm_dense_grouped", blocks)) return rc;
-    hipLaunchKernelGGL((grouped_rows_kernel<T, BM, BN, BACKWARD>), dim3((unsigned)blocks), dim3(THREADS), 0, st, (const E *)x, (const E *)W,
+    hipLaunchKernelGGL((grouped_rows_kernel<S, BACKWARD>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x, (const E *)W,
                        (const E *)bias, (const E *)mask, (E *)out, (const long long *)offsets, G, M, NO, C, relu, 8);
     WM_LAUNCH_CHECK("grouped_rows_kernel");
     return WM_OK;
+}
+
+template <class T> struct Tiles {                       // 16-bit types
+    typedef Shape<T, 256, 256, 2, 4> Large;
+    typedef Shape<T, 128, 128, 2, 2> Medium;
+};
+template <> struct Tiles<F32> {
+    typedef Shape<F32, 256, 128, 4, 2> Large;
+    typedef Shape<F32, 128, 128, 2, 2> Medium;
+};
+
+bool large(int G, int M, int N, int K) { (void)K; return M / G >= 512 && N >= 512; }
+
+template <class T, bool BACKWARD>
+int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
+               int C, int relu, hipStream_t st)
+{
+    if (large(G, M, NO, C)) return rows_launch<typename Tiles<T>::Large, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    return rows_launch<typename Tiles<T>::Medium, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
 template <bool BACKWARD>
@@ -223,9 +234,9 @@ int rows_any(int dtype, const void *x, const void *W, const void *bias, const vo
              int C, int relu, hipStream_t st)
 {
     switch (dtype) {
-    case WM_F32: return rows_launch<F32, 128, 128, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-    case WM_BF16: return rows_launch<BF16, 128, 128, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-    default: return rows_launch<F16, 128, 128, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    case WM_F32: return rows_typed<F32, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    case WM_BF16: return rows_typed<BF16, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    default: return rows_typed<F16, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
     }
 }
 
@@ -248,8 +259,16 @@ int weights_launch(const void *x, const void *gy, void *gW, void *gb, void *work
     const int S = weight_splits(M, N, K, G);
     const long long blocks = (long long)S * G * ((N + WB_TILE - 1) / WB_TILE) * ((K + WB_TILE - 1) / WB_TILE);
     if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
-    hipLaunchKernelGGL((grouped_weights_kernel<T, WB_TILE, WB_TILE>), dim3((unsigned)blocks), dim3(THREADS), 0, st, (const E *)gy, (const E *)x,
-                       (E *)gW, S > 1 ? (float *)workspace : nullptr, (const long long *)offsets, G, M, N, K, S);
+    if (large(1, N, K, M) && S == 1) {
+        typedef typename Tiles<T>::Large L;
+        const long long lb = (long long)G * ((N + L::BM - 1) / L::BM) * ((K + L::BN - 1) / L::BN);
+        hipLaunchKernelGGL((grouped_weights_kernel<L>), dim3((unsigned)lb), dim3(L::THREADS), 0, st, (const E *)gy, (const E *)x,
+                           (E *)gW, (float *)nullptr, (const long long *)offsets, G, M, N, K, S);
+    } else {
+        typedef typename Tiles<T>::Medium Md;
+        hipLaunchKernelGGL((grouped_weights_kernel<Md>), dim3((unsigned)blocks), dim3(Md::THREADS), 0, st, (const E *)gy, (const E *)x,
+                           (E *)gW, S > 1 ? (float *)workspace : nullptr, (const long long *)offsets, G, M, N, K, S);
+    }
     WM_LAUNCH_CHECK("grouped_weights_kernel");
     if (S > 1) {
         const long long count = (long long)G * N * K;

@@ -10,6 +10,8 @@ namespace {
 
 using namespace tile;
 
+constexpr int THREADS = 256;                 // of the kernels without tiles
+
 // One workgroup a row.  Codes go to q with row stride ldq >= K, zeros behind K.
 template <class E>
 __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restrict__ x, int K, int8_t *__restrict__ q, long long ldq,
@@ -45,13 +47,14 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restr
     if (threadIdx.x == 0) scale[m] = s;
 }
 
-template <class E, int BM, int BN>
-__global__ __launch_bounds__(THREADS) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
+template <class E, class S>
+__global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
                                                            const int8_t *__restrict__ W, const float *__restrict__ wscale,
                                                            const float *__restrict__ bias, E *__restrict__ y,
                                                            const long long *__restrict__ offsets, int G, int M, int N, int K, int relu, int band)
 {
-    __shared__ __attribute__((aligned(16))) char lds[lds_bytes_one<I8, BM, BN>()];
+    constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     int rt, ct;
     if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (N + BN - 1) / BN, band, rt, ct)) return;
     const Segment s = row_tile(offsets, G, M, BM, rt);
@@ -60,19 +63,14 @@ __global__ __launch_bounds__(THREADS) void dense_i8_kernel(const int8_t *__restr
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) y[(long long)(s.row0 + e / cols) * N + n0 + e % cols] = (E)0.0f;
         return;
     }
-    Contiguous<I8, BN> a;
-    Contiguous<I8, BM> b;
+    Contiguous<I8, BN, THREADS> a;
+    Contiguous<I8, BM, THREADS> b;
     a.init(W + ((long long)s.g * N + n0) * K, K, cols, K, W + (long long)G * N * K);
     b.init(q + s.row0 * ldq, ldq, s.rows, K, q + M * ldq);
-    constexpr int MI = BM / 32, NI = BN / 32;
-    i32x4 acc[MI][NI];
-#pragma unroll
-    for (int m = 0; m < MI; ++m)
-#pragma unroll
-        for (int n = 0; n < NI; ++n) acc[m][n] = i32x4{0, 0, 0, 0};
-    product<I8, BM, BN>(a, b, K, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int ni0 = (wave & 1) * (BN / 2) + 4 * (lane >> 4), mi0 = (wave >> 1) * (BM / 2) + (lane & 15);
+    constexpr int MI = S::MI, NI = S::NI;
+    typename S::Acc acc = {};
+    product<S>(a, b, K, lds, acc);
+    const int ni0 = S::col(), mi0 = S::row();
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
         const int r = mi0 + 16 * m;
@@ -118,6 +116,18 @@ template <class E> int quantize(const void *x, int M, int K, int8_t *q, long lon
     return WM_OK;
 }
 
+template <class E, class S>
+int dense_tiles(const int8_t *q, long long ldq, const float *scale, const int8_t *W, const float *wscale, const float *b, void *y,
+                const int64_t *offsets, int G, int M, int N, int K, int relu, hipStream_t st)
+{
+    const long long blocks = row_tiles_most(G, M, S::BM) * ((N + S::BN - 1) / S::BN);
+    WM_REQUIRE(blocks <= (1ll << 32) / 512 - 1, WM_ERR_UNSUPPORTED, "wm_dense_i8: %lld tiles are too many for one launch", blocks);
+    hipLaunchKernelGGL((dense_i8_kernel<E, S>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
+                       (const long long *)offsets, G, M, N, K, relu, 8);
+    WM_LAUNCH_CHECK("dense_i8_kernel");
+    return WM_OK;
+}
+
 template <class E>
 int dense(const void *x, const int8_t *W, const float *wscale, const float *b, void *y, const int64_t *offsets, int G, int M, int N, int K, int relu,
           void *workspace, hipStream_t st)
@@ -126,12 +136,8 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     int8_t *q = (int8_t *)workspace + wm_align_up((size_t)M * sizeof(float), 256);
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
-    const long long blocks = row_tiles_most(G, M, 128) * ((N + 127) / 128);
-    WM_REQUIRE(blocks <= (1ll << 32) / THREADS - 1, WM_ERR_UNSUPPORTED, "wm_dense_i8: %lld tiles are too many for one launch", blocks);
-    hipLaunchKernelGGL((dense_i8_kernel<E, 128, 128>), dim3((unsigned)blocks), dim3(THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
-                       (const long long *)offsets, G, M, N, K, relu, 8);
-    WM_LAUNCH_CHECK("dense_i8_kernel");
-    return WM_OK;
+    if (M / G >= 512 && N >= 512) return dense_tiles<E, Shape<I8, 256, 256, 2, 4>>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
 }
 
 }  // namespace

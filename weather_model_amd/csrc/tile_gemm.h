@@ -23,8 +23,6 @@
 
 namespace tile {
 
-constexpr int THREADS = 256;                 // four waves, 2 x 2 over the tile
-
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32u __attribute__((aligned(1)));
@@ -129,7 +127,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t out[3])
 }
 
 // ---- an operand with c along memory: rows of `ld` elements, ROWS of them a tile
-template <class T, int ROWS> struct Contiguous {
+template <class T, int ROWS, int THREADS> struct Contiguous {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * T::ECH, PER = ROWS * BKC / THREADS, LOADS = T::PLANES == 3 ? 2 : 1;
     static_assert(PER >= 1, "tile too small for the workgroup");
@@ -195,7 +193,7 @@ template <class T, int ROWS> struct Contiguous {
 };
 
 // ---- an operand with the tile's rows along memory: element (row r, c) at base + c * ld + r
-template <class T, int ROWS> struct Strided {
+template <class T, int ROWS, int THREADS> struct Strided {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * 8, BLOCKS = THREADS / BKC, W = ROWS / BLOCKS;   // W rows x 8 c a thread
     static constexpr int WORDS = W * sizeof(E) / 4, PER_WORD = 4 / sizeof(E);
@@ -281,75 +279,105 @@ template <class T, int ROWS> struct Strided {
     }
 };
 
-template <class T, int BM, int BN> constexpr int lds_bytes_one() { return (BM + BN) * T::BKC * 16 * T::PLANES; }
+// ---- a shape of tile: BM rows by BN columns of C over WM x WN waves
+template <class T_, int BM_, int BN_, int WM_, int WN_> struct Shape {
+    typedef T_ T;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
+    static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;             // 16 x 16 results a wave
+    static constexpr int A_BYTES = BN * T::BKC * 16 * T::PLANES, B_BYTES = BM * T::BKC * 16 * T::PLANES;
+    static constexpr int LDS = 2 * (A_BYTES + B_BYTES);                    // two steps
+    typedef typename T::acc Acc[MI][NI];
+    // where a lane's results lie: rows row() + 16 m, columns col() + 16 n .. + 3
+    static __device__ __forceinline__ int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM) + (int)(threadIdx.x & 15); }
+    static __device__ __forceinline__ int col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN) + 4 * ((int)(threadIdx.x & 63) >> 4); }
+};
 
 // ---- the core: acc[mi][ni] += A B^T over c = 0 .. count; A gives i (BN), B gives j (BM)
-template <class T, int BM, int BN>
-__device__ __forceinline__ void multiply(const char *la, const char *lb, typename T::acc (&acc)[BM / 32][BN / 32])
-{
-    constexpr int MI = BM / 32, NI = BN / 32, BKC = T::BKC, P = T::PLANES;
-    constexpr int A_PLANE = BN * BKC * 16, B_PLANE = BM * BKC * 16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int i0 = (wave & 1) * (BN / 2) + (lane & 15), j0 = (wave >> 1) * (BM / 2) + (lane & 15), g = lane >> 4;
-#pragma unroll
-    for (int s = 0; s < BKC / 4; ++s) {
-        u32x4 fa[P][NI], fb[P][MI];
+template <class S> struct Fragments {
+    typedef typename S::T T;
+    static constexpr int P = T::PLANES, BKC = T::BKC;
+    u32x4 a[P][S::NI], b[P][S::MI];
+    __device__ __forceinline__ void read(const char *lds, int s)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int i0 = wave % S::WN * (S::BN / S::WN) + (lane & 15), j0 = wave / S::WN * (S::BM / S::WM) + (lane & 15), q = 4 * s + (lane >> 4);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
 #pragma unroll
-            for (int n = 0; n < NI; ++n) fa[p][n] = *reinterpret_cast<const u32x4 *>(la + p * A_PLANE + lds_at<BKC>(i0 + 16 * n, 4 * s + g));
+            for (int n = 0; n < S::NI; ++n) a[p][n] = *reinterpret_cast<const u32x4 *>(lds + p * (S::BN * BKC * 16) + lds_at<BKC>(i0 + 16 * n, q));
 #pragma unroll
-            for (int m = 0; m < MI; ++m) fb[p][m] = *reinterpret_cast<const u32x4 *>(lb + p * B_PLANE + lds_at<BKC>(j0 + 16 * m, 4 * s + g));
+            for (int m = 0; m < S::MI; ++m)
+                b[p][m] = *reinterpret_cast<const u32x4 *>(lds + S::A_BYTES + p * (S::BM * BKC * 16) + lds_at<BKC>(j0 + 16 * m, q));
         }
+    }
+    __device__ __forceinline__ void multiply(typename S::Acc &acc) const
+    {
 #pragma unroll
-        for (int m = 0; m < MI; ++m)
+        for (int m = 0; m < S::MI; ++m)
 #pragma unroll
-            for (int n = 0; n < NI; ++n) {
+            for (int n = 0; n < S::NI; ++n) {
                 if constexpr (P == 1) {
-                    acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[0][n], b[0][m], acc[m][n]);
                 } else {                     // smallest first
-                    acc[m][n] = T::mma(fa[1][n], fb[1][m], acc[m][n]);
-                    acc[m][n] = T::mma(fa[2][n], fb[0][m], acc[m][n]);
-                    acc[m][n] = T::mma(fa[0][n], fb[2][m], acc[m][n]);
-                    acc[m][n] = T::mma(fa[1][n], fb[0][m], acc[m][n]);
-                    acc[m][n] = T::mma(fa[0][n], fb[1][m], acc[m][n]);
-                    acc[m][n] = T::mma(fa[0][n], fb[0][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[1][n], b[1][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[2][n], b[0][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[0][n], b[2][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[1][n], b[0][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[0][n], b[1][m], acc[m][n]);
+                    acc[m][n] = T::mma(a[0][n], b[0][m], acc[m][n]);
                 }
             }
     }
-}
+};
 
-// Whole steps: the next step's loads are in flight while this one is multiplied (the last step loads itself once
-// more instead of branching: a branch around the loads makes the compiler wait for them at its end).  What is left
-// of the last step goes through the guarded loads, which put zeros behind the end on both sides.
-template <class T, int BM, int BN, class LA, class LB>
-__device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename T::acc (&acc)[BM / 32][BN / 32])
+// Whole steps: while one is multiplied, the next goes from registers to the other half of LDS and the one after that is
+// loaded (the last steps load themselves once more instead of branching: a branch around the loads makes the
+// compiler wait for them at its end).  What is left of the last step goes through the guarded loads, which put zeros
+// behind the end on both sides.
+template <class S, class LA, class LB>
+__device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename S::Acc &acc)
 {
-    constexpr int STEP = LA::STEP;
+    constexpr int STEP = LA::STEP, SUB = S::T::BKC / 4, HALF = S::A_BYTES + S::B_BYTES;
     static_assert(LA::STEP == LB::STEP, "one step for both operands");
-    char *la = lds, *lb = lds + BN * T::BKC * 16 * T::PLANES;
     const int full = a.slow || b.slow ? 0 : count / STEP * STEP;
+    Fragments<S> f;
     if (full > 0) {
         a.load(0);
         b.load(0);
-        for (int c0 = STEP; c0 <= full; c0 += STEP) {
-            a.store(la);
-            b.store(lb);
-            __syncthreads();
-            const int next = min(c0, full - STEP);
+        a.store(lds);
+        b.store(lds + S::A_BYTES);
+        const int second = min(STEP, full - STEP);
+        a.load(second);
+        b.load(second);
+        __syncthreads();
+        int here = 0;
+        for (int c0 = 0; c0 < full; c0 += STEP) {
+            f.read(lds + here, 0);
+            here ^= HALF;
+            a.store(lds + here);
+            b.store(lds + here + S::A_BYTES);
+            const int next = min(c0 + 2 * STEP, full - STEP);
             a.load(next);
             b.load(next);
-            multiply<T, BM, BN>(la, lb, acc);
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+                if (s > 0) f.read(lds + (here ^ HALF), s);
+                f.multiply(acc);
+            }
             __syncthreads();
         }
     }
     for (int c0 = full; c0 < count; c0 += STEP) {
         a.load_guarded(c0);
         b.load_guarded(c0);
-        a.store(la);
-        b.store(lb);
+        a.store(lds);
+        b.store(lds + S::A_BYTES);
         __syncthreads();
-        multiply<T, BM, BN>(la, lb, acc);
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+            f.read(lds, s);
+            f.multiply(acc);
+        }
         __syncthreads();
     }
 }

@@ -987,11 +987,13 @@ def _out_any(out, shape, like, name):
 
 def _call(device, fn, *args):
     """``fn(*args, stream)`` on the current stream of ``device``, which is made current for the call."""
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, _stream()))
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)       # 0.1 us; the Stream object costs 2.7
+    if torch.cuda.current_device() == index:
+        _lib.check(fn(*args, stream))
     else:
         with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream()))
+            _lib.check(fn(*args, stream))
 
 
 def _grouped_args(x, weight, offsets):
@@ -1126,7 +1128,7 @@ def dropout_forward(x, p, seed, offset=0, residual=None, out=None):
         residual = _req_any(residual, "residual", x)
         if residual.shape != x.shape:
             raise ValueError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
-    y = _out_any(out, x.shape, x, "out")
+    y = torch.empty_like(x) if out is None else _out_any(out, x.shape, x, "out")
     _call(x.device, _lib.lib().wm_dropout, x.data_ptr(), 0 if residual is None else residual.data_ptr(),
           y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, seed, off, off_dev)
     return y
