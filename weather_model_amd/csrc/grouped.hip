@@ -5,7 +5,7 @@
 //             gW[g][n][k] = sum_{r of g} gy[r][n] x[r][k],   gb[g][n] = sum_{r of g} gy[r][n]
 // The number of rows of an expert is only known on the device, so a launch has as many workgroups as any
 // partition of M rows can need tiles, and each finds its tile from the offsets (tile_gemm.h).
-#include "tile_gemm.h"
+#include "few_rows.h"
 
 namespace {
 
@@ -89,10 +89,11 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
 }
 
 // ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
-// with S > 1 the shares go to `partial` (S, G, N, K) and grouped_weights_sum_kernel adds them in order.
+// with S > 1 the shares go to `partial` (S, G, N, K), and to (S, G, N) behind it, and grouped_weights_sum_kernel adds
+// them in order.  gb is summed by the workgroups of the first columns from the registers that feed LDS.
 template <class S, class E = typename S::T::elem>
 __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
-                                                                     float *__restrict__ partial, const long long *__restrict__ offsets, int G,
+                                                                     E *__restrict__ gb, float *__restrict__ partial, const long long *__restrict__ offsets, int G,
                                                                      int M, int N, int K, int splits)
 {
     typedef typename S::T T;
@@ -116,12 +117,19 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
     typename S::Acc acc = {};
     const int ks = min(BN, K), ns = min(BM, N);
     const E *xt = x + (long long)row0 * K + k0, *yt = gy + (long long)row0 * N + n0;
+    const bool sums = gb && k0 == 0;
+    float total = 0.0f;
     if (rows > 0) {
         Strided<T, BN, THREADS> a;
         Strided<T, BM, THREADS> b;
         a.init(xt, K, ks, rows, x + (long long)M * K);
         b.init(yt, N, ns, rows, gy + (long long)M * N);
-        product<S>(a, b, rows, lds, acc);
+        product<S, true>(a, b, rows, lds, acc, sums);
+        if (sums) total = b.total((float *)lds);
+    }
+    if (sums && (int)threadIdx.x < ns) {
+        if (partial) partial[(long long)splits * G * N * K + ((long long)split * G + g) * N + n0 + threadIdx.x] = total;
+        else gb[(long long)g * N + n0 + threadIdx.x] = from_float<E>(total);
     }
     const int ni0 = S::col(), mi0 = S::row();
     const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
@@ -155,30 +163,71 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
 }
 
 template <class E>
-__global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const float *__restrict__ partial, E *__restrict__ gW, long long count, int S)
+__global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const float *__restrict__ partial, E *__restrict__ gW, long long count,
+                                                                      E *__restrict__ gb, long long bcount, int S)
 {
-    for (long long e = (long long)blockIdx.x * THREADS + threadIdx.x; e < count; e += (long long)gridDim.x * THREADS) {
-        float s = partial[e];
-        for (int p = 1; p < S; ++p) s += partial[p * count + e];
-        gW[e] = from_float<E>(s);
+    const float *bias = partial + S * count;
+    for (long long e = (long long)blockIdx.x * THREADS + threadIdx.x; e < count + (gb ? bcount : 0); e += (long long)gridDim.x * THREADS) {
+        const bool w = e < count;
+        const float *p = w ? partial + e : bias + (e - count);
+        const long long step = w ? count : bcount;
+        float s = p[0];
+        for (int k = 1; k < S; ++k) s += p[k * step];
+        if (w) gW[e] = from_float<E>(s);
+        else gb[e - count] = from_float<E>(s);
     }
 }
 
-// ---- bias: gb[g][n], a workgroup per 64 columns of an expert; four waves take every fourth row
-template <class E>
-__global__ __launch_bounds__(THREADS) void grouped_bias_kernel(const E *__restrict__ gy, E *__restrict__ gb, const long long *__restrict__ offsets,
-                                                               int G, int M, int N)
+// ---- few rows: y (M, N) for groups of a handful of rows.  One read of the weights is the cost, so a workgroup takes 16
+// outputs of one expert, its waves share the contraction, and the MFMA operands come straight from memory.
+template <class T>
+__global__ __launch_bounds__(few::THREADS) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
+                                                                   const typename T::elem *__restrict__ bias, typename T::elem *__restrict__ y,
+                                                                   const long long *__restrict__ offsets, int G, int M, int N, int K, int relu)
 {
-    __shared__ float part[4][64];
-    const int g = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
+    typedef typename T::elem E;
+    __shared__ f32x4 part[few::WAVES][64];
+    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int row0, rows;
+    if (g == G) {                                    // rows of no expert: zeros
+        int end;
+        group_rows(offsets, G, M, 0, row0, rows);
+        group_rows(offsets, G, M, G - 1, end, rows);
+        end += rows;
+        const int cols = min(16, N - n0);
+        for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += few::THREADS) {
+            const int r = e / cols;
+            y[(long long)(r < row0 ? r : r - row0 + end) * N + n0 + e % cols] = (E)0.0f;
+        }
+        return;
+    }
     group_rows(offsets, G, M, g, row0, rows);
-    float s = 0.0f;
-    if (n < N)
-        for (int r = wave; r < rows; r += 4) s += to_float(gy[(long long)(row0 + r) * N + n]);
-    part[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && n < N) gb[(long long)g * N + n] = from_float<E>((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
+    const E *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+        const int r = min(r0 + (lane & 15), rows - 1);
+        const f32x4 acc = few::dot<T>(wrow, W + (long long)G * N * K, x + (long long)(row0 + r) * K, x + (long long)M * K, K);
+        if (wave > 0) part[wave][lane] = acc;
+        __syncthreads();
+        if (wave == 0) {
+            f32x4 v = acc;
+#pragma unroll
+            for (int w = 1; w < few::WAVES; ++w) v += part[w][lane];
+            const int n = n0 + 4 * (lane >> 4), have = min(4, N - n);
+            if (r0 + (lane & 15) < rows && have > 0) {
+                E *at = y + (long long)(row0 + r) * N + n;
+                const E *b = bias ? bias + (long long)g * N + n : nullptr;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (b && k < have) v[k] += to_float(b[k]);
+                    if (relu) v[k] = relu_of(v[k]);
+                }
+                if (have == 4) store4(at, v);
+                else
+                    for (int k = 0; k < have; ++k) at[k] = from_float<E>(v[k]);
+            }
+        }
+        __syncthreads();
+    }
 }
 
 int check(const char *who, int M, int N, int K, int G, int dtype)
@@ -229,6 +278,19 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
     return rows_launch<typename Tiles<T>::Medium, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
+// The few-rows kernel reads an expert's weights once for every 16 of its rows.
+bool few_rows(int G, int M) { return M <= 64 || M / G <= 8; }
+
+template <class T> int few_launch(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
+                                  int relu, hipStream_t st)
+{
+    typedef typename T::elem E;
+    hipLaunchKernelGGL(grouped_few_kernel<T>, dim3((N + 15) / 16, G + 1), dim3(few::THREADS), 0, st, (const E *)x, (const E *)W, (const E *)b,
+                       (E *)y, (const long long *)offsets, G, M, N, K, relu);
+    WM_LAUNCH_CHECK("grouped_few_kernel");
+    return WM_OK;
+}
+
 template <bool BACKWARD>
 int rows_any(int dtype, const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
              int C, int relu, hipStream_t st)
@@ -263,24 +325,20 @@ int weights_launch(const void *x, const void *gy, void *gW, void *gb, void *work
         typedef typename Tiles<T>::Large L;
         const long long lb = (long long)G * ((N + L::BM - 1) / L::BM) * ((K + L::BN - 1) / L::BN);
         hipLaunchKernelGGL((grouped_weights_kernel<L>), dim3((unsigned)lb), dim3(L::THREADS), 0, st, (const E *)gy, (const E *)x,
-                           (E *)gW, (float *)nullptr, (const long long *)offsets, G, M, N, K, S);
+                           (E *)gW, (E *)gb, (float *)nullptr, (const long long *)offsets, G, M, N, K, S);
     } else {
         typedef typename Tiles<T>::Medium Md;
         hipLaunchKernelGGL((grouped_weights_kernel<Md>), dim3((unsigned)blocks), dim3(Md::THREADS), 0, st, (const E *)gy, (const E *)x,
-                           (E *)gW, S > 1 ? (float *)workspace : nullptr, (const long long *)offsets, G, M, N, K, S);
+                           (E *)gW, (E *)gb, S > 1 ? (float *)workspace : nullptr, (const long long *)offsets, G, M, N, K, S);
     }
     WM_LAUNCH_CHECK("grouped_weights_kernel");
     if (S > 1) {
         const long long count = (long long)G * N * K;
         long long grid = (count + THREADS - 1) / THREADS;
         if (grid > 4096) grid = 4096;
-        hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid), dim3(THREADS), 0, st, (const float *)workspace, (E *)gW, count, S);
+        hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid), dim3(THREADS), 0, st, (const float *)workspace, (E *)gW, count,
+                           (E *)gb, (long long)G * N, S);
         WM_LAUNCH_CHECK("grouped_weights_sum_kernel");
-    }
-    if (gb) {
-        hipLaunchKernelGGL(grouped_bias_kernel<E>, dim3((N + 63) / 64, G), dim3(THREADS), 0, st, (const E *)gy, (E *)gb,
-                           (const long long *)offsets, G, M, N);
-        WM_LAUNCH_CHECK("grouped_bias_kernel");
     }
     return WM_OK;
 }
@@ -293,6 +351,14 @@ extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b,
     if (int rc = check("wm_dense_grouped_fwd", M, N, K, G, dtype)) return rc;
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
+    if (few_rows(G, M) && G < 65535) {
+        hipStream_t st = (hipStream_t)stream;
+        switch (dtype) {
+        case WM_F32: return few_launch<F32>(x, W, b, y, offsets, G, M, N, K, relu, st);
+        case WM_BF16: return few_launch<BF16>(x, W, b, y, offsets, G, M, N, K, relu, st);
+        default: return few_launch<F16>(x, W, b, y, offsets, G, M, N, K, relu, st);
+        }
+    }
     return rows_any<false>(dtype, x, W, b, nullptr, y, offsets, G, M, N, K, relu, (hipStream_t)stream);
 }
 
@@ -309,7 +375,7 @@ extern "C" size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, i
 {
     if (M < 0 || N <= 0 || K <= 0 || G <= 0) return 0;
     const int S = weight_splits(M, N, K, G);
-    return S > 1 ? wm_align_up((size_t)S * G * N * K * sizeof(float), 256) : 0;
+    return S > 1 ? wm_align_up((size_t)S * G * N * (K + 1) * sizeof(float), 256) : 0;
 }
 
 extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, void *workspace, size_t workspace_bytes,

@@ -4,7 +4,7 @@
 // The integer sum is exact (K <= 2^17 keeps it within 32 bits, -128 among the codes included); it is rounded
 // to float32 once and scaled there.  A row of zeros has s = 0 and codes 0; a row that holds an infinity or a
 // NaN has s = NaN and codes 0, so that all its outputs are NaN.
-#include "tile_gemm.h"
+#include "few_rows.h"
 
 namespace {
 
@@ -97,6 +97,60 @@ __global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__re
     }
 }
 
+// ---- few rows: one read of the weights (few_rows.h)
+template <class E>
+__global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
+                                                                    const int8_t *__restrict__ W, const float *__restrict__ wscale,
+                                                                    const float *__restrict__ bias, E *__restrict__ y,
+                                                                    const long long *__restrict__ offsets, int G, int M, int N, int K, int relu)
+{
+    __shared__ i32x4 part[few::WAVES][64];
+    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int row0 = 0, rows = M;
+    if (g == G) {                                    // rows of no expert: zeros
+        int end;
+        group_rows(offsets, G, M, 0, row0, rows);
+        group_rows(offsets, G, M, G - 1, end, rows);
+        end += rows;
+        const int cols = min(16, N - n0);
+        for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += few::THREADS) {
+            const int r = e / cols;
+            y[(long long)(r < row0 ? r : r - row0 + end) * N + n0 + e % cols] = (E)0.0f;
+        }
+        return;
+    }
+    if (offsets) group_rows(offsets, G, M, g, row0, rows);
+    const int8_t *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
+    for (int r0 = 0; r0 < rows; r0 += 16) {
+        const int r = min(r0 + (lane & 15), rows - 1);
+        const i32x4 acc = few::dot<I8>(wrow, W + (long long)G * N * K, q + (row0 + r) * ldq, q + M * ldq, K);
+        if (wave > 0) part[wave][lane] = acc;
+        __syncthreads();
+        if (wave == 0) {
+            i32x4 s = acc;
+#pragma unroll
+            for (int w = 1; w < few::WAVES; ++w) s += part[w][lane];
+            const int n = n0 + 4 * (lane >> 4), have = min(4, N - n);
+            if (r0 + (lane & 15) < rows && have > 0) {
+                E *at = y + (long long)(row0 + r) * N + n;
+                const float qs = qscale[row0 + r];
+                const long long c = (long long)g * N + n;
+                f32x4 v;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int kk = min(k, have - 1);
+                    v[k] = (float)s[k] * qs * wscale[c + kk] + (bias ? bias[c + kk] : 0.0f);
+                    if (relu) v[k] = relu_of(v[k]);
+                }
+                if (have == 4) store4(at, v);
+                else
+                    for (int k = 0; k < have; ++k) at[k] = from_float<E>(v[k]);
+            }
+        }
+        __syncthreads();
+    }
+}
+
 size_t padded(int K) { return wm_align_up((size_t)K, 128); }
 
 int check(const char *who, int M, int K, int dtype)
@@ -136,6 +190,12 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     int8_t *q = (int8_t *)workspace + wm_align_up((size_t)M * sizeof(float), 256);
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
+    if ((M <= 64 || M / G <= 8) && G < 65535) {
+        hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, q, ldq, scale, W, wscale, b,
+                           (E *)y, (const long long *)offsets, G, M, N, K, relu);
+        WM_LAUNCH_CHECK("dense_i8_few_kernel");
+        return WM_OK;
+    }
     if (M / G >= 512 && N >= 512) return dense_tiles<E, Shape<I8, 256, 256, 2, 4>>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
     return dense_tiles<E, Shape<I8, 128, 128, 2, 2>>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
 }

@@ -203,6 +203,7 @@ template <class T, int ROWS, int THREADS> struct Strided {
     const E *base;
     long long ld;
     int r0, q, count;
+    float sum[W];                            // of what add_up() saw
     int most;                                // rows that exist, at least 1
     bool slow;                               // fewer rows than a thread's vector: load() does not fit (workgroup-uniform)
 
@@ -214,6 +215,8 @@ template <class T, int ROWS, int THREADS> struct Strided {
         q = threadIdx.x / BLOCKS;
         most = rows_left;
         slow = rows_left < W;
+#pragma unroll
+        for (int i = 0; i < W; ++i) sum[i] = 0.0f;
         // a vector that would leave the rows moves back into them: two threads then write the same values to the
         // same place, and rows that do not exist keep whatever LDS held (their results are not stored)
         r0 = slow ? 0 : min((int)(threadIdx.x % BLOCKS) * W, rows_left - W);
@@ -250,6 +253,29 @@ template <class T, int ROWS, int THREADS> struct Strided {
                     }
                 reg[e][w] = v;
             }
+    }
+    // adds what the registers hold to the sums of this thread's rows over c
+    __device__ __forceinline__ void add_up()
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if constexpr (sizeof(E) == 4) sum[i] += __builtin_bit_cast(float, reg[e][i]);
+                else sum[i] += to_float(__builtin_bit_cast(E, (uint16_t)(reg[e][i / 2] >> (16 * (i & 1)))));
+            }
+    }
+    // the sums over all c, in a fixed order: LDS holds BKC x ROWS floats; returns that of row threadIdx.x < ROWS
+    __device__ __forceinline__ float total(float *lds)
+    {
+#pragma unroll
+        for (int i = 0; i < W; ++i) lds[q * ROWS + r0 + i] = sum[i];
+        __syncthreads();
+        float s = 0.0f;
+        if (threadIdx.x < ROWS)
+#pragma unroll
+            for (int k = 0; k < BKC; ++k) s += lds[k * ROWS + threadIdx.x];
+        return s;
     }
     __device__ __forceinline__ void store(char *lds)
     {
@@ -334,8 +360,9 @@ template <class S> struct Fragments {
 // loaded (the last steps load themselves once more instead of branching: a branch around the loads makes the
 // compiler wait for them at its end).  What is left of the last step goes through the guarded loads, which put zeros
 // behind the end on both sides.
-template <class S, class LA, class LB>
-__device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename S::Acc &acc)
+// `sums`: add up B's rows over c as well (a Strided operand; workgroup-uniform).
+template <class S, bool SUMS = false, class LA, class LB>
+__device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename S::Acc &acc, bool sums = false)
 {
     constexpr int STEP = LA::STEP, SUB = S::T::BKC / 4, HALF = S::A_BYTES + S::B_BYTES;
     static_assert(LA::STEP == LB::STEP, "one step for both operands");
@@ -346,6 +373,8 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
         b.load(0);
         a.store(lds);
         b.store(lds + S::A_BYTES);
+        if constexpr (SUMS)
+            if (sums) b.add_up();
         const int second = min(STEP, full - STEP);
         a.load(second);
         b.load(second);
@@ -356,6 +385,8 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
             here ^= HALF;
             a.store(lds + here);
             b.store(lds + here + S::A_BYTES);
+            if constexpr (SUMS)
+                if (sums && c0 + STEP < full) b.add_up();
             const int next = min(c0 + 2 * STEP, full - STEP);
             a.load(next);
             b.load(next);
@@ -370,6 +401,8 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
     for (int c0 = full; c0 < count; c0 += STEP) {
         a.load_guarded(c0);
         b.load_guarded(c0);
+        if constexpr (SUMS)
+            if (sums) b.add_up();
         a.store(lds);
         b.store(lds + S::A_BYTES);
         __syncthreads();
