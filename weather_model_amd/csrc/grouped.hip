@@ -5,6 +5,7 @@
 //             gW[g][n][k] = sum_{r of g} gy[r][n] x[r][k],   gb[g][n] = sum_{r of g} gy[r][n]
 // The number of rows of an expert is only known on the device, so a launch has as many workgroups as any
 // partition of M rows can need tiles, and each finds its tile from the offsets (tile_gemm.h).
+#include "direct_gemm.h"
 #include "few_rows.h"
 
 namespace {
@@ -20,7 +21,7 @@ template <class T> __device__ __forceinline__ f32x4 load4_f32(const T *p)
 
 // ---- rows: out (M, NO) = x (M, C) times W[g], forward (W[g] is (NO, C), its c along memory) or backward
 // (W[g] is (C, NO)).  bias and relu are the forward's, mask the backward's.
-template <class S, bool BACKWARD, class E = typename S::T::elem>
+template <class S, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
 __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
                                                                   const E *__restrict__ mask, E *__restrict__ out,
                                                                   const long long *__restrict__ offsets, int G, int M, int NO, int C, int relu,
@@ -39,14 +40,22 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
     }
     const E *wg = W + (long long)s.g * NO * C;
     const E *xr = x + (long long)s.row0 * C;
-    typename std::conditional<BACKWARD, Strided<T, BN, THREADS>, Contiguous<T, BN, THREADS>>::type a;
-    Contiguous<T, BM, THREADS> b;
     const E *wt = BACKWARD ? wg + n0 : wg + (long long)n0 * C;
-    a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
-    b.init(xr, C, s.rows, C, x + (long long)M * C);
     constexpr int MI = S::MI, NI = S::NI;
     typename S::Acc acc = {};
-    product<S>(a, b, C, lds, acc);
+    if constexpr (DIRECT) {
+        typename std::conditional<BACKWARD, DirectCols<T, BN, THREADS>, DirectRows<T, BN, THREADS>>::type a;
+        DirectRows<T, BM, THREADS> b;
+        a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
+        b.init(xr, C, s.rows, C, x + (long long)M * C);
+        product_direct<S>(a, b, C, lds, acc);
+    } else {
+        typename std::conditional<BACKWARD, Strided<T, BN, THREADS>, Contiguous<T, BN, THREADS>>::type a;
+        Contiguous<T, BM, THREADS> b;
+        a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
+        b.init(xr, C, s.rows, C, x + (long long)M * C);
+        product<S>(a, b, C, lds, acc);
+    }
 
     const int ni0 = S::col(), mi0 = S::row();
 #pragma unroll
@@ -91,7 +100,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
 // ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
 // with S > 1 the shares go to `partial` (S, G, N, K), and to (S, G, N) behind it, and grouped_weights_sum_kernel adds
 // them in order.  gb is summed by the workgroups of the first columns from the registers that feed LDS.
-template <class S, class E = typename S::T::elem>
+template <class S, bool DIRECT, class E = typename S::T::elem>
 __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
                                                                      E *__restrict__ gb, float *__restrict__ partial, const long long *__restrict__ offsets, int G,
                                                                      int M, int N, int K, int splits)
@@ -118,18 +127,36 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
     const int ks = min(BN, K), ns = min(BM, N);
     const E *xt = x + (long long)row0 * K + k0, *yt = gy + (long long)row0 * N + n0;
     const bool sums = gb && k0 == 0;
-    float total = 0.0f;
-    if (rows > 0) {
-        Strided<T, BN, THREADS> a;
-        Strided<T, BM, THREADS> b;
-        a.init(xt, K, ks, rows, x + (long long)M * K);
-        b.init(yt, N, ns, rows, gy + (long long)M * N);
-        product<S, true>(a, b, rows, lds, acc, sums);
-        if (sums) total = b.total((float *)lds);
-    }
-    if (sums && (int)threadIdx.x < ns) {
-        if (partial) partial[(long long)splits * G * N * K + ((long long)split * G + g) * N + n0 + threadIdx.x] = total;
-        else gb[(long long)g * N + n0 + threadIdx.x] = from_float<E>(total);
+    auto bias = [&](int j, float v) {
+        if (j >= ns) return;
+        if (partial) partial[(long long)splits * G * N * K + ((long long)split * G + g) * N + n0 + j] = v;
+        else gb[(long long)g * N + n0 + j] = from_float<E>(v);
+    };
+    if constexpr (DIRECT) {
+        float sum[MI] = {};
+        if (rows > 0) {
+            DirectCols<T, BN, THREADS> a;
+            DirectCols<T, BM, THREADS> b;
+            a.init(xt, K, ks, rows, nullptr);
+            b.init(yt, N, ns, rows, nullptr);
+            // the sums cost registers and branches: their own code
+            if (sums) product_direct<S, true>(a, b, rows, lds, acc, S::wave_col() == 0, sum);
+            else product_direct<S>(a, b, rows, lds, acc);
+        }
+        if (sums && S::wave_col() == 0 && (threadIdx.x & 63) < 16)
+#pragma unroll
+            for (int m = 0; m < MI; ++m) bias(S::row() + 16 * m, sum[m]);
+    } else {
+        float total = 0.0f;
+        if (rows > 0) {
+            Strided<T, BN, THREADS> a;
+            Strided<T, BM, THREADS> b;
+            a.init(xt, K, ks, rows, x + (long long)M * K);
+            b.init(yt, N, ns, rows, gy + (long long)M * N);
+            product<S, true>(a, b, rows, lds, acc, sums);
+            if (sums) total = b.total((float *)lds);
+        }
+        if (sums) bias(threadIdx.x, total);
     }
     const int ni0 = S::col(), mi0 = S::row();
     const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
@@ -246,14 +273,14 @@ int blocks_ok(const char *who, long long blocks)
     return WM_OK;
 }
 
-template <class S, bool BACKWARD>
+template <class S, bool BACKWARD, bool DIRECT>
 int rows_launch(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                 int C, int relu, hipStream_t st)
 {
     typedef typename S::T::elem E;
     const long long blocks = row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN);
     if (int rc = blocks_ok("wm_dense_grouped", blocks)) return rc;
-    hipLaunchKernelGGL((grouped_rows_kernel<S, BACKWARD>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x, (const E *)W,
+    hipLaunchKernelGGL((grouped_rows_kernel<S, BACKWARD, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x, (const E *)W,
                        (const E *)bias, (const E *)mask, (E *)out, (const long long *)offsets, G, M, NO, C, relu, 8);
     WM_LAUNCH_CHECK("grouped_rows_kernel");
     return WM_OK;
@@ -274,8 +301,15 @@ template <class T, bool BACKWARD>
 int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                int C, int relu, hipStream_t st)
 {
-    if (large(G, M, NO, C)) return rows_launch<typename Tiles<T>::Large, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-    return rows_launch<typename Tiles<T>::Medium, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    typedef typename Tiles<T>::Large L;
+    typedef typename Tiles<T>::Medium Md;
+    if constexpr (T::PLANES == 1) {
+        if (direct_ok(x, 2ll * C) && direct_ok(W, BACKWARD ? 2ll * NO : 2ll * C)) {
+            if (large(G, M, NO, C)) return rows_launch<L, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+            return rows_launch<Md, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+        }
+    } else if (large(G, M, NO, C)) return rows_launch<L, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    return rows_launch<Md, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows.
@@ -321,16 +355,24 @@ int weights_launch(const void *x, const void *gy, void *gW, void *gb, void *work
     const int S = weight_splits(M, N, K, G);
     const long long blocks = (long long)S * G * ((N + WB_TILE - 1) / WB_TILE) * ((K + WB_TILE - 1) / WB_TILE);
     if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
-    if (large(1, N, K, M) && S == 1) {
-        typedef typename Tiles<T>::Large L;
-        const long long lb = (long long)G * ((N + L::BM - 1) / L::BM) * ((K + L::BN - 1) / L::BN);
-        hipLaunchKernelGGL((grouped_weights_kernel<L>), dim3((unsigned)lb), dim3(L::THREADS), 0, st, (const E *)gy, (const E *)x,
-                           (E *)gW, (E *)gb, (float *)nullptr, (const long long *)offsets, G, M, N, K, S);
+    float *partial = S > 1 ? (float *)workspace : nullptr;
+    typedef typename Tiles<T>::Large L;
+    typedef typename Tiles<T>::Medium Md;
+    const bool big = large(1, N, K, M) && S == 1;
+    const long long lb = (long long)G * ((N + L::BM - 1) / L::BM) * ((K + L::BN - 1) / L::BN);
+#define WM_WEIGHTS(SHAPE, DIRECT, BLOCKS)                                                                                              \
+    hipLaunchKernelGGL((grouped_weights_kernel<SHAPE, DIRECT>), dim3((unsigned)(BLOCKS)), dim3(SHAPE::THREADS), 0, st, (const E *)gy, \
+                       (const E *)x, (E *)gW, (E *)gb, partial, (const long long *)offsets, G, M, N, K, S)
+    if constexpr (T::PLANES == 1) {
+        const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N);
+        if (direct && big) WM_WEIGHTS(L, true, lb);
+        else if (direct) WM_WEIGHTS(Md, true, blocks);
+        else WM_WEIGHTS(Md, false, blocks);
     } else {
-        typedef typename Tiles<T>::Medium Md;
-        hipLaunchKernelGGL((grouped_weights_kernel<Md>), dim3((unsigned)blocks), dim3(Md::THREADS), 0, st, (const E *)gy, (const E *)x,
-                           (E *)gW, (E *)gb, S > 1 ? (float *)workspace : nullptr, (const long long *)offsets, G, M, N, K, S);
+        if (big) WM_WEIGHTS(L, false, lb);
+        else WM_WEIGHTS(Md, false, blocks);
     }
+#undef WM_WEIGHTS
     WM_LAUNCH_CHECK("grouped_weights_kernel");
     if (S > 1) {
         const long long count = (long long)G * N * K;

@@ -7,8 +7,6 @@
 // LDS holds both operands as [row][c], `BKC` chunks of 16 bytes a row, whatever their layout in memory:
 //   contiguous  c runs along memory: a chunk is one 16-byte load (two for float32)
 //   strided     i (or j) runs along memory: a thread loads 8 c of a few rows and transposes in registers
-// and the chunk at position q of row r lies in slot q ^ swz(r), so that the 16 rows of an MFMA operand, the
-// 8 rows a loader's wave writes, and the 8-row steps of a transposed write all spread over the banks.
 //
 // float32 is split into three bf16 pieces, x = h + m + l (each the nearest to what is left: 24 bits), and a
 // product is the six piece products that are not below 2^-24 of it: hh, hm, mh, hl, lh, mm, each exact in the
@@ -69,12 +67,16 @@ struct I8 {
 // max(v, 0) that keeps a NaN
 __device__ __forceinline__ float relu_of(float v) { return v < 0.0f ? 0.0f : v; }
 
-template <int BKC> __device__ __forceinline__ int swz(int row)
+// Byte address of chunk q of a row.  A line of 128 bytes is one row of eight chunks or two of four; the slot of a chunk
+// in its line is exclusive-ored with the row, so that the 8 rows that a step of an MFMA operand's read touches, and the
+// chunks that a step of a loader's write brings, lie in different banks.  16 rows on, the slots are the same again:
+// an operand's other rows are immediate offsets.
+template <int BKC> __device__ __forceinline__ int lds_at(int row, int q)
 {
-    return BKC == 8 ? (row ^ (row >> 3)) & 7 : ((row >> 1) ^ (row >> 3)) & 3;
+    if constexpr (BKC == 8) return row * 128 + ((q ^ (row & 7)) << 4);
+    const int p = row >> 1, h = (p & 3) | (((p ^ (p >> 1)) & 1) << 2);
+    return p * 128 + (((((row & 1) << 2) | q) ^ h) << 4);
 }
-// byte address of chunk q of a row
-template <int BKC> __device__ __forceinline__ int lds_at(int row, int q) { return row * (16 * BKC) + ((q ^ swz<BKC>(row)) << 4); }
 
 // ---- global loads
 // 16 bytes at p of which `avail` elements count; the rest read as zero.  Nothing at or beyond `end` is read.
@@ -130,6 +132,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t out[3])
 template <class T, int ROWS, int THREADS> struct Contiguous {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * T::ECH, PER = ROWS * BKC / THREADS, LOADS = T::PLANES == 3 ? 2 : 1;
+    static constexpr int N_LOADS = PER * LOADS, N_STORES = PER * T::PLANES;      // instructions of load() and store()
     static_assert(PER >= 1, "tile too small for the workgroup");
     u32x4 reg[PER][LOADS];
     const E *base, *end;                     // (row 0 of the tile, c = 0) and the end of the tensor
@@ -197,6 +200,7 @@ template <class T, int ROWS, int THREADS> struct Strided {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * 8, BLOCKS = THREADS / BKC, W = ROWS / BLOCKS;   // W rows x 8 c a thread
     static constexpr int WORDS = W * sizeof(E) / 4, PER_WORD = 4 / sizeof(E);
+    static constexpr int N_LOADS = 8, N_STORES = W * T::PLANES;
     static_assert(WORDS >= 1 && T::ECH == 8, "tile too small for the workgroup");
     typedef uint32_t words __attribute__((ext_vector_type(WORDS), aligned(sizeof(E))));
     uint32_t reg[8][WORDS];
@@ -212,21 +216,21 @@ template <class T, int ROWS, int THREADS> struct Strided {
         base = tensor_row0;
         ld = ld_;
         count = c_count;
-        q = threadIdx.x / BLOCKS;
+        q = threadIdx.x % BKC;
         most = rows_left;
         slow = rows_left < W;
 #pragma unroll
         for (int i = 0; i < W; ++i) sum[i] = 0.0f;
         // a vector that would leave the rows moves back into them: two threads then write the same values to the
         // same place, and rows that do not exist keep whatever LDS held (their results are not stored)
-        r0 = slow ? 0 : min((int)(threadIdx.x % BLOCKS) * W, rows_left - W);
+        r0 = slow ? 0 : min((int)(threadIdx.x / BKC) * W, rows_left - W);
     }
     __device__ __forceinline__ void load(int c0)
     {
         const E *at = base + (long long)c0 * ld;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const E *p = at + (uint32_t)((q * 8 + e) * (int)ld + r0);
+            const E *p = at + e * ld + (uint32_t)(q * 8 * (int)ld + r0);       // scalar base, one offset register
             if constexpr (WORDS == 1) {
                 reg[e][0] = *reinterpret_cast<const u32u *>(p);
             } else {
@@ -316,24 +320,27 @@ template <class T_, int BM_, int BN_, int WM_, int WN_> struct Shape {
     // where a lane's results lie: rows row() + 16 m, columns col() + 16 n .. + 3
     static __device__ __forceinline__ int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM) + (int)(threadIdx.x & 15); }
     static __device__ __forceinline__ int col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN) + 4 * ((int)(threadIdx.x & 63) >> 4); }
+    static __device__ __forceinline__ int wave_col() { return (int)(threadIdx.x >> 6) % WN; }
 };
 
 // ---- the core: acc[mi][ni] += A B^T over c = 0 .. count; A gives i (BN), B gives j (BM)
 template <class S> struct Fragments {
     typedef typename S::T T;
     static constexpr int P = T::PLANES, BKC = T::BKC;
+    static constexpr int N_READS = P * (S::NI + S::MI), N_MFMA = S::NI * S::MI * (P == 1 ? 1 : 6);
     u32x4 a[P][S::NI], b[P][S::MI];
+    // chunks 4 s .. 4 s + 3 of the rows of this lane's operands
     __device__ __forceinline__ void read(const char *lds, int s)
     {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int i0 = wave % S::WN * (S::BN / S::WN) + (lane & 15), j0 = wave / S::WN * (S::BM / S::WM) + (lane & 15), q = 4 * s + (lane >> 4);
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = 4 * s + (lane >> 4);
+        const char *pa = lds + wave % S::WN * (S::BN / S::WN * BKC * 16) + lds_at<BKC>(lane & 15, q);
+        const char *pb = lds + S::A_BYTES + wave / S::WN * (S::BM / S::WM * BKC * 16) + lds_at<BKC>(lane & 15, q);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
 #pragma unroll
-            for (int n = 0; n < S::NI; ++n) a[p][n] = *reinterpret_cast<const u32x4 *>(lds + p * (S::BN * BKC * 16) + lds_at<BKC>(i0 + 16 * n, q));
+            for (int n = 0; n < S::NI; ++n) a[p][n] = *reinterpret_cast<const u32x4 *>(pa + (p * S::BN + 16 * n) * (BKC * 16));
 #pragma unroll
-            for (int m = 0; m < S::MI; ++m)
-                b[p][m] = *reinterpret_cast<const u32x4 *>(lds + S::A_BYTES + p * (S::BM * BKC * 16) + lds_at<BKC>(j0 + 16 * m, q));
+            for (int m = 0; m < S::MI; ++m) b[p][m] = *reinterpret_cast<const u32x4 *>(pb + (p * S::BM + 16 * m) * (BKC * 16));
         }
     }
     __device__ __forceinline__ void multiply(typename S::Acc &acc) const
@@ -356,10 +363,28 @@ template <class S> struct Fragments {
     }
 };
 
-// Whole steps: while one is multiplied, the next goes from registers to the other half of LDS and the one after that is
-// loaded (the last steps load themselves once more instead of branching: a branch around the loads makes the
-// compiler wait for them at its end).  What is left of the last step goes through the guarded loads, which put zeros
-// behind the end on both sides.
+// Scheduling of one multiplication: each instruction of the other kinds is issued behind its share of matrix
+// instructions, so that the matrix unit never waits for a run of them.
+template <int MFMA, int READS, int STORES, int LOADS> __device__ __forceinline__ void interleave()
+{
+    // the last quarter of the matrix instructions covers the latency of the last read
+    constexpr int OTHERS = READS + STORES + LOADS, BEHIND = MFMA * 3 / 4, EACH = OTHERS ? BEHIND / OTHERS : 0, MORE = OTHERS ? BEHIND % OTHERS : 0;
+#pragma unroll
+    for (int k = 0; k < OTHERS; ++k) {
+        if (k < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        else if (k < READS + STORES) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+        else __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+        if (k < MORE) __builtin_amdgcn_sched_group_barrier(0x8, EACH + 1, 0);
+        else if (EACH > 0) __builtin_amdgcn_sched_group_barrier(0x8, EACH, 0);
+    }
+}
+
+// Whole steps, each of SUB reads of operands: while one step is multiplied, the next goes from registers to the other
+// half of LDS and the one after that is loaded (the last steps load themselves once more instead of branching: a
+// branch around the loads makes the compiler wait for them at its end).  There is one barrier a step, before its last
+// multiplication: behind it the next step lies in LDS, so that its first operands are read under that multiplication, and
+// every wave has read the last of this step's, so that its half may be overwritten.  What is left of the last step goes through the
+// guarded loads, which put zeros behind the end on both sides.
 // `sums`: add up B's rows over c as well (a Strided operand; workgroup-uniform).
 template <class S, bool SUMS = false, class LA, class LB>
 __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename S::Acc &acc, bool sums = false)
@@ -367,8 +392,8 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
     constexpr int STEP = LA::STEP, SUB = S::T::BKC / 4, HALF = S::A_BYTES + S::B_BYTES;
     static_assert(LA::STEP == LB::STEP, "one step for both operands");
     const int full = a.slow || b.slow ? 0 : count / STEP * STEP;
-    Fragments<S> f;
     if (full > 0) {
+        Fragments<S> f[2];
         a.load(0);
         b.load(0);
         a.store(lds);
@@ -380,25 +405,34 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
         b.load(second);
         __syncthreads();
         int here = 0;
+        if constexpr (SUB == 2) f[0].read(lds, 0);
         for (int c0 = 0; c0 < full; c0 += STEP) {
-            f.read(lds + here, 0);
-            here ^= HALF;
-            a.store(lds + here);
-            b.store(lds + here + S::A_BYTES);
+            const int there = HALF - here;
+            f[1].read(lds + here, SUB - 1);
+            a.store(lds + there);
+            b.store(lds + there + S::A_BYTES);
             if constexpr (SUMS)
                 if (sums && c0 + STEP < full) b.add_up();
             const int next = min(c0 + 2 * STEP, full - STEP);
             a.load(next);
             b.load(next);
-#pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-                if (s > 0) f.read(lds + (here ^ HALF), s);
-                f.multiply(acc);
+            if constexpr (SUB == 2) {
+                f[0].multiply(acc);
+                interleave<Fragments<S>::N_MFMA, Fragments<S>::N_READS, LA::N_STORES + LB::N_STORES, LA::N_LOADS + LB::N_LOADS>();
+                __syncthreads();
+                f[0].read(lds + there, 0);
+                f[1].multiply(acc);
+                interleave<Fragments<S>::N_MFMA, Fragments<S>::N_READS, 0, 0>();
+            } else {
+                f[1].multiply(acc);
+                __syncthreads();
             }
-            __syncthreads();
+            here = there;
         }
+        __syncthreads();
     }
     for (int c0 = full; c0 < count; c0 += STEP) {
+        Fragments<S> f;
         a.load_guarded(c0);
         b.load_guarded(c0);
         if constexpr (SUMS)
@@ -448,6 +482,9 @@ __device__ __forceinline__ void segment_bounds(const long long *offsets, int G, 
     if ((threadIdx.x & 63) == 0) lo = carry;
 }
 
+// a lane's value, in a scalar register
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
 __device__ __forceinline__ int wave_scan(int v)          // inclusive
 {
 #pragma unroll
@@ -464,8 +501,8 @@ __device__ __forceinline__ int row_tiles(const long long *offsets, int G, int M,
     for (int s0 = 0; s0 < G + 2; s0 += 64) {
         int lo, hi;
         segment_bounds(offsets, G, M, s0, carry, lo, hi);
-        total += __shfl(wave_scan((hi - lo + BM - 1) / BM), 63, 64);
-        carry = __shfl(hi, 63, 64);
+        total += lane_value(wave_scan((hi - lo + BM - 1) / BM), 63);
+        carry = lane_value(hi, 63);
     }
     return total;
 }
@@ -481,12 +518,12 @@ __device__ __forceinline__ Segment row_tile(const long long *offsets, int G, int
         const uint64_t holds = __ballot(t < upto);
         if (holds) {
             const int l = __builtin_ctzll(holds);
-            const int first = __shfl(upto - n, l, 64), rlo = __shfl(lo, l, 64), rhi = __shfl(hi, l, 64);
+            const int first = lane_value(upto - n, l), rlo = lane_value(lo, l), rhi = lane_value(hi, l);
             const int row0 = rlo + (t - first) * BM;
             return {s0 + l - 1, row0, min(rhi - row0, BM)};
         }
-        before = __shfl(upto, 63, 64);
-        carry = __shfl(hi, 63, 64);
+        before = lane_value(upto, 63);
+        carry = lane_value(hi, 63);
     }
     return {0, 0, -1};
 }
@@ -499,11 +536,11 @@ __device__ __forceinline__ void group_rows(const long long *offsets, int G, int 
         int lo, hi;
         segment_bounds(offsets, G, M, s0, carry, lo, hi);
         if (g + 1 < s0 + 64) {
-            row0 = __builtin_amdgcn_readfirstlane(__shfl(lo, g + 1 - s0, 64));
-            rows = __builtin_amdgcn_readfirstlane(__shfl(hi, g + 1 - s0, 64)) - row0;
+            row0 = lane_value(lo, g + 1 - s0);
+            rows = lane_value(hi, g + 1 - s0) - row0;
             return;
         }
-        carry = __shfl(hi, 63, 64);
+        carry = lane_value(hi, 63);
     }
     row0 = rows = 0;
 }
