@@ -48,7 +48,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
         DirectRows<T, BM, THREADS> b;
         a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
         b.init(xr, C, s.rows, C, x + (long long)M * C);
-        product_direct<S>(a, b, C, lds, acc);
+        product_direct<S, S::RING>(a, b, C, lds, acc);
     } else {
         typename std::conditional<BACKWARD, Strided<T, BN, THREADS>, Contiguous<T, BN, THREADS>>::type a;
         Contiguous<T, BM, THREADS> b;
@@ -140,8 +140,8 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
             a.init(xt, K, ks, rows, nullptr);
             b.init(yt, N, ns, rows, nullptr);
             // the sums cost registers and branches: their own code
-            if (sums) product_direct<S, true>(a, b, rows, lds, acc, S::wave_col() == 0, sum);
-            else product_direct<S>(a, b, rows, lds, acc);
+            if (sums) product_direct<S, S::RING, true>(a, b, rows, lds, acc, S::wave_col() == 0, sum);
+            else product_direct<S, S::RING>(a, b, rows, lds, acc);
         }
         if (sums && S::wave_col() == 0 && (threadIdx.x & 63) < 16)
 #pragma unroll

@@ -315,7 +315,7 @@ template <class T_, int BM_, int BN_, int WM_, int WN_> struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;             // 16 x 16 results a wave
     static constexpr int A_BYTES = BN * T::BKC * 16 * T::PLANES, B_BYTES = BM * T::BKC * 16 * T::PLANES;
-    static constexpr int LDS = 2 * (A_BYTES + B_BYTES);                    // two steps
+    static constexpr int RING = BM * BN == 65536 ? 5 : 4, LDS = T::PLANES == 1 ? RING * (A_BYTES + B_BYTES) / 2 : 2 * (A_BYTES + B_BYTES);
     typedef typename T::acc Acc[MI][NI];
     // where a lane's results lie: rows row() + 16 m, columns col() + 16 n .. + 3
     static __device__ __forceinline__ int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM) + (int)(threadIdx.x & 15); }
