@@ -143,8 +143,10 @@ template <class S, class DA, class DB> struct DirectFragments {
 // that: behind it stage s + 1 has landed (issued RING - 1 stages ago) and every wave has read stage s, so its place in the
 // ring takes stage s + RING.  The loads behind the last stage are issued all the same, to a place that nobody reads
 // and with nothing in their bounds, so that the count of loads in flight is always the same.
+// A wave whose rows (of B, `rows` exist) all lie behind the end only takes part in the loads.
+// SUMS: sum[m] becomes the sum of B's row m over the c of this wave's share of the stages, every WN-th.
 template <class S, int RING, bool SUMS = false, class DA, class DB>
-__device__ __forceinline__ void product_direct(DA &a, DB &b, int count, char *lds, typename S::Acc &acc, bool sums = false, float *sum = nullptr)
+__device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows, char *lds, typename S::Acc &acc, float *sum = nullptr)
 {
     constexpr int STEP = DA::STEP, STAGE = DA::BYTES + DB::BYTES;
     static_assert(DA::STEP == DB::STEP, "one step for both operands");
@@ -152,6 +154,8 @@ __device__ __forceinline__ void product_direct(DA &a, DB &b, int count, char *ld
     const uint32_t base = lds_address(lds);
     DirectFragments<S, DA, DB> f[2];
     float add[S::MI] = {};
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int turn = wave % S::WN;
 #pragma unroll
     for (int k = 0; k < RING; ++k) {
         a.issue(base + k * STAGE);
@@ -159,34 +163,44 @@ __device__ __forceinline__ void product_direct(DA &a, DB &b, int count, char *ld
     }
     wait_loads<(RING - 1) * (DA::N + DB::N)>();
     __syncthreads();
-    f[0].read(lds);
     int here = 0;                            // where the stage lies that is in registers
-    for (int c0 = 0; c0 < count; c0 += 2 * STEP) {
+    auto next = [&]() {
+        wait_loads<(RING - 2) * (DA::N + DB::N)>();
+        __syncthreads();
+        a.issue(base + here);
+        b.issue(base + here + DA::BYTES);
+        here = here == (RING - 1) * STAGE ? 0 : here + STAGE;
+    };
+    if (wave / S::WN * (S::BM / S::WM) < rows) {
+        f[0].read(lds);
+        for (int c0 = 0; c0 < count; c0 += 2 * STEP) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {        // an odd number of stages ends with one of zeros
-            wait_loads<(RING - 2) * (DA::N + DB::N)>();
-            __syncthreads();
-            a.issue(base + here);
-            b.issue(base + here + DA::BYTES);
-            here = here == (RING - 1) * STAGE ? 0 : here + STAGE;
-            f[k ^ 1].read(lds + here);
-            f[k].multiply(acc);
-            interleave<MFMA, READS, 0, 0>();
-            if constexpr (SUMS)
-                if (sums) f[k].add_up(add);
+            for (int k = 0; k < 2; ++k) {    // an odd number of stages ends with one of zeros
+                next();
+                f[k ^ 1].read(lds + here);
+                f[k].multiply(acc);
+                interleave<MFMA, READS, 0, 0>();
+                if constexpr (SUMS) {
+                    if (turn == 0) f[k].add_up(add);
+                    turn = turn == 0 ? S::WN - 1 : turn - 1;
+                }
+            }
+        }
+    } else {
+        for (int c0 = 0; c0 < count; c0 += 2 * STEP) {
+            next();
+            next();
         }
     }
     wait_loads<0>();
     __syncthreads();
-    if constexpr (SUMS) {
-        if (sums) {                          // lanes i, i + 16, i + 32, i + 48 hold the row's four parts
+    if constexpr (SUMS) {                    // lanes i, i + 16, i + 32, i + 48 hold the row's four parts
 #pragma unroll
-            for (int m = 0; m < S::MI; ++m) {
-                float v = add[m];
-                v += __shfl_xor(v, 16, 64);
-                v += __shfl_xor(v, 32, 64);
-                sum[m] = v;
-            }
+        for (int m = 0; m < S::MI; ++m) {
+            float v = add[m];
+            v += __shfl_xor(v, 16, 64);
+            v += __shfl_xor(v, 32, 64);
+            sum[m] = v;
         }
     }
 }

@@ -31,8 +31,9 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     int rt, ct;
-    if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (NO + BN - 1) / BN, band, rt, ct)) return;
-    const Segment s = row_tile(offsets, G, M, BM, rt);
+    const RowTiles<BM> tiles(offsets, G, M);
+    if (!tile_of_block(blockIdx.x, tiles.total, (NO + BN - 1) / BN, band, rt, ct)) return;
+    const Segment s = tiles.tile(rt);
     const int n0 = min(ct * BN, max(0, NO - BN)), cols = min(BN, NO);       // the last tile moves back over its neighbour
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) out[(long long)(s.row0 + e / cols) * NO + n0 + e % cols] = (E)0.0f;
@@ -48,7 +49,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
         DirectRows<T, BM, THREADS> b;
         a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
         b.init(xr, C, s.rows, C, x + (long long)M * C);
-        product_direct<S, S::RING>(a, b, C, lds, acc);
+        product_direct<S, S::RING>(a, b, C, s.rows, lds, acc);
     } else {
         typename std::conditional<BACKWARD, Strided<T, BN, THREADS>, Contiguous<T, BN, THREADS>>::type a;
         Contiguous<T, BM, THREADS> b;
@@ -57,42 +58,45 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
         product<S>(a, b, C, lds, acc);
     }
 
-    const int ni0 = S::col(), mi0 = S::row();
+    if constexpr (T::PLANES == 3) {                  // what the split made a NaN of
+        const int ni0 = S::col(), mi0 = S::row();
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i = ni0 + 16 * n + k, r = mi0 + 16 * m;
+                    if (acc[m][n][k] != acc[m][n][k] && i < cols && r < s.rows)
+                        acc[m][n][k] = BACKWARD ? dot_again(wt + i, NO, xr + (long long)r * C, 1, C)
+                                                : dot_again(wt + (long long)i * C, 1, xr + (long long)r * C, 1, C);
+                }
+    }
+    typedef Out<S, E> O;
+    const int col = O::col(), have = min(O::V, cols - col);
+    if (S::wave_col() * O::COLS >= cols) return;
+    float add[O::V] = {};
+    if (!BACKWARD && bias) O::load(bias + (long long)s.g * NO + n0 + col, have, add);
+    E *to = out + (long long)s.row0 * NO + n0 + col;
+    const E *mk = mask ? mask + (long long)s.row0 * NO + n0 + col : nullptr;
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-        const int r = mi0 + 16 * m;
-        if (r >= s.rows) continue;
-        const long long row = (long long)(s.row0 + r) * NO + n0;
+        float v[O::TURNS][O::V], k[O::TURNS][O::V];
+        if (BACKWARD && mk)
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const int i = ni0 + 16 * n;
-            if (i >= cols) continue;
-            const int have = min(4, cols - i);
-            f32x4 v = acc[m][n];
-            if constexpr (T::PLANES == 3) {
+            for (int t = 0; t < O::TURNS; ++t)
+                if (O::row(m, t) < s.rows) O::load(mk + (long long)O::row(m, t) * NO, have, k[t]);
+        O::turn(lds, v, [&](int n) { return acc[m][n]; });
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (v[k] != v[k] && k < have)
-                        v[k] = BACKWARD ? dot_again(wt + i + k, NO, xr + (long long)r * C, 1, C)
-                                        : dot_again(wt + (long long)(i + k) * C, 1, xr + (long long)r * C, 1, C);
+        for (int t = 0; t < O::TURNS; ++t) {
+            if (O::row(m, t) >= s.rows) continue;
+#pragma unroll
+            for (int e = 0; e < O::V; ++e) {
+                if (!BACKWARD) v[t][e] += add[e];
+                if (!BACKWARD && relu) v[t][e] = relu_of(v[t][e]);
+                if (BACKWARD && mk) v[t][e] = k[t][e] > 0.0f ? v[t][e] : 0.0f;
             }
-            if (have == 4) {
-                if (!BACKWARD && bias) v += load4_f32(bias + (long long)s.g * NO + n0 + i);
-                if (!BACKWARD && relu) v = (f32x4){relu_of(v[0]), relu_of(v[1]), relu_of(v[2]), relu_of(v[3])};
-                if (BACKWARD && mask) {
-                    const f32x4 k = load4_f32(mask + row + i);
-                    v = (f32x4){k[0] > 0 ? v[0] : 0, k[1] > 0 ? v[1] : 0, k[2] > 0 ? v[2] : 0, k[3] > 0 ? v[3] : 0};
-                }
-                store4(out + row + i, v);
-            } else {
-                for (int k = 0; k < have; ++k) {
-                    float o = v[k];
-                    if (!BACKWARD && bias) o += to_float(bias[(long long)s.g * NO + n0 + i + k]);
-                    if (!BACKWARD && relu) o = relu_of(o);
-                    if (BACKWARD && mask) o = to_float(mask[row + i + k]) > 0 ? o : 0.0f;
-                    out[row + i + k] = from_float<E>(o);
-                }
-            }
+            O::store(to + (long long)O::row(m, t) * NO, have, v[t]);
         }
     }
 }
@@ -140,12 +144,22 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
             a.init(xt, K, ks, rows, nullptr);
             b.init(yt, N, ns, rows, nullptr);
             // the sums cost registers and branches: their own code
-            if (sums) product_direct<S, S::RING, true>(a, b, rows, lds, acc, S::wave_col() == 0, sum);
-            else product_direct<S, S::RING>(a, b, rows, lds, acc);
+            if (sums) product_direct<S, S::RING, true>(a, b, rows, ns, lds, acc, sum);
+            else product_direct<S, S::RING>(a, b, rows, ns, lds, acc);
         }
-        if (sums && S::wave_col() == 0 && (threadIdx.x & 63) < 16)
+        if (sums) {
+            // sum: of every WN-th stage; the waves of a row of waves are joined in order
+            float *part = (float *)lds;
+            if ((threadIdx.x & 63) < 16)
 #pragma unroll
-            for (int m = 0; m < MI; ++m) bias(S::row() + 16 * m, sum[m]);
+                for (int m = 0; m < MI; ++m) part[S::wave_col() * BM + S::row() + 16 * m] = sum[m];
+            __syncthreads();
+            float v = 0.0f;
+            if ((int)threadIdx.x < BM)
+#pragma unroll
+                for (int w = 0; w < S::WN; ++w) v += part[w * BM + threadIdx.x];
+            if ((int)threadIdx.x < BM) bias(threadIdx.x, v);
+        }
     } else {
         float total = 0.0f;
         if (rows > 0) {
@@ -156,37 +170,37 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
             product<S, true>(a, b, rows, lds, acc, sums);
             if (sums) total = b.total((float *)lds);
         }
-        if (sums) bias(threadIdx.x, total);
+        if (sums && (int)threadIdx.x < BM) bias(threadIdx.x, total);
     }
-    const int ni0 = S::col(), mi0 = S::row();
+    if constexpr (T::PLANES == 3) {
+        const int ni0 = S::col(), mi0 = S::row();
+#pragma unroll
+        for (int m = 0; m < MI; ++m)
+#pragma unroll
+            for (int n = 0; n < NI; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int i = ni0 + 16 * n + k, j = mi0 + 16 * m;
+                    if (acc[m][n][k] != acc[m][n][k] && i < ks && j < ns) acc[m][n][k] = dot_again(xt + i, K, yt + j, N, rows);
+                }
+    }
     const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
+    auto leave = [&](auto *to) {
+        typedef Out<S, typename std::remove_pointer<decltype(to)>::type> O;
+        const int col = O::col(), have = min(O::V, ks - col);
+        if (S::wave_col() * O::COLS >= ks) return;
 #pragma unroll
-    for (int m = 0; m < MI; ++m) {
-        const int j = mi0 + 16 * m;
-        if (j >= ns) continue;
+        for (int m = 0; m < MI; ++m) {
+            float v[O::TURNS][O::V];
+            O::turn(lds, v, [&](int n) { return acc[m][n]; });
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const int i = ni0 + 16 * n;
-            if (i >= ks) continue;
-            const int have = min(4, ks - i);
-            f32x4 v = acc[m][n];
-            if constexpr (T::PLANES == 3) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (v[k] != v[k] && k < have) v[k] = dot_again(xt + i + k, K, yt + j, N, rows);
-            }
-            const long long e = at + (long long)j * K + i;
-            if (partial) {
-                if (have == 4) store4(partial + e, v);
-                else
-                    for (int k = 0; k < have; ++k) partial[e + k] = v[k];
-            } else {
-                if (have == 4) store4(gW + e, v);
-                else
-                    for (int k = 0; k < have; ++k) gW[e + k] = from_float<E>(v[k]);
-            }
+            for (int t = 0; t < O::TURNS; ++t)
+                if (O::row(m, t) < ns) O::store(to + (long long)O::row(m, t) * K + col, have, v[t]);
         }
-    }
+    };
+    __syncthreads();                                 // the bias sums have left LDS
+    if (partial) leave(partial + at);
+    else leave(gW + at);
 }
 
 template <class E>

@@ -4,6 +4,7 @@
 // The integer sum is exact (K <= 2^17 keeps it within 32 bits, -128 among the codes included); it is rounded
 // to float32 once and scaled there.  A row of zeros has s = 0 and codes 0; a row that holds an infinity or a
 // NaN has s = NaN and codes 0, so that all its outputs are NaN.
+#include "direct_gemm.h"
 #include "few_rows.h"
 
 namespace {
@@ -12,42 +13,94 @@ using namespace tile;
 
 constexpr int THREADS = 256;                 // of the kernels without tiles
 
-// One workgroup a row.  Codes go to q with row stride ldq >= K, zeros behind K.
-template <class E>
-__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restrict__ x, int K, int8_t *__restrict__ q, long long ldq,
-                                                                float *__restrict__ scale)
+// x / s rounded to even, as float32 division gives it.  x times the reciprocal is within 2^-22 of the quotient, relatively:
+// only next to a tie (within 2^-15, |x / s| <= 128) can that round to another integer, and there it divides.
+__device__ __forceinline__ float code_of(float x, float s, float r)
 {
-    __shared__ float part[4];
-    const long long m = blockIdx.x;
-    const E *row = x + m * K;
-    float top = 0.0f;
-    bool bad = false;
-    for (int k = threadIdx.x; k < K; k += THREADS) {
-        const float a = fabsf(to_float(row[k]));
-        bad |= !(a <= 3.4028235e38f);
-        top = fmaxf(top, a);
-    }
-    if (bad) top = __builtin_nanf("");
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t = __shfl_xor(top, o, 64);
-        top = top != top || t != t ? __builtin_nanf("") : fmaxf(top, t);
-    }
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-    __syncthreads();
-    float s = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) s = part[w] != part[w] || s != s ? __builtin_nanf("") : fmaxf(s, part[w]);
-    s = s / 127.0f;
-    for (int k = threadIdx.x; k < ldq; k += THREADS) {
-        float c = 0.0f;
-        if (k < K && s > 0.0f) c = fminf(fmaxf(rintf(to_float(row[k]) / s), -127.0f), 127.0f);
-        q[m * ldq + k] = (int8_t)c;
-    }
-    if (threadIdx.x == 0) scale[m] = s;
+    const float t = x * r, n = rintf(t);
+    if (fabsf(t - n) > 0.49996f) return rintf(x / s);
+    return n;
 }
 
-template <class E, class S>
+// `LANES` threads a row, each NV vectors of 8 values in registers between the two passes; what does not fit (K > 8 LANES
+// NV) is read again.  Codes go to q with row stride ldq >= K, zeros behind K.
+template <class E, int LANES, int NV>
+__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restrict__ x, int M, int K, int8_t *__restrict__ q, long long ldq,
+                                                                float *__restrict__ scale)
+{
+    typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
+    typedef uint32_t codes __attribute__((ext_vector_type(2), aligned(1)));
+    __shared__ float part[THREADS / 64];
+    const int m = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES;
+    if (LANES == 64 && m >= M) return;       // whole waves
+    const E *row = x + (long long)m * K;
+    auto load = [&](int k, float (&v)[8]) {
+        if (k + 8 <= K) {
+            const vec u = *reinterpret_cast<const vec *>(row + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = to_float((E)u[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = k + e < K ? to_float(row[k + e]) : 0.0f;
+        }
+    };
+    float v[NV][8], top = 0.0f;
+    bool bad = false;
+    auto see = [&](const float (&u)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = fabsf(u[e]);
+            bad |= !(a <= 3.4028235e38f);
+            top = fmaxf(top, a);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load(8 * (t + i * LANES), v[i]);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) see(v[i]);
+    for (int k = 8 * (t + NV * LANES); k < K; k += 8 * LANES) {
+        float u[8];
+        load(k, u);
+        see(u);
+    }
+    if (bad) top = __builtin_inff();         // fmaxf drops a NaN: an infinity stands for both
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if constexpr (LANES == THREADS) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) top = fmaxf(top, part[w]);
+    }
+    const float s = top > 3.4028235e38f ? __builtin_nanf("") : top / 127.0f;
+    const float r = s > 0.0f ? 1.0f / s : 0.0f;
+    const bool near = r > 3.4028235e38f;     // a subnormal scale has no reciprocal
+    int8_t *to = q + m * ldq;
+    auto put = [&](int k, const float (&u)[8]) {
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float c = 0.0f;
+            if (s > 0.0f) c = near ? rintf(u[e] / s) : code_of(u[e], s, r);
+            c = fminf(fmaxf(c, -127.0f), 127.0f);
+            w[e / 4] |= (uint32_t)(uint8_t)(int8_t)c << (8 * (e % 4));
+        }
+        if (k + 8 <= ldq) *reinterpret_cast<codes *>(to + k) = codes{w[0], w[1]};
+        else
+            for (int e = 0; e < 8 && k + e < ldq; ++e) to[k + e] = (int8_t)(w[e / 4] >> (8 * (e % 4)));
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (8 * (t + i * LANES) < ldq) put(8 * (t + i * LANES), v[i]);
+    for (int k = 8 * (t + NV * LANES); k < ldq; k += 8 * LANES) {
+        float u[8];
+        load(k, u);
+        put(k, u);
+    }
+    if (t == 0) scale[m] = s;
+}
+
+template <class E, class S, bool DIRECT>
 __global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
                                                            const int8_t *__restrict__ W, const float *__restrict__ wscale,
                                                            const float *__restrict__ bias, E *__restrict__ y,
@@ -56,43 +109,55 @@ __global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__re
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     int rt, ct;
-    if (!tile_of_block(blockIdx.x, row_tiles(offsets, G, M, BM), (N + BN - 1) / BN, band, rt, ct)) return;
-    const Segment s = row_tile(offsets, G, M, BM, rt);
+    const RowTiles<BM> tiles(offsets, G, M);
+    if (!tile_of_block(blockIdx.x, tiles.total, (N + BN - 1) / BN, band, rt, ct)) return;
+    const Segment s = tiles.tile(rt);
     const int n0 = min(ct * BN, max(0, N - BN)), cols = min(BN, N);         // the last tile moves back over its neighbour
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) y[(long long)(s.row0 + e / cols) * N + n0 + e % cols] = (E)0.0f;
         return;
     }
-    Contiguous<I8, BN, THREADS> a;
-    Contiguous<I8, BM, THREADS> b;
+    typedef typename std::conditional<DIRECT, DirectRows<I8, BN, THREADS>, Contiguous<I8, BN, THREADS>>::type LA;
+    typedef typename std::conditional<DIRECT, DirectRows<I8, BM, THREADS>, Contiguous<I8, BM, THREADS>>::type LB;
+    LA a;
+    LB b;
     a.init(W + ((long long)s.g * N + n0) * K, K, cols, K, W + (long long)G * N * K);
     b.init(q + s.row0 * ldq, ldq, s.rows, K, q + M * ldq);
-    constexpr int MI = S::MI, NI = S::NI;
+    constexpr int MI = S::MI;
     typename S::Acc acc = {};
-    product<S>(a, b, K, lds, acc);
-    const int ni0 = S::col(), mi0 = S::row();
+    if constexpr (DIRECT) product_direct<S, S::RING>(a, b, K, s.rows, lds, acc);
+    else product<S>(a, b, K, lds, acc);
+    // the compiler would convert the sums to float in the loop, on every turn
+#pragma unroll
+    for (int m = 0; m < MI; ++m)
+#pragma unroll
+        for (int n = 0; n < S::NI; ++n) asm volatile("" : "+v"(acc[m][n]));
+    typedef Out<S, E> O;
+    const int col = O::col(), have = min(O::V, cols - col);
+    if (S::wave_col() * O::COLS >= cols) return;
+    float ws[O::V], add[O::V];
+    const long long c = (long long)s.g * N + n0 + col;
+#pragma unroll
+    for (int e = 0; e < O::V; ++e) {
+        ws[e] = e < have ? wscale[c + e] : 0.0f;
+        add[e] = bias && e < have ? bias[c + e] : 0.0f;
+    }
+    E *to = y + (long long)s.row0 * N + n0 + col;
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
-        const int r = mi0 + 16 * m;
-        if (r >= s.rows) continue;
-        const long long row = (long long)(s.row0 + r) * N + n0;
-        const float qs = qscale[s.row0 + r];
+        float v[O::TURNS][O::V], qs[O::TURNS];
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const int i = ni0 + 16 * n;
-            if (i >= cols) continue;
-            const int have = min(4, cols - i);
-            const long long c = (long long)s.g * N + n0 + i;
-            f32x4 v;
+        for (int t = 0; t < O::TURNS; ++t) qs[t] = qscale[s.row0 + min(O::row(m, t), s.rows - 1)];
+        O::turn(lds, v, [&](int n) { return __builtin_convertvector(acc[m][n], f32x4); });
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int kk = min(k, have - 1);
-                v[k] = (float)acc[m][n][k] * qs * wscale[c + kk] + (bias ? bias[c + kk] : 0.0f);
-                if (relu) v[k] = relu_of(v[k]);
+        for (int t = 0; t < O::TURNS; ++t) {
+            if (O::row(m, t) >= s.rows) continue;
+#pragma unroll
+            for (int e = 0; e < O::V; ++e) {
+                v[t][e] = v[t][e] * qs[t] * ws[e] + add[e];
+                if (relu) v[t][e] = relu_of(v[t][e]);
             }
-            if (have == 4) store4(y + row + i, v);
-            else
-                for (int k = 0; k < have; ++k) y[row + i + k] = from_float<E>(v[k]);
+            O::store(to + (long long)O::row(m, t) * N, have, v[t]);
         }
     }
 }
@@ -163,20 +228,29 @@ int check(const char *who, int M, int K, int dtype)
     return WM_OK;
 }
 
+// A wave a row up to 1024 values, a workgroup beyond (8192 rows of 4096 bf16: 54 us by single values, 2 passes; see DESIGN).
 template <class E> int quantize(const void *x, int M, int K, int8_t *q, long long ldq, float *scale, hipStream_t st)
 {
-    hipLaunchKernelGGL(quantize_rows_kernel<E>, dim3(M), dim3(THREADS), 0, st, (const E *)x, K, q, ldq, scale);
+#define WM_QUANTIZE(LANES, NV)                                                                                                       \
+    hipLaunchKernelGGL((quantize_rows_kernel<E, LANES, NV>), dim3((M + THREADS / LANES - 1) / (THREADS / LANES)), dim3(THREADS), 0, \
+                       st, (const E *)x, M, K, q, ldq, scale)
+    if (K <= 512) WM_QUANTIZE(64, 1);
+    else if (K <= 1024) WM_QUANTIZE(64, 2);
+    else if (K <= 2048) WM_QUANTIZE(THREADS, 1);
+    else if (K <= 4096) WM_QUANTIZE(THREADS, 2);
+    else WM_QUANTIZE(THREADS, 4);
+#undef WM_QUANTIZE
     WM_LAUNCH_CHECK("quantize_rows_kernel");
     return WM_OK;
 }
 
-template <class E, class S>
+template <class E, class S, bool DIRECT>
 int dense_tiles(const int8_t *q, long long ldq, const float *scale, const int8_t *W, const float *wscale, const float *b, void *y,
                 const int64_t *offsets, int G, int M, int N, int K, int relu, hipStream_t st)
 {
     const long long blocks = row_tiles_most(G, M, S::BM) * ((N + S::BN - 1) / S::BN);
     WM_REQUIRE(blocks <= (1ll << 32) / 512 - 1, WM_ERR_UNSUPPORTED, "wm_dense_i8: %lld tiles are too many for one launch", blocks);
-    hipLaunchKernelGGL((dense_i8_kernel<E, S>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
+    hipLaunchKernelGGL((dense_i8_kernel<E, S, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
                        (const long long *)offsets, G, M, N, K, relu, 8);
     WM_LAUNCH_CHECK("dense_i8_kernel");
     return WM_OK;
@@ -196,8 +270,12 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
         return WM_OK;
     }
-    if (M / G >= 512 && N >= 512) return dense_tiles<E, Shape<I8, 256, 256, 2, 4>>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
-    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+    if (direct_ok(W, K)) {
+        if (M / G >= 512 && N >= 512)
+            return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+        return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+    }
+    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
 }
 
 }  // namespace

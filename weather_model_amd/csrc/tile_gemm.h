@@ -321,6 +321,7 @@ template <class T_, int BM_, int BN_, int WM_, int WN_> struct Shape {
     static __device__ __forceinline__ int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM) + (int)(threadIdx.x & 15); }
     static __device__ __forceinline__ int col() { return (int)(threadIdx.x >> 6) % WN * (BN / WN) + 4 * ((int)(threadIdx.x & 63) >> 4); }
     static __device__ __forceinline__ int wave_col() { return (int)(threadIdx.x >> 6) % WN; }
+    static __device__ __forceinline__ int wave_row() { return (int)(threadIdx.x >> 6) / WN; }
 };
 
 // ---- the core: acc[mi][ni] += A B^T over c = 0 .. count; A gives i (BN), B gives j (BM)
@@ -449,6 +450,62 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
     }
 }
 
+// ---- the way out: a wave turns 16 rows of its results through LDS (its own piece: no barrier) so that a lane holds 16 bytes
+// of a row and a row's part of the tile leaves as whole lines; four results a lane, as the MFMA leaves them, are 8 bytes of
+// 16 rows a store, and a tile of 256 x 256 took 15 us to leave that way.
+template <class S, class E> struct Out {
+    static constexpr int V = 16 / sizeof(E), COLS = S::NI * 16, LD = COLS + 4, LANES = COLS / V, ROWS = 64 / LANES, TURNS = 16 / ROWS;
+    static_assert(S::WM * S::WN * 16 * LD * 4 <= S::LDS, "LDS");
+    static __device__ __forceinline__ int col() { return S::wave_col() * COLS + (int)(threadIdx.x & 63) % LANES * V; }
+    static __device__ __forceinline__ int row(int m, int t) { return S::wave_row() * (S::BM / S::WM) + 16 * m + t * ROWS + (int)(threadIdx.x & 63) / LANES; }
+    // the values of block m at (row(m, t), col() ..), all t; `block(n)` gives the MFMA's four values of column block n
+    template <class B> static __device__ __forceinline__ void turn(char *lds, float (&v)[TURNS][V], B block)
+    {
+        const int lane = threadIdx.x & 63;
+        float *own = (float *)lds + (threadIdx.x >> 6) * (16 * LD);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int n = 0; n < S::NI; ++n) wm_store4(own + (lane & 15) * LD + 16 * n + 4 * (lane >> 4), block(n));
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < TURNS; ++t)
+#pragma unroll
+            for (int k = 0; k < V; k += 4) {
+                const f32x4 f = wm_load4(own + (t * ROWS + lane / LANES) * LD + lane % LANES * V + k);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[t][k + e] = f[e];
+            }
+        __builtin_amdgcn_wave_barrier();
+    }
+    // up to V consecutive elements
+    static __device__ __forceinline__ void load(const E *p, int have, float (&v)[V])
+    {
+        typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+        if (have >= V) {
+            const vec x = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = to_float((E)x[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k) v[k] = k < have ? to_float(p[k]) : 0.0f;
+        }
+    }
+    static __device__ __forceinline__ void store(E *p, int have, const float (&v)[V])
+    {
+        typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+        if (have >= V) {
+            vec x;
+#pragma unroll
+            for (int k = 0; k < V; ++k) x[k] = from_float<E>(v[k]);
+            *reinterpret_cast<vec *>(p) = x;
+        } else {
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                if (k < have) p[k] = from_float<E>(v[k]);
+        }
+    }
+};
+
 // C[i][j] once more in float32, for elements that the split made a NaN of
 __device__ __forceinline__ float dot_again(const float *a, long long sa, const float *b, long long sb, int count)
 {
@@ -461,7 +518,7 @@ __device__ __forceinline__ float dot_again(const float *a, long long sa, const f
 // the nearest inside, one below an earlier one as that one, so any values give a partition of the rows.
 // Rows that no group owns are the segments -1 (before offsets[0]) and G (behind offsets[G]).
 struct Segment {
-    int g, row0, rows;                       // rows of this tile, rows < 0: no such tile
+    int g, row0, rows;                       // group, first row and rows of a tile
 };
 
 // Bounds of 64 segments s0 .. s0 + 63 in the lanes (segment s is group s - 1); `carry` is the bound before s0.
@@ -495,38 +552,40 @@ __device__ __forceinline__ int wave_scan(int v)          // inclusive
     return v;
 }
 
-__device__ __forceinline__ int row_tiles(const long long *offsets, int G, int M, int BM)
-{
-    int total = 0, carry = 0;
-    for (int s0 = 0; s0 < G + 2; s0 += 64) {
-        int lo, hi;
-        segment_bounds(offsets, G, M, s0, carry, lo, hi);
-        total += lane_value(wave_scan((hi - lo + BM - 1) / BM), 63);
-        carry = lane_value(hi, 63);
-    }
-    return total;
-}
+// The map from a tile's number to its rows, built once a workgroup; what up to 62 groups need stays in the lanes.
+template <int BM> struct RowTiles {
+    const long long *offsets;
+    int G, M, lo, hi, total;                 // bounds of the first 64 segments
 
-// the t-th tile of BM rows
-__device__ __forceinline__ Segment row_tile(const long long *offsets, int G, int M, int BM, int t)
-{
-    int before = 0, carry = 0;
-    for (int s0 = 0; s0 < G + 2; s0 += 64) {
-        int lo, hi;
-        segment_bounds(offsets, G, M, s0, carry, lo, hi);
-        const int n = (hi - lo + BM - 1) / BM, upto = before + wave_scan(n);
-        const uint64_t holds = __ballot(t < upto);
-        if (holds) {
-            const int l = __builtin_ctzll(holds);
-            const int first = lane_value(upto - n, l), rlo = lane_value(lo, l), rhi = lane_value(hi, l);
-            const int row0 = rlo + (t - first) * BM;
-            return {s0 + l - 1, row0, min(rhi - row0, BM)};
+    __device__ __forceinline__ RowTiles(const long long *offsets_, int G_, int M_) : offsets(offsets_), G(G_), M(M_), total(0)
+    {
+        int carry = 0;
+        for (int s0 = 0; s0 < G + 2; s0 += 64) {
+            int l, h;
+            segment_bounds(offsets, G, M, s0, carry, l, h);
+            if (s0 == 0) lo = l, hi = h;
+            total += lane_value(wave_scan((h - l + BM - 1) / BM), 63);
+            carry = lane_value(h, 63);
         }
-        before = lane_value(upto, 63);
-        carry = lane_value(hi, 63);
     }
-    return {0, 0, -1};
-}
+    __device__ __forceinline__ Segment tile(int t) const
+    {
+        int before = 0, carry = 0, l = lo, h = hi;
+        for (int s0 = 0; s0 < G + 2; s0 += 64) {
+            if (s0 > 0) segment_bounds(offsets, G, M, s0, carry, l, h);
+            const int n = (h - l + BM - 1) / BM, upto = before + wave_scan(n);
+            const uint64_t holds = __ballot(t < upto);
+            if (holds) {
+                const int k = __builtin_ctzll(holds);
+                const int row0 = lane_value(l, k) + (t - lane_value(upto - n, k)) * BM;
+                return {s0 + k - 1, row0, min(lane_value(h, k) - row0, BM)};
+            }
+            before = lane_value(upto, 63);
+            carry = lane_value(h, 63);
+        }
+        return {0, 0, 0};
+    }
+};
 
 // rows of group g (workgroup-uniform)
 __device__ __forceinline__ void group_rows(const long long *offsets, int G, int M, int g, int &row0, int &rows)
