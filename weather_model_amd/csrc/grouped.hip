@@ -163,12 +163,12 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
     } else {
         float total = 0.0f;
         if (rows > 0) {
-            Strided<T, BN, THREADS> a;
-            Strided<T, BM, THREADS> b;
-            a.init(xt, K, ks, rows, x + (long long)M * K);
-            b.init(yt, N, ns, rows, gy + (long long)M * N);
-            product<S, true>(a, b, rows, lds, acc, sums);
-            if (sums) total = b.total((float *)lds);
+            static_assert(BM == BN, "a pair");
+            StridedPair<T, BM, THREADS> pair;
+            Nothing<T> none;
+            pair.init(xt, K, ks, yt, N, ns, rows);
+            product<S, true>(pair, none, rows, lds, acc, sums);
+            if (sums) total = pair.total((float *)lds);
         }
         if (sums && (int)threadIdx.x < BM) bias(threadIdx.x, total);
     }
@@ -305,8 +305,8 @@ template <class T> struct Tiles {                       // 16-bit types
     typedef Shape<T, 128, 128, 2, 2> Medium;
 };
 template <> struct Tiles<F32> {
-    typedef Shape<F32, 256, 128, 4, 2> Large;
-    typedef Shape<F32, 128, 128, 2, 2> Medium;
+    typedef Shape<F32, 128, 128, 2, 2, 1> Large;
+    typedef Shape<F32, 128, 128, 2, 2, 1> Medium;
 };
 
 bool large(int G, int M, int N, int K) { (void)K; return M / G >= 512 && N >= 512; }
@@ -350,52 +350,56 @@ int rows_any(int dtype, const void *x, const void *W, const void *bias, const vo
     }
 }
 
-constexpr int WB_TILE = 128;
-
+// Shares of the rows of an expert, whatever tile is taken: enough workgroups of 128 x 128 for two rounds of 256 CUs, at
+// least 256 rows of an average expert each.
 int weight_splits(int M, int N, int K, int G)
 {
-    // enough workgroups for two rounds of 256 CUs, at least 256 rows of an average expert each
-    const long long tiles = (long long)G * ((N + WB_TILE - 1) / WB_TILE) * ((K + WB_TILE - 1) / WB_TILE);
+    const long long tiles = (long long)G * ((N + 127) / 128) * ((K + 127) / 128);
     const long long want = (512 + tiles - 1) / tiles, most = M / ((long long)G * 256);
     const long long s = want < most ? want : most;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
 
+template <class S, bool DIRECT>
+int weights_launch(const void *x, const void *gy, void *gW, void *gb, float *partial, const int64_t *offsets, int G, int M, int N, int K,
+                   int splits, hipStream_t st)
+{
+    typedef typename S::T::elem E;
+    const long long blocks = (long long)splits * G * ((N + S::BM - 1) / S::BM) * ((K + S::BN - 1) / S::BN);
+    if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
+    hipLaunchKernelGGL((grouped_weights_kernel<S, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)gy, (const E *)x, (E *)gW,
+                       (E *)gb, partial, (const long long *)offsets, G, M, N, K, splits);
+    WM_LAUNCH_CHECK("grouped_weights_kernel");
+    return WM_OK;
+}
+
 template <class T>
-int weights_launch(const void *x, const void *gy, void *gW, void *gb, void *workspace, const int64_t *offsets, int G, int M, int N, int K,
-                   hipStream_t st)
+int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *workspace, const int64_t *offsets, int G, int M, int N, int K,
+                  hipStream_t st)
 {
     typedef typename T::elem E;
-    const int S = weight_splits(M, N, K, G);
-    const long long blocks = (long long)S * G * ((N + WB_TILE - 1) / WB_TILE) * ((K + WB_TILE - 1) / WB_TILE);
-    if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
-    float *partial = S > 1 ? (float *)workspace : nullptr;
     typedef typename Tiles<T>::Large L;
     typedef typename Tiles<T>::Medium Md;
-    const bool big = large(1, N, K, M) && S == 1;
-    const long long lb = (long long)G * ((N + L::BM - 1) / L::BM) * ((K + L::BN - 1) / L::BN);
-#define WM_WEIGHTS(SHAPE, DIRECT, BLOCKS)                                                                                              \
-    hipLaunchKernelGGL((grouped_weights_kernel<SHAPE, DIRECT>), dim3((unsigned)(BLOCKS)), dim3(SHAPE::THREADS), 0, st, (const E *)gy, \
-                       (const E *)x, (E *)gW, (E *)gb, partial, (const long long *)offsets, G, M, N, K, S)
+    const int splits = weight_splits(M, N, K, G);
+    float *partial = splits > 1 ? (float *)workspace : nullptr;
+    const bool big = large(1, N, K, M) && splits == 1;
+    int rc;
     if constexpr (T::PLANES == 1) {
         const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N);
-        if (direct && big) WM_WEIGHTS(L, true, lb);
-        else if (direct) WM_WEIGHTS(Md, true, blocks);
-        else WM_WEIGHTS(Md, false, blocks);
+        rc = direct && big ? weights_launch<L, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
+             : direct      ? weights_launch<Md, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
+                           : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
     } else {
-        if (big) WM_WEIGHTS(L, false, lb);
-        else WM_WEIGHTS(Md, false, blocks);
+        rc = big ? weights_launch<L, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
+                 : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
     }
-#undef WM_WEIGHTS
-    WM_LAUNCH_CHECK("grouped_weights_kernel");
-    if (S > 1) {
-        const long long count = (long long)G * N * K;
-        long long grid = (count + THREADS - 1) / THREADS;
-        if (grid > 4096) grid = 4096;
-        hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid), dim3(THREADS), 0, st, (const float *)workspace, (E *)gW, count,
-                           (E *)gb, (long long)G * N, S);
-        WM_LAUNCH_CHECK("grouped_weights_sum_kernel");
-    }
+    if (rc != WM_OK || splits == 1) return rc;
+    const long long count = (long long)G * N * K;
+    long long grid = (count + THREADS - 1) / THREADS;
+    if (grid > 4096) grid = 4096;
+    hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid), dim3(THREADS), 0, st, (const float *)workspace, (E *)gW, count, (E *)gb,
+                       (long long)G * N, splits);
+    WM_LAUNCH_CHECK("grouped_weights_sum_kernel");
     return WM_OK;
 }
 
@@ -444,8 +448,8 @@ extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, 
                "wm_dense_grouped_bwd_wb: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case WM_F32: return weights_launch<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
-    case WM_BF16: return weights_launch<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
-    default: return weights_launch<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    case WM_F32: return weights_typed<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    case WM_BF16: return weights_typed<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    default: return weights_typed<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
     }
 }

@@ -195,7 +195,8 @@ template <class T, int ROWS, int THREADS> struct Contiguous {
     }
 };
 
-// ---- an operand with the tile's rows along memory: element (row r, c) at base + c * ld + r
+// ---- an operand with the tile's rows along memory: element (row r, c) at base + c * ld + r; THREADS of the workgroup load it,
+// from number `first` on
 template <class T, int ROWS, int THREADS> struct Strided {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * 8, BLOCKS = THREADS / BKC, W = ROWS / BLOCKS;   // W rows x 8 c a thread
@@ -211,7 +212,7 @@ template <class T, int ROWS, int THREADS> struct Strided {
     int most;                                // rows that exist, at least 1
     bool slow;                               // fewer rows than a thread's vector: load() does not fit (workgroup-uniform)
 
-    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *)
+    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *, int first = 0)
     {
         base = tensor_row0;
         ld = ld_;
@@ -223,7 +224,7 @@ template <class T, int ROWS, int THREADS> struct Strided {
         for (int i = 0; i < W; ++i) sum[i] = 0.0f;
         // a vector that would leave the rows moves back into them: two threads then write the same values to the
         // same place, and rows that do not exist keep whatever LDS held (their results are not stored)
-        r0 = slow ? 0 : min((int)(threadIdx.x / BKC) * W, rows_left - W);
+        r0 = slow ? 0 : min(((int)threadIdx.x - first) / BKC * W, rows_left - W);
     }
     __device__ __forceinline__ void load(int c0)
     {
@@ -270,10 +271,11 @@ template <class T, int ROWS, int THREADS> struct Strided {
             }
     }
     // the sums over all c, in a fixed order: LDS holds BKC x ROWS floats; returns that of row threadIdx.x < ROWS
-    __device__ __forceinline__ float total(float *lds)
+    __device__ __forceinline__ float total(float *lds, bool mine = true)
     {
+        if (mine)
 #pragma unroll
-        for (int i = 0; i < W; ++i) lds[q * ROWS + r0 + i] = sum[i];
+            for (int i = 0; i < W; ++i) lds[q * ROWS + r0 + i] = sum[i];
         __syncthreads();
         float s = 0.0f;
         if (threadIdx.x < ROWS)
@@ -309,13 +311,40 @@ template <class T, int ROWS, int THREADS> struct Strided {
     }
 };
 
+// Two strided operands of as many rows each: one half of the waves loads the one, the other half the other, so that a thread's
+// loads are twice as wide.  Stands in both places of product().
+template <class T, int ROWS, int THREADS> struct StridedPair : Strided<T, ROWS, THREADS / 2> {
+    typedef Strided<T, ROWS, THREADS / 2> Half;
+    bool second;
+    __device__ __forceinline__ void init(const typename T::elem *a, long long lda, int rows_a, const typename T::elem *b, long long ldb, int rows_b,
+                                         int count)
+    {
+        second = __builtin_amdgcn_readfirstlane(threadIdx.x) >= THREADS / 2;
+        Half::init(second ? b : a, second ? ldb : lda, second ? rows_b : rows_a, count, nullptr, second ? THREADS / 2 : 0);
+        this->slow = rows_a < Half::W || rows_b < Half::W;
+        if (this->slow) this->r0 = ((int)threadIdx.x - (second ? THREADS / 2 : 0)) / Half::BKC * Half::W;
+    }
+    __device__ __forceinline__ void store(char *lds) { Half::store(lds + (second ? ROWS * Half::BKC * 16 * T::PLANES : 0)); }
+    __device__ __forceinline__ void add_up() { if (second) Half::add_up(); }
+    __device__ __forceinline__ float total(float *lds) { return Half::total(lds, second); }
+};
+// the other place
+template <class T> struct Nothing {
+    static constexpr int STEP = T::BKC * 8, N_LOADS = 0, N_STORES = 0;
+    static constexpr bool slow = false;
+    __device__ __forceinline__ void load(int) {}
+    __device__ __forceinline__ void load_guarded(int) {}
+    __device__ __forceinline__ void store(char *) {}
+};
+
 // ---- a shape of tile: BM rows by BN columns of C over WM x WN waves
-template <class T_, int BM_, int BN_, int WM_, int WN_> struct Shape {
+template <class T_, int BM_, int BN_, int WM_, int WN_, int BUFFERS_ = 2> struct Shape {
     typedef T_ T;
+    static constexpr int BUFFERS = BUFFERS_; // steps in LDS
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;             // 16 x 16 results a wave
     static constexpr int A_BYTES = BN * T::BKC * 16 * T::PLANES, B_BYTES = BM * T::BKC * 16 * T::PLANES;
-    static constexpr int RING = BM * BN == 65536 ? 5 : 4, LDS = T::PLANES == 1 ? RING * (A_BYTES + B_BYTES) / 2 : 2 * (A_BYTES + B_BYTES);
+    static constexpr int RING = BM * BN == 65536 ? 5 : 4, LDS = T::PLANES == 1 ? RING * (A_BYTES + B_BYTES) / 2 : BUFFERS * (A_BYTES + B_BYTES);
     typedef typename T::acc Acc[MI][NI];
     // where a lane's results lie: rows row() + 16 m, columns col() + 16 n .. + 3
     static __device__ __forceinline__ int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM) + (int)(threadIdx.x & 15); }
@@ -380,6 +409,9 @@ template <int MFMA, int READS, int STORES, int LOADS> __device__ __forceinline__
     }
 }
 
+template <class LA, class LB> __device__ __forceinline__ LB &summed(LA &, LB &b) { return b; }
+template <class LA, class T> __device__ __forceinline__ LA &summed(LA &a, Nothing<T> &) { return a; }
+
 // Whole steps, each of SUB reads of operands: while one step is multiplied, the next goes from registers to the other
 // half of LDS and the one after that is loaded (the last steps load themselves once more instead of branching: a
 // branch around the loads makes the compiler wait for them at its end).  There is one barrier a step, before its last
@@ -400,20 +432,38 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
         a.store(lds);
         b.store(lds + S::A_BYTES);
         if constexpr (SUMS)
-            if (sums) b.add_up();
+            if (sums) summed(a, b).add_up();
         const int second = min(STEP, full - STEP);
         a.load(second);
         b.load(second);
         __syncthreads();
         int here = 0;
-        if constexpr (SUB == 2) f[0].read(lds, 0);
-        for (int c0 = 0; c0 < full; c0 += STEP) {
+        if constexpr (S::BUFFERS == 1) {
+            for (int c0 = 0; c0 < full; c0 += STEP) {
+#pragma unroll
+                for (int s = 0; s < SUB; ++s) {
+                    f[0].read(lds, s);
+                    f[0].multiply(acc);
+                }
+                __syncthreads();
+                a.store(lds);
+                b.store(lds + S::A_BYTES);
+                if constexpr (SUMS)
+                    if (sums && c0 + STEP < full) summed(a, b).add_up();
+                const int next = min(c0 + 2 * STEP, full - STEP);
+                a.load(next);
+                b.load(next);
+                __syncthreads();
+            }
+        }
+        if constexpr (SUB == 2 && S::BUFFERS == 2) f[0].read(lds, 0);
+        if constexpr (S::BUFFERS == 2) for (int c0 = 0; c0 < full; c0 += STEP) {
             const int there = HALF - here;
             f[1].read(lds + here, SUB - 1);
             a.store(lds + there);
             b.store(lds + there + S::A_BYTES);
             if constexpr (SUMS)
-                if (sums && c0 + STEP < full) b.add_up();
+                if (sums && c0 + STEP < full) summed(a, b).add_up();
             const int next = min(c0 + 2 * STEP, full - STEP);
             a.load(next);
             b.load(next);
@@ -437,7 +487,7 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
         a.load_guarded(c0);
         b.load_guarded(c0);
         if constexpr (SUMS)
-            if (sums) b.add_up();
+            if (sums) summed(a, b).add_up();
         a.store(lds);
         b.store(lds + S::A_BYTES);
         __syncthreads();
