@@ -75,7 +75,7 @@ template <class T, int ROWS, int THREADS> struct DirectCols {
     long long ld, left;                      // bytes; left: from `at` to the end of the last c's part of this tile
     uint32_t voffset[2];                     // of this thread's even and odd hops
     // the permutation of 32-byte blocks at c (bits 2 and 5 are fixed in a read instruction)
-    static __device__ __forceinline__ int mix(int c) { return (c & 3) | ((((c >> 3) ^ (c >> 4)) & 1) << 2); }
+    static __device__ __forceinline__ int mix(int c) { return ((c & 3) | ((((c >> 3) ^ (c >> 4)) & 1) << 2)) & (ROWS / 16 - 1); }
 
     __device__ __forceinline__ void init(const typename T::elem *row0, long long ld_, int rows, int c_count, const typename T::elem *)
     {

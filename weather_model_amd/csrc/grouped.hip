@@ -21,20 +21,15 @@ template <class T> __device__ __forceinline__ f32x4 load4_f32(const T *p)
 
 // ---- rows: out (M, NO) = x (M, C) times W[g], forward (W[g] is (NO, C), its c along memory) or backward
 // (W[g] is (C, NO)).  bias and relu are the forward's, mask the backward's.
-template <class S, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
-__global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
-                                                                  const E *__restrict__ mask, E *__restrict__ out,
-                                                                  const long long *__restrict__ offsets, int G, int M, int NO, int C, int relu,
-                                                                  int band)
+template <class S, bool BACKWARD, bool DIRECT, class E>
+__device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias, const E *__restrict__ mask,
+                                          E *__restrict__ out, char *lds, Segment s, int n0, int G, int M, int NO, int C, int relu)
 {
     typedef typename S::T T;
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    int rt, ct;
-    const RowTiles<BM> tiles(offsets, G, M);
-    if (!tile_of_block(blockIdx.x, tiles.total, (NO + BN - 1) / BN, band, rt, ct)) return;
-    const Segment s = tiles.tile(rt);
-    const int n0 = min(ct * BN, max(0, NO - BN)), cols = min(BN, NO);       // the last tile moves back over its neighbour
+    s.rows = min(s.rows, BM);
+    const int cols = min(BN, NO - n0);
+    if (s.rows <= 0 || cols <= 0) return;
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) out[(long long)(s.row0 + e / cols) * NO + n0 + e % cols] = (E)0.0f;
         return;
@@ -101,13 +96,37 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
     }
 }
 
+template <class S, class Sub, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
+__global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
+                                                                  const E *__restrict__ mask, E *__restrict__ out,
+                                                                  const long long *__restrict__ offsets, int G, int M, int NO, int C, int relu,
+                                                                  int slots)
+{
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+    const RowTiles<S::BM> tiles(offsets, G, M);
+    const int across = (NO + S::BN - 1) / S::BN;
+    const Cut<S, Sub> cut(blockIdx.x, tiles.total * across, slots);
+    if (cut.tile < 0) return;
+    int rt, ct;
+    place_of_tile(cut.tile, tiles.total, across, 8, rt, ct);
+    Segment s = tiles.tile(rt);
+    const int n0 = min(ct * S::BN, max(0, NO - S::BN));      // the last tile moves back over its neighbour
+    if (!cut.part) {
+        rows_tile<S, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0, G, M, NO, C, relu);
+    } else {
+        s.row0 += cut.row;
+        s.rows -= cut.row;
+        rows_tile<Sub, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
+    }
+}
+
 // ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
 // with S > 1 the shares go to `partial` (S, G, N, K), and to (S, G, N) behind it, and grouped_weights_sum_kernel adds
 // them in order.  gb is summed by the workgroups of the first columns from the registers that feed LDS.
 template <class S, bool DIRECT, class E = typename S::T::elem>
 __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
                                                                      E *__restrict__ gb, float *__restrict__ partial, const long long *__restrict__ offsets, int G,
-                                                                     int M, int N, int K, int splits)
+                                                                     int M, int N, int K, int splits, int first)
 {
     typedef typename S::T T;
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
@@ -119,9 +138,9 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
     id /= kt;
     const int n0 = min(id % nt * BM, max(0, N - BM));
     id /= nt;
-    const int g = id % G, split = id / G;
-    int row0, rows;
-    group_rows(offsets, G, M, g, row0, rows);
+    const int split = id % splits, turn = id / splits;
+    int g, row0, rows;
+    group_in_turn(offsets, G, M, turn, first, g, row0, rows);
     constexpr int STEP = T::BKC * 8;
     const int share = ((rows + splits - 1) / splits + STEP - 1) / STEP * STEP;
     row0 += min(rows, split * share);
@@ -287,43 +306,48 @@ int blocks_ok(const char *who, long long blocks)
     return WM_OK;
 }
 
-template <class S, bool BACKWARD, bool DIRECT>
+constexpr int LDS_PER_CU = 160 << 10;
+
+template <class S, class Sub, bool BACKWARD, bool DIRECT>
 int rows_launch(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                 int C, int relu, hipStream_t st)
 {
     typedef typename S::T::elem E;
-    const long long blocks = row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN);
+    const int slots = wm_num_cus() * (S::LDS <= LDS_PER_CU / 2 ? 2 : 1);
+    const long long blocks = Cut<S, Sub>::blocks(row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN), slots);
     if (int rc = blocks_ok("wm_dense_grouped", blocks)) return rc;
-    hipLaunchKernelGGL((grouped_rows_kernel<S, BACKWARD, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x, (const E *)W,
-                       (const E *)bias, (const E *)mask, (E *)out, (const long long *)offsets, G, M, NO, C, relu, 8);
+    hipLaunchKernelGGL((grouped_rows_kernel<S, Sub, BACKWARD, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x,
+                       (const E *)W, (const E *)bias, (const E *)mask, (E *)out, (const long long *)offsets, G, M, NO, C, relu, slots);
     WM_LAUNCH_CHECK("grouped_rows_kernel");
     return WM_OK;
 }
 
 template <class T> struct Tiles {                       // 16-bit types
     typedef Shape<T, 256, 256, 2, 4> Large;
+    typedef Shape<T, 128, 256, 2, 4> LargePart;
     typedef Shape<T, 128, 128, 2, 2> Medium;
+    typedef Shape<T, 64, 64, 2, 2> MediumPart;
 };
 template <> struct Tiles<F32> {
-    typedef Shape<F32, 128, 128, 2, 2, 1> Large;
     typedef Shape<F32, 128, 128, 2, 2, 1> Medium;
+    typedef Shape<F32, 64, 64, 2, 2, 1> MediumPart;
 };
 
-bool large(int G, int M, int N, int K) { (void)K; return M / G >= 512 && N >= 512; }
+bool large(int G, int M, int N) { return M / G >= 512 && N >= 512; }
 
 template <class T, bool BACKWARD>
 int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                int C, int relu, hipStream_t st)
 {
-    typedef typename Tiles<T>::Large L;
-    typedef typename Tiles<T>::Medium Md;
+    typedef Tiles<T> Z;
     if constexpr (T::PLANES == 1) {
         if (direct_ok(x, 2ll * C) && direct_ok(W, BACKWARD ? 2ll * NO : 2ll * C)) {
-            if (large(G, M, NO, C)) return rows_launch<L, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-            return rows_launch<Md, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+            if (large(G, M, NO))
+                return rows_launch<typename Z::Large, typename Z::LargePart, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+            return rows_launch<typename Z::Medium, typename Z::MediumPart, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
         }
-    } else if (large(G, M, NO, C)) return rows_launch<L, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-    return rows_launch<Md, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    }
+    return rows_launch<typename Z::Medium, typename Z::MediumPart, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows.
@@ -367,8 +391,10 @@ int weights_launch(const void *x, const void *gy, void *gW, void *gb, float *par
     typedef typename S::T::elem E;
     const long long blocks = (long long)splits * G * ((N + S::BM - 1) / S::BM) * ((K + S::BN - 1) / S::BN);
     if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
+    // groups begun on empty CUs, where all workgroups run at once
+    const long long first = blocks <= 2ll * wm_num_cus() && S::LDS <= LDS_PER_CU / 2 ? wm_num_cus() / (blocks / G) : G;
     hipLaunchKernelGGL((grouped_weights_kernel<S, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)gy, (const E *)x, (E *)gW,
-                       (E *)gb, partial, (const long long *)offsets, G, M, N, K, splits);
+                       (E *)gb, partial, (const long long *)offsets, G, M, N, K, splits, (int)first);
     WM_LAUNCH_CHECK("grouped_weights_kernel");
     return WM_OK;
 }
@@ -378,20 +404,18 @@ int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *works
                   hipStream_t st)
 {
     typedef typename T::elem E;
-    typedef typename Tiles<T>::Large L;
     typedef typename Tiles<T>::Medium Md;
     const int splits = weight_splits(M, N, K, G);
     float *partial = splits > 1 ? (float *)workspace : nullptr;
-    const bool big = large(1, N, K, M) && splits == 1;
     int rc;
     if constexpr (T::PLANES == 1) {
-        const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N);
+        typedef typename Tiles<T>::Large L;
+        const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N), big = large(1, N, K) && splits == 1;
         rc = direct && big ? weights_launch<L, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
              : direct      ? weights_launch<Md, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
                            : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
     } else {
-        rc = big ? weights_launch<L, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
-                 : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
+        rc = weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
     }
     if (rc != WM_OK || splits == 1) return rc;
     const long long count = (long long)G * N * K;

@@ -101,18 +101,14 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restr
 }
 
 template <class E, class S, bool DIRECT>
-__global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
-                                                           const int8_t *__restrict__ W, const float *__restrict__ wscale,
-                                                           const float *__restrict__ bias, E *__restrict__ y,
-                                                           const long long *__restrict__ offsets, int G, int M, int N, int K, int relu, int band)
+__device__ __forceinline__ void i8_tile(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
+                                        const int8_t *__restrict__ W, const float *__restrict__ wscale, const float *__restrict__ bias,
+                                        E *__restrict__ y, char *lds, Segment s, int n0, int G, int M, int N, int K, int relu)
 {
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    int rt, ct;
-    const RowTiles<BM> tiles(offsets, G, M);
-    if (!tile_of_block(blockIdx.x, tiles.total, (N + BN - 1) / BN, band, rt, ct)) return;
-    const Segment s = tiles.tile(rt);
-    const int n0 = min(ct * BN, max(0, N - BN)), cols = min(BN, N);         // the last tile moves back over its neighbour
+    s.rows = min(s.rows, BM);
+    const int cols = min(BN, N - n0);
+    if (s.rows <= 0 || cols <= 0) return;
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
         for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) y[(long long)(s.row0 + e / cols) * N + n0 + e % cols] = (E)0.0f;
         return;
@@ -159,6 +155,30 @@ __global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__re
             }
             O::store(to + (long long)O::row(m, t) * N, have, v[t]);
         }
+    }
+}
+
+template <class E, class S, class Sub, bool DIRECT>
+__global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
+                                                              const int8_t *__restrict__ W, const float *__restrict__ wscale,
+                                                              const float *__restrict__ bias, E *__restrict__ y,
+                                                              const long long *__restrict__ offsets, int G, int M, int N, int K, int relu, int slots)
+{
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+    const RowTiles<S::BM> tiles(offsets, G, M);
+    const int across = (N + S::BN - 1) / S::BN;
+    const Cut<S, Sub> cut(blockIdx.x, tiles.total * across, slots);
+    if (cut.tile < 0) return;
+    int rt, ct;
+    place_of_tile(cut.tile, tiles.total, across, 8, rt, ct);
+    Segment s = tiles.tile(rt);
+    const int n0 = min(ct * S::BN, max(0, N - S::BN));       // the last tile moves back over its neighbour
+    if (!cut.part) {
+        i8_tile<E, S, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0, G, M, N, K, relu);
+    } else {
+        s.row0 += cut.row;
+        s.rows -= cut.row;
+        i8_tile<E, Sub, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0 + cut.col, G, M, N, K, relu);
     }
 }
 
@@ -244,14 +264,15 @@ template <class E> int quantize(const void *x, int M, int K, int8_t *q, long lon
     return WM_OK;
 }
 
-template <class E, class S, bool DIRECT>
+template <class E, class S, class Sub, bool DIRECT>
 int dense_tiles(const int8_t *q, long long ldq, const float *scale, const int8_t *W, const float *wscale, const float *b, void *y,
                 const int64_t *offsets, int G, int M, int N, int K, int relu, hipStream_t st)
 {
-    const long long blocks = row_tiles_most(G, M, S::BM) * ((N + S::BN - 1) / S::BN);
+    const int slots = wm_num_cus() * (S::LDS <= 80 << 10 ? 2 : 1);
+    const long long blocks = Cut<S, Sub>::blocks(row_tiles_most(G, M, S::BM) * ((N + S::BN - 1) / S::BN), slots);
     WM_REQUIRE(blocks <= (1ll << 32) / 512 - 1, WM_ERR_UNSUPPORTED, "wm_dense_i8: %lld tiles are too many for one launch", blocks);
-    hipLaunchKernelGGL((dense_i8_kernel<E, S, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
-                       (const long long *)offsets, G, M, N, K, relu, 8);
+    hipLaunchKernelGGL((dense_i8_kernel<E, S, Sub, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
+                       (const long long *)offsets, G, M, N, K, relu, slots);
     WM_LAUNCH_CHECK("dense_i8_kernel");
     return WM_OK;
 }
@@ -272,10 +293,10 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     }
     if (direct_ok(W, K)) {
         if (M / G >= 512 && N >= 512)
-            return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
-        return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+            return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, Shape<I8, 128, 256, 2, 4>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+        return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
     }
-    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2>, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
 }
 
 }  // namespace

@@ -658,16 +658,59 @@ inline long long row_tiles_most(int G, int M, int BM) { return (M + (long long)(
 
 // Workgroups go round the eight XCDs in turn: logical tiles are dealt out so that an XCD works on a run of
 // them, and a run keeps to `band` row tiles and walks the columns, so that its operands stay in its L2.
-__device__ __forceinline__ bool tile_of_block(int block, int row_tiles, int col_tiles, int band, int &rt, int &ct)
+__device__ __forceinline__ void place_of_tile(int t, int row_tiles, int col_tiles, int band, int &rt, int &ct)
 {
-    const int total = row_tiles * col_tiles;
-    if (block >= total) return false;
-    const int per = total / 8, extra = total % 8, xcd = block % 8, k = block / 8;
-    const int id = xcd * per + min(xcd, extra) + k;
+    const int total = row_tiles * col_tiles, per = total / 8, extra = total % 8, xcd = t % 8;
+    const int id = xcd * per + min(xcd, extra) + t / 8;
     const int b = id / (band * col_tiles), in = id - b * band * col_tiles, height = min(band, row_tiles - b * band);
     rt = b * band + in % height;
     ct = in / height;
-    return true;
+}
+
+// The work of a workgroup: a tile of S, or part of one.  `slots` workgroups run at once; the tiles that are left when they
+// have been filled a whole number of times are cut into tiles of Sub where those find room at once, so that a
+// launch ends after a part of a tile's time instead of a whole one.
+template <class S, class Sub> struct Cut {
+    static constexpr int ACROSS = S::BN / Sub::BN, PARTS = S::BM / Sub::BM * ACROSS;
+    static_assert(S::THREADS == Sub::THREADS && Sub::LDS <= S::LDS, "one launch");
+    int tile, row, col;                      // tile < 0: nothing; row and col of the part in it
+    bool part;
+    __device__ __forceinline__ Cut(int block, int total, int slots)
+    {
+        const int left = total % slots, whole = left * PARTS <= slots ? total - left : total;
+        part = block >= whole;
+        const int k = part ? block - whole : 0;
+        tile = part ? whole + k / PARTS : block;
+        row = k % PARTS / ACROSS * Sub::BM;
+        col = k % PARTS % ACROSS * Sub::BN;
+        if (tile >= total) tile = -1;
+    }
+    static long long blocks(long long total_most, int slots) { return total_most + (long long)slots / PARTS * (PARTS - 1); }
+};
+
+// The order in which the groups' products over rows are taken up: the longest first, so that a launch does not end on one of
+// them; where two workgroups share a CU from the start (`first` groups are begun on empty CUs), the shortest are put beside the
+// longest.  More than 62 groups are taken as they come.  Gives the group and its rows.
+__device__ __forceinline__ void group_in_turn(const long long *offsets, int G, int M, int turn, int first, int &g, int &row0, int &rows)
+{
+    if (G > 62) {
+        g = turn;
+        group_rows(offsets, G, M, g, row0, rows);
+        return;
+    }
+    int lo, hi;
+    segment_bounds(offsets, G, M, 0, 0, lo, hi);
+    const int lane = threadIdx.x & 63, size = hi - lo;
+    int rank = 0;
+    for (int j = 1; j <= G; ++j) {
+        const int other = lane_value(size, j);
+        rank += other > size || (other == size && j < lane) ? 1 : 0;
+    }
+    const int want = turn < first ? turn : G - 1 - (turn - first);
+    const int k = __builtin_ctzll(__ballot(lane >= 1 && lane <= G && rank == want));
+    g = k - 1;
+    row0 = lane_value(lo, k);
+    rows = lane_value(hi, k) - row0;
 }
 
 }  // namespace tile
