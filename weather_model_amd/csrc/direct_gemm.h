@@ -96,6 +96,36 @@ template <class T, int ROWS, int THREADS> struct DirectCols {
         at += STEP * ld;
         left -= STEP * ld;
     }
+    // Sums over c of two rows of the tile, threadIdx.x % (ROWS / 2) * 2 and the next, over the 8 c that fall to this thread:
+    // the sums of a stage are spread evenly over all threads, as one thread that is late holds up the barrier for all.
+    static __device__ __forceinline__ void add_up(const char *lds, float (&sum)[2])
+    {
+        static_assert(THREADS == 2 * ROWS, "8 c a thread");
+        const int pair = threadIdx.x % (ROWS / 2), c0 = threadIdx.x / (ROWS / 2) * 8;
+        uint32_t v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = *reinterpret_cast<const uint32_t *>(lds + (c0 + e) * (ROWS * 2) + ((pair / 8 ^ mix(c0 + e)) << 5) + pair % 8 * 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sum[0] += to_float(__builtin_bit_cast(typename T::elem, (uint16_t)v[e]));
+            sum[1] += to_float(__builtin_bit_cast(typename T::elem, (uint16_t)(v[e] >> 16)));
+        }
+    }
+    // their total, of row threadIdx.x < ROWS, in a fixed order; LDS holds 4 x ROWS floats
+    static __device__ __forceinline__ float total(float *lds, const float (&sum)[2])
+    {
+        const int pair = threadIdx.x % (ROWS / 2);
+        float *own = lds + threadIdx.x / (ROWS / 2) * ROWS + 2 * pair;
+        own[0] = sum[0];
+        own[1] = sum[1];
+        __syncthreads();
+        float s = 0.0f;
+        if (threadIdx.x < ROWS)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += lds[k * ROWS + threadIdx.x];
+        return s;
+    }
     static __device__ __forceinline__ u32x4 read(const char *lds, int row)
     {
         typedef short s4 __attribute__((ext_vector_type(4)));
@@ -127,16 +157,6 @@ template <class S, class DA, class DB> struct DirectFragments {
 #pragma unroll
             for (int n = 0; n < S::NI; ++n) acc[m][n] = T::mma(a[n], b[m], acc[m][n]);
     }
-    // adds the values of B's rows over this lane's c
-    __device__ __forceinline__ void add_up(float (&sum)[S::MI]) const
-    {
-#pragma unroll
-        for (int m = 0; m < S::MI; ++m)
-#pragma unroll
-            for (int d = 0; d < 4; ++d)
-                sum[m] += to_float(__builtin_bit_cast(typename T::elem, (uint16_t)b[m][d])) +
-                          to_float(__builtin_bit_cast(typename T::elem, (uint16_t)(b[m][d] >> 16)));
-    }
 };
 
 // Stage s is multiplied from registers while the operands of stage s + 1 are read.  The one barrier a stage lies before
@@ -144,18 +164,16 @@ template <class S, class DA, class DB> struct DirectFragments {
 // ring takes stage s + RING.  The loads behind the last stage are issued all the same, to a place that nobody reads
 // and with nothing in their bounds, so that the count of loads in flight is always the same.
 // A wave whose rows (of B, `rows` exist) all lie behind the end only takes part in the loads.
-// SUMS: sum[m] becomes the sum of B's row m over the c of this wave's share of the stages, every WN-th.
-template <class S, int RING, bool SUMS = false, class DA, class DB>
-__device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows, char *lds, typename S::Acc &acc, float *sum = nullptr)
+// SUMS: B's rows (DirectCols) are summed over c as well, into this thread's `sum`.
+template <class S, int RING, bool SUMS, class DA, class DB>
+__device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows, char *lds, typename S::Acc &acc, float (&sum)[2])
 {
     constexpr int STEP = DA::STEP, STAGE = DA::BYTES + DB::BYTES;
     static_assert(DA::STEP == DB::STEP, "one step for both operands");
     constexpr int MFMA = S::NI * S::MI, READS = S::NI * DA::READS + S::MI * DB::READS;
     const uint32_t base = lds_address(lds);
     DirectFragments<S, DA, DB> f[2];
-    float add[S::MI] = {};
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int turn = wave % S::WN;
 #pragma unroll
     for (int k = 0; k < RING; ++k) {
         a.issue(base + k * STAGE);
@@ -171,8 +189,9 @@ __device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows
         b.issue(base + here + DA::BYTES);
         here = here == (RING - 1) * STAGE ? 0 : here + STAGE;
     };
-    if (wave / S::WN * (S::BM / S::WM) < rows) {
+    if (SUMS || wave / S::WN * (S::BM / S::WM) < rows) {
         f[0].read(lds);
+        if constexpr (SUMS) DB::add_up(lds + DA::BYTES, sum);
         for (int c0 = 0; c0 < count; c0 += 2 * STEP) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) {    // an odd number of stages ends with one of zeros
@@ -180,10 +199,7 @@ __device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows
                 f[k ^ 1].read(lds + here);
                 f[k].multiply(acc);
                 interleave<MFMA, READS, 0, 0>();
-                if constexpr (SUMS) {
-                    if (turn == 0) f[k].add_up(add);
-                    turn = turn == 0 ? S::WN - 1 : turn - 1;
-                }
+                if constexpr (SUMS) DB::add_up(lds + here + DA::BYTES, sum);
             }
         }
     } else {
@@ -194,15 +210,12 @@ __device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows
     }
     wait_loads<0>();
     __syncthreads();
-    if constexpr (SUMS) {                    // lanes i, i + 16, i + 32, i + 48 hold the row's four parts
-#pragma unroll
-        for (int m = 0; m < S::MI; ++m) {
-            float v = add[m];
-            v += __shfl_xor(v, 16, 64);
-            v += __shfl_xor(v, 32, 64);
-            sum[m] = v;
-        }
-    }
+}
+template <class S, int RING, class DA, class DB>
+__device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows, char *lds, typename S::Acc &acc)
+{
+    float none[2];
+    product_direct<S, RING, false>(a, b, count, rows, lds, acc, none);
 }
 
 inline bool direct_ok(const void *p, long long ld_bytes) { return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0; }

@@ -156,28 +156,18 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
         else gb[(long long)g * N + n0 + j] = from_float<E>(v);
     };
     if constexpr (DIRECT) {
-        float sum[MI] = {};
+        float sum[2] = {0.0f, 0.0f};
         if (rows > 0) {
             DirectCols<T, BN, THREADS> a;
             DirectCols<T, BM, THREADS> b;
             a.init(xt, K, ks, rows, nullptr);
             b.init(yt, N, ns, rows, nullptr);
-            // the sums cost registers and branches: their own code
             if (sums) product_direct<S, S::RING, true>(a, b, rows, ns, lds, acc, sum);
             else product_direct<S, S::RING>(a, b, rows, ns, lds, acc);
         }
         if (sums) {
-            // sum: of every WN-th stage; the waves of a row of waves are joined in order
-            float *part = (float *)lds;
-            if ((threadIdx.x & 63) < 16)
-#pragma unroll
-                for (int m = 0; m < MI; ++m) part[S::wave_col() * BM + S::row() + 16 * m] = sum[m];
-            __syncthreads();
-            float v = 0.0f;
-            if ((int)threadIdx.x < BM)
-#pragma unroll
-                for (int w = 0; w < S::WN; ++w) v += part[w * BM + threadIdx.x];
-            if ((int)threadIdx.x < BM) bias(threadIdx.x, v);
+            const float total = DirectCols<T, BM, THREADS>::total((float *)lds, sum);
+            if ((int)threadIdx.x < BM) bias(threadIdx.x, total);
         }
     } else {
         float total = 0.0f;
