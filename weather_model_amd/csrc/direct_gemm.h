@@ -69,7 +69,8 @@ template <class T, int ROWS, int THREADS> struct DirectRows {
 };
 
 template <class T, int ROWS, int THREADS> struct DirectCols {
-    static constexpr int BYTES = ROWS * 64, SLOTS = ROWS / 8, N = BYTES / (THREADS * 16), STEP = 32, READS = 2, HOP = THREADS / SLOTS;
+    static constexpr int BYTES = ROWS * 64, SLOTS = ROWS / 8, N = BYTES / (THREADS * 16), STEP = 32, READS = 2, HOP = THREADS / SLOTS,
+                         SHARE = STEP * ROWS / 2 / THREADS;
     static_assert(sizeof(typename T::elem) == 2 && HOP % 8 == 0, "16-bit types");
     const char *at;
     long long ld, left;                      // bytes; left: from `at` to the end of the last c's part of this tile
@@ -96,23 +97,22 @@ template <class T, int ROWS, int THREADS> struct DirectCols {
         at += STEP * ld;
         left -= STEP * ld;
     }
-    // Sums over c of two rows of the tile, threadIdx.x % (ROWS / 2) * 2 and the next, over the 8 c that fall to this thread:
+    // Sums over c of two rows of the tile, threadIdx.x % (ROWS / 2) * 2 and the next, over the SHARE c that fall to this thread:
     // the sums of a stage are spread evenly over all threads, as one thread that is late holds up the barrier for all.
     static __device__ __forceinline__ void add_up(const char *lds, float (&sum)[2])
     {
-        static_assert(THREADS == 2 * ROWS, "8 c a thread");
-        const int pair = threadIdx.x % (ROWS / 2), c0 = threadIdx.x / (ROWS / 2) * 8;
-        uint32_t v[8];
+        const int pair = threadIdx.x % (ROWS / 2), c0 = threadIdx.x / (ROWS / 2) * SHARE;
+        uint32_t v[SHARE];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < SHARE; ++e)
             v[e] = *reinterpret_cast<const uint32_t *>(lds + (c0 + e) * (ROWS * 2) + ((pair / 8 ^ mix(c0 + e)) << 5) + pair % 8 * 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < SHARE; ++e) {
             sum[0] += to_float(__builtin_bit_cast(typename T::elem, (uint16_t)v[e]));
             sum[1] += to_float(__builtin_bit_cast(typename T::elem, (uint16_t)(v[e] >> 16)));
         }
     }
-    // their total, of row threadIdx.x < ROWS, in a fixed order; LDS holds 4 x ROWS floats
+    // their total, of row threadIdx.x < ROWS, in a fixed order; LDS holds 32 / SHARE x ROWS floats
     static __device__ __forceinline__ float total(float *lds, const float (&sum)[2])
     {
         const int pair = threadIdx.x % (ROWS / 2);
@@ -123,7 +123,7 @@ template <class T, int ROWS, int THREADS> struct DirectCols {
         float s = 0.0f;
         if (threadIdx.x < ROWS)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s += lds[k * ROWS + threadIdx.x];
+            for (int k = 0; k < STEP / SHARE; ++k) s += lds[k * ROWS + threadIdx.x];
         return s;
     }
     static __device__ __forceinline__ u32x4 read(const char *lds, int row)

@@ -97,7 +97,7 @@ __device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__re
 }
 
 template <class S, class Sub, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
-__global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
+__global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
                                                                   const E *__restrict__ mask, E *__restrict__ out,
                                                                   const long long *__restrict__ offsets, int G, int M, int NO, int C, int relu,
                                                                   int slots)
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_rows_kernel(const E *__res
 // with S > 1 the shares go to `partial` (S, G, N, K), and to (S, G, N) behind it, and grouped_weights_sum_kernel adds
 // them in order.  gb is summed by the workgroups of the first columns from the registers that feed LDS.
 template <class S, bool DIRECT, class E = typename S::T::elem>
-__global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
+__global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
                                                                      E *__restrict__ gb, float *__restrict__ partial, const long long *__restrict__ offsets, int G,
                                                                      int M, int N, int K, int splits, int first)
 {
@@ -175,7 +175,7 @@ __global__ __launch_bounds__(S::THREADS) void grouped_weights_kernel(const E *__
             static_assert(BM == BN, "a pair");
             StridedPair<T, BM, THREADS> pair;
             Nothing<T> none;
-            pair.init(xt, K, ks, yt, N, ns, rows);
+            pair.init(xt, K, ks, x + (long long)M * K, yt, N, ns, gy + (long long)M * N, rows);
             product<S, true>(pair, none, rows, lds, acc, sums);
             if (sums) total = pair.total((float *)lds);
         }
@@ -316,11 +316,11 @@ template <class T> struct Tiles {                       // 16-bit types
     typedef Shape<T, 256, 256, 2, 4> Large;
     typedef Shape<T, 128, 256, 2, 4> LargePart;
     typedef Shape<T, 128, 128, 2, 2> Medium;
-    typedef Shape<T, 64, 64, 2, 2> MediumPart;
+    typedef Shape<T, 64, 64, 2, 2, 2, 2> MediumPart;
 };
 template <> struct Tiles<F32> {
     typedef Shape<F32, 128, 128, 2, 2, 1> Medium;
-    typedef Shape<F32, 64, 64, 2, 2, 1> MediumPart;
+    typedef Shape<F32, 64, 64, 2, 2, 1, 2> MediumPart;
 };
 
 bool large(int G, int M, int N) { return M / G >= 512 && N >= 512; }

@@ -159,7 +159,7 @@ __device__ __forceinline__ void i8_tile(const int8_t *__restrict__ q, long long 
 }
 
 template <class E, class S, class Sub, bool DIRECT>
-__global__ __launch_bounds__(S::THREADS) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
+__global__ __launch_bounds__(S::THREADS, 2) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
                                                               const int8_t *__restrict__ W, const float *__restrict__ wscale,
                                                               const float *__restrict__ bias, E *__restrict__ y,
                                                               const long long *__restrict__ offsets, int G, int M, int N, int K, int relu, int slots)
@@ -294,9 +294,9 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     if (direct_ok(W, K)) {
         if (M / G >= 512 && N >= 512)
             return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, Shape<I8, 128, 256, 2, 4>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
-        return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+        return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2, 2, 2>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
     }
-    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2>, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2, 2, 2>, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
 }
 
 }  // namespace

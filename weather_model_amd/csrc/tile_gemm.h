@@ -128,16 +128,24 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t out[3])
     }
 }
 
-// ---- an operand with c along memory: rows of `ld` elements, ROWS of them a tile
+// ---- operands.  load() brings a step of STEP values of c into registers without looking at the end of c; what lies behind the
+// end is made zero by trim() before store().  That reads up to STEP - 1 values too many, which `safe` says lie within the
+// tensor; where they do not, the last step takes load_guarded(), which reads nothing beyond what it is to read.
+
+// c along memory: rows of `ld` elements, ROWS of them a tile
 template <class T, int ROWS, int THREADS> struct Contiguous {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * T::ECH, PER = ROWS * BKC / THREADS, LOADS = T::PLANES == 3 ? 2 : 1;
     static constexpr int N_LOADS = PER * LOADS, N_STORES = PER * T::PLANES;      // instructions of load() and store()
     static_assert(PER >= 1, "tile too small for the workgroup");
-    u32x4 reg[PER][LOADS];
+    struct Regs {
+        u32x4 v[PER][LOADS];
+    };
     const E *base, *end;                     // (row 0 of the tile, c = 0) and the end of the tensor
     uint32_t off[PER];                       // element offset of this thread's rows, chunk included
     int q, count;                            // count: values of c there are
+    bool safe;
+    static constexpr bool slow = false;      // every whole step can take load()
 
     // rows_left >= 1: rows from row0 on that exist; later ones repeat the last
     __device__ __forceinline__ void init(const E *tensor_row0, long long ld, int rows_left, int c_count, const E *tensor_end)
@@ -146,43 +154,57 @@ template <class T, int ROWS, int THREADS> struct Contiguous {
         end = tensor_end;
         count = c_count;
         q = threadIdx.x % BKC;
+        safe = end - base >= (long long)(min(ROWS, rows_left) - 1) * ld + (c_count + STEP - 1) / STEP * STEP;
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int r = threadIdx.x / BKC + j * (THREADS / BKC);
             off[j] = (uint32_t)((long long)min(r, rows_left - 1) * ld) + (uint32_t)(q * T::ECH);
         }
     }
-    static constexpr bool slow = false;      // every whole step can take load()
-    __device__ __forceinline__ void load(int c0)
+    __device__ __forceinline__ void load(Regs &reg, int c0) const
     {
         const E *at = base + c0;
 #pragma unroll
         for (int j = 0; j < PER; ++j)
 #pragma unroll
-            for (int h = 0; h < LOADS; ++h) reg[j][h] = *reinterpret_cast<const u32x4u *>(at + off[j] + h * 4);
+            for (int h = 0; h < LOADS; ++h) reg.v[j][h] = *reinterpret_cast<const u32x4u *>(at + off[j] + h * 4);
     }
-    __device__ __forceinline__ void load_guarded(int c0)
+    __device__ __forceinline__ void trim(Regs &reg, int c0) const
+    {
+#pragma unroll
+        for (int h = 0; h < LOADS; ++h) {
+            const int bytes = (count - c0 - q * T::ECH) * (int)sizeof(E) - h * 16;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const int keep = bytes - 4 * d;
+                const uint32_t m = keep >= 4 ? 0xFFFFFFFFu : keep <= 0 ? 0u : (1u << (8 * keep)) - 1u;
+#pragma unroll
+                for (int j = 0; j < PER; ++j) reg.v[j][h][d] &= m;
+            }
+        }
+    }
+    __device__ __forceinline__ void load_guarded(Regs &reg, int c0) const
     {
         const E *at = base + c0;
 #pragma unroll
         for (int j = 0; j < PER; ++j)
 #pragma unroll
             for (int h = 0; h < LOADS; ++h)
-                reg[j][h] = load16_guarded<E>(at + off[j] + h * 4, end, count - c0 - q * T::ECH - h * 4);
+                reg.v[j][h] = load16_guarded<E>(at + off[j] + h * 4, end, count - c0 - q * T::ECH - h * 4);
     }
-    __device__ __forceinline__ void store(char *lds)
+    __device__ __forceinline__ void store(const Regs &reg, char *lds) const
     {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const int r = threadIdx.x / BKC + j * (THREADS / BKC);
             if constexpr (T::PLANES == 1) {
-                *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = reg[j][0];
+                *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = reg.v[j][0];
             } else {
                 u32x4 piece[3];
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     uint32_t o[3];
-                    const f32x4 f = __builtin_bit_cast(f32x4, reg[j][d / 2]);
+                    const f32x4 f = __builtin_bit_cast(f32x4, reg.v[j][d / 2]);
                     split2(f[2 * (d & 1)], f[2 * (d & 1) + 1], o);
 #pragma unroll
                     for (int p = 0; p < 3; ++p) piece[p][d] = o[p];
@@ -195,8 +217,7 @@ template <class T, int ROWS, int THREADS> struct Contiguous {
     }
 };
 
-// ---- an operand with the tile's rows along memory: element (row r, c) at base + c * ld + r; THREADS of the workgroup load it,
-// from number `first` on
+// the tile's rows along memory: element (row r, c) at base + c * ld + r; THREADS of the workgroup load it, from number `first` on
 template <class T, int ROWS, int THREADS> struct Strided {
     typedef typename T::elem E;
     static constexpr int BKC = T::BKC, STEP = BKC * 8, BLOCKS = THREADS / BKC, W = ROWS / BLOCKS;   // W rows x 8 c a thread
@@ -204,15 +225,18 @@ template <class T, int ROWS, int THREADS> struct Strided {
     static constexpr int N_LOADS = 8, N_STORES = W * T::PLANES;
     static_assert(WORDS >= 1 && T::ECH == 8, "tile too small for the workgroup");
     typedef uint32_t words __attribute__((ext_vector_type(WORDS), aligned(sizeof(E))));
-    uint32_t reg[8][WORDS];
+    struct Regs {
+        uint32_t v[8][WORDS];
+    };
     const E *base;
     long long ld;
     int r0, q, count;
     float sum[W];                            // of what add_up() saw
     int most;                                // rows that exist, at least 1
+    bool safe;
     bool slow;                               // fewer rows than a thread's vector: load() does not fit (workgroup-uniform)
 
-    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *, int first = 0)
+    __device__ __forceinline__ void init(const E *tensor_row0, long long ld_, int rows_left, int c_count, const E *end, int first = 0)
     {
         base = tensor_row0;
         ld = ld_;
@@ -220,28 +244,36 @@ template <class T, int ROWS, int THREADS> struct Strided {
         q = threadIdx.x % BKC;
         most = rows_left;
         slow = rows_left < W;
+        safe = end - base >= ((c_count + STEP - 1) / STEP * STEP - 1) * ld + min(ROWS, rows_left);
 #pragma unroll
         for (int i = 0; i < W; ++i) sum[i] = 0.0f;
         // a vector that would leave the rows moves back into them: two threads then write the same values to the
         // same place, and rows that do not exist keep whatever LDS held (their results are not stored)
         r0 = slow ? 0 : min(((int)threadIdx.x - first) / BKC * W, rows_left - W);
     }
-    __device__ __forceinline__ void load(int c0)
+    __device__ __forceinline__ void load(Regs &reg, int c0) const
     {
         const E *at = base + (long long)c0 * ld;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const E *p = at + e * ld + (uint32_t)(q * 8 * (int)ld + r0);       // scalar base, one offset register
             if constexpr (WORDS == 1) {
-                reg[e][0] = *reinterpret_cast<const u32u *>(p);
+                reg.v[e][0] = *reinterpret_cast<const u32u *>(p);
             } else {
                 const words v = *reinterpret_cast<const words *>(p);
 #pragma unroll
-                for (int w = 0; w < WORDS; ++w) reg[e][w] = v[w];
+                for (int w = 0; w < WORDS; ++w) reg.v[e][w] = v[w];
             }
         }
     }
-    __device__ __forceinline__ void load_guarded(int c0)
+    __device__ __forceinline__ void trim(Regs &reg, int c0) const
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) reg.v[e][w] = c0 + q * 8 + e < count ? reg.v[e][w] : 0u;
+    }
+    __device__ __forceinline__ void load_guarded(Regs &reg, int c0) const
     {
         const E *at = base + (long long)c0 * ld;
 #pragma unroll
@@ -256,22 +288,22 @@ template <class T, int ROWS, int THREADS> struct Strided {
                         if constexpr (PER_WORD == 1) v = __builtin_bit_cast(uint32_t, *p);
                         else v |= (uint32_t)__builtin_bit_cast(uint16_t, *p) << (16 * i);
                     }
-                reg[e][w] = v;
+                reg.v[e][w] = v;
             }
     }
     // adds what the registers hold to the sums of this thread's rows over c
-    __device__ __forceinline__ void add_up()
+    __device__ __forceinline__ void add_up(const Regs &reg)
     {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                if constexpr (sizeof(E) == 4) sum[i] += __builtin_bit_cast(float, reg[e][i]);
-                else sum[i] += to_float(__builtin_bit_cast(E, (uint16_t)(reg[e][i / 2] >> (16 * (i & 1)))));
+                if constexpr (sizeof(E) == 4) sum[i] += __builtin_bit_cast(float, reg.v[e][i]);
+                else sum[i] += to_float(__builtin_bit_cast(E, (uint16_t)(reg.v[e][i / 2] >> (16 * (i & 1)))));
             }
     }
     // the sums over all c, in a fixed order: LDS holds BKC x ROWS floats; returns that of row threadIdx.x < ROWS
-    __device__ __forceinline__ float total(float *lds, bool mine = true)
+    __device__ __forceinline__ float total(float *lds, bool mine = true) const
     {
         if (mine)
 #pragma unroll
@@ -283,7 +315,7 @@ template <class T, int ROWS, int THREADS> struct Strided {
             for (int k = 0; k < BKC; ++k) s += lds[k * ROWS + threadIdx.x];
         return s;
     }
-    __device__ __forceinline__ void store(char *lds)
+    __device__ __forceinline__ void store(const Regs &reg, char *lds) const
     {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
@@ -292,14 +324,14 @@ template <class T, int ROWS, int THREADS> struct Strided {
                 u32x4 v;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)
-                    v[d] = __builtin_amdgcn_perm(reg[2 * d + 1][i / 2], reg[2 * d][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
+                    v[d] = __builtin_amdgcn_perm(reg.v[2 * d + 1][i / 2], reg.v[2 * d][i / 2], i & 1 ? 0x07060302u : 0x05040100u);
                 *reinterpret_cast<u32x4 *>(lds + lds_at<BKC>(r, q)) = v;
             } else {
                 u32x4 piece[3];
 #pragma unroll
                 for (int d = 0; d < 4; ++d) {
                     uint32_t o[3];
-                    split2(__builtin_bit_cast(float, reg[2 * d][i]), __builtin_bit_cast(float, reg[2 * d + 1][i]), o);
+                    split2(__builtin_bit_cast(float, reg.v[2 * d][i]), __builtin_bit_cast(float, reg.v[2 * d + 1][i]), o);
 #pragma unroll
                     for (int p = 0; p < 3; ++p) piece[p][d] = o[p];
                 }
@@ -315,32 +347,39 @@ template <class T, int ROWS, int THREADS> struct Strided {
 // loads are twice as wide.  Stands in both places of product().
 template <class T, int ROWS, int THREADS> struct StridedPair : Strided<T, ROWS, THREADS / 2> {
     typedef Strided<T, ROWS, THREADS / 2> Half;
+    typedef typename T::elem E;
+    typedef typename Half::Regs Regs;
     bool second;
-    __device__ __forceinline__ void init(const typename T::elem *a, long long lda, int rows_a, const typename T::elem *b, long long ldb, int rows_b,
+    __device__ __forceinline__ void init(const E *a, long long lda, int rows_a, const E *a_end, const E *b, long long ldb, int rows_b, const E *b_end,
                                          int count)
     {
+        Half other;                          // the bounds of both halves hold for all waves
         second = __builtin_amdgcn_readfirstlane(threadIdx.x) >= THREADS / 2;
-        Half::init(second ? b : a, second ? ldb : lda, second ? rows_b : rows_a, count, nullptr, second ? THREADS / 2 : 0);
+        other.init(second ? a : b, second ? lda : ldb, second ? rows_a : rows_b, count, second ? a_end : b_end);
+        Half::init(second ? b : a, second ? ldb : lda, second ? rows_b : rows_a, count, second ? b_end : a_end, second ? THREADS / 2 : 0);
+        this->safe = this->safe && other.safe;
         this->slow = rows_a < Half::W || rows_b < Half::W;
         if (this->slow) this->r0 = ((int)threadIdx.x - (second ? THREADS / 2 : 0)) / Half::BKC * Half::W;
     }
-    __device__ __forceinline__ void store(char *lds) { Half::store(lds + (second ? ROWS * Half::BKC * 16 * T::PLANES : 0)); }
-    __device__ __forceinline__ void add_up() { if (second) Half::add_up(); }
-    __device__ __forceinline__ float total(float *lds) { return Half::total(lds, second); }
+    __device__ __forceinline__ void store(const Regs &reg, char *lds) const { Half::store(reg, lds + (second ? ROWS * Half::BKC * 16 * T::PLANES : 0)); }
+    __device__ __forceinline__ void add_up(const Regs &reg) { if (second) Half::add_up(reg); }
+    __device__ __forceinline__ float total(float *lds) const { return Half::total(lds, second); }
 };
 // the other place
 template <class T> struct Nothing {
     static constexpr int STEP = T::BKC * 8, N_LOADS = 0, N_STORES = 0;
-    static constexpr bool slow = false;
-    __device__ __forceinline__ void load(int) {}
-    __device__ __forceinline__ void load_guarded(int) {}
-    __device__ __forceinline__ void store(char *) {}
+    static constexpr bool slow = false, safe = true;
+    struct Regs {};
+    __device__ __forceinline__ void load(Regs &, int) const {}
+    __device__ __forceinline__ void load_guarded(Regs &, int) const {}
+    __device__ __forceinline__ void trim(Regs &, int) const {}
+    __device__ __forceinline__ void store(const Regs &, char *) const {}
 };
 
 // ---- a shape of tile: BM rows by BN columns of C over WM x WN waves
-template <class T_, int BM_, int BN_, int WM_, int WN_, int BUFFERS_ = 2> struct Shape {
+template <class T_, int BM_, int BN_, int WM_, int WN_, int BUFFERS_ = 2, int DEPTH_ = 1> struct Shape {
     typedef T_ T;
-    static constexpr int BUFFERS = BUFFERS_; // steps in LDS
+    static constexpr int BUFFERS = BUFFERS_, DEPTH = DEPTH_;               // steps in LDS, and in registers (product())
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, THREADS = 64 * WM * WN;
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;             // 16 x 16 results a wave
     static constexpr int A_BYTES = BN * T::BKC * 16 * T::PLANES, B_BYTES = BM * T::BKC * 16 * T::PLANES;
@@ -409,87 +448,102 @@ template <int MFMA, int READS, int STORES, int LOADS> __device__ __forceinline__
     }
 }
 
-template <class LA, class LB> __device__ __forceinline__ LB &summed(LA &, LB &b) { return b; }
-template <class LA, class T> __device__ __forceinline__ LA &summed(LA &a, Nothing<T> &) { return a; }
+template <class LA, class LB> __device__ __forceinline__ void add_up(LA &, typename LA::Regs &, LB &b, typename LB::Regs &rb) { b.add_up(rb); }
+template <class LA, class T> __device__ __forceinline__ void add_up(LA &a, typename LA::Regs &ra, Nothing<T> &, typename Nothing<T>::Regs &) { a.add_up(ra); }
 
-// Whole steps, each of SUB reads of operands: while one step is multiplied, the next goes from registers to the other
-// half of LDS and the one after that is loaded (the last steps load themselves once more instead of branching: a
-// branch around the loads makes the compiler wait for them at its end).  There is one barrier a step, before its last
-// multiplication: behind it the next step lies in LDS, so that its first operands are read under that multiplication, and
-// every wave has read the last of this step's, so that its half may be overwritten.  What is left of the last step goes through the
-// guarded loads, which put zeros behind the end on both sides.
-// `sums`: add up B's rows over c as well (a Strided operand; workgroup-uniform).
+// While one step is multiplied, the next goes from registers to LDS and later ones are loaded: S::DEPTH sets of registers hold
+// as many steps in flight (the last steps load themselves once more instead of branching: a branch around the loads makes the
+// compiler wait for them at its end).
+// Two buffers (one barrier a step, before its last multiplication): behind the barrier the next step lies in the other half of
+// LDS, so that its first operands are read under that multiplication, and every wave has read the last of this step's, so that its
+// half may be overwritten.  One buffer (two barriers a step): half the LDS, for two workgroups a CU that fill each other's waits.
+// `sums`: add up B's rows over c as well (a Strided operand or a pair; workgroup-uniform).
 template <class S, bool SUMS = false, class LA, class LB>
 __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, typename S::Acc &acc, bool sums = false)
 {
-    constexpr int STEP = LA::STEP, SUB = S::T::BKC / 4, HALF = S::A_BYTES + S::B_BYTES;
+    constexpr int STEP = LA::STEP, SUB = S::T::BKC / 4, HALF = S::A_BYTES + S::B_BYTES, D = S::DEPTH;
     static_assert(LA::STEP == LB::STEP, "one step for both operands");
-    const int full = a.slow || b.slow ? 0 : count / STEP * STEP;
-    if (full > 0) {
+    // whole steps, and the step that the loads end on: what is left behind them, if it may be read whole
+    const int steps = a.slow || b.slow ? 0 : count / STEP, rest = count - count / STEP * STEP;
+    const bool tail = rest > 0 && !a.slow && !b.slow && a.safe && b.safe;
+    const int last = steps - 1 + (tail ? 1 : 0);
+    typename LA::Regs ra[D];
+    typename LB::Regs rb[D];
+    if (last >= 0) {
         Fragments<S> f[2];
-        a.load(0);
-        b.load(0);
-        a.store(lds);
-        b.store(lds + S::A_BYTES);
-        if constexpr (SUMS)
-            if (sums) summed(a, b).add_up();
-        const int second = min(STEP, full - STEP);
-        a.load(second);
-        b.load(second);
-        __syncthreads();
-        int here = 0;
-        if constexpr (S::BUFFERS == 1) {
-            for (int c0 = 0; c0 < full; c0 += STEP) {
-#pragma unroll
-                for (int s = 0; s < SUB; ++s) {
-                    f[0].read(lds, s);
-                    f[0].multiply(acc);
-                }
-                __syncthreads();
-                a.store(lds);
-                b.store(lds + S::A_BYTES);
-                if constexpr (SUMS)
-                    if (sums && c0 + STEP < full) summed(a, b).add_up();
-                const int next = min(c0 + 2 * STEP, full - STEP);
-                a.load(next);
-                b.load(next);
-                __syncthreads();
-            }
-        }
-        if constexpr (SUB == 2 && S::BUFFERS == 2) f[0].read(lds, 0);
-        if constexpr (S::BUFFERS == 2) for (int c0 = 0; c0 < full; c0 += STEP) {
-            const int there = HALF - here;
-            f[1].read(lds + here, SUB - 1);
-            a.store(lds + there);
-            b.store(lds + there + S::A_BYTES);
+        auto load = [&](int k, int step) {
+            const int c0 = min(step, last) * STEP;
+            a.load(ra[k], c0);
+            b.load(rb[k], c0);
+        };
+        // step `step` from registers to LDS
+        auto store = [&](int k, int step, char *to) {
             if constexpr (SUMS)
-                if (sums && c0 + STEP < full) summed(a, b).add_up();
-            const int next = min(c0 + 2 * STEP, full - STEP);
-            a.load(next);
-            b.load(next);
-            if constexpr (SUB == 2) {
-                f[0].multiply(acc);
-                interleave<Fragments<S>::N_MFMA, Fragments<S>::N_READS, LA::N_STORES + LB::N_STORES, LA::N_LOADS + LB::N_LOADS>();
-                __syncthreads();
-                f[0].read(lds + there, 0);
-                f[1].multiply(acc);
-                interleave<Fragments<S>::N_MFMA, Fragments<S>::N_READS, 0, 0>();
-            } else {
-                f[1].multiply(acc);
-                __syncthreads();
+                if (sums && step < steps) add_up(a, ra[k], b, rb[k]);
+            a.store(ra[k], to);
+            b.store(rb[k], to + S::A_BYTES);
+        };
+#pragma unroll
+        for (int k = 0; k < D; ++k) load(k, k);
+        if (steps > 0) {
+            store(0, 0, lds);
+            load(0, D);
+            __syncthreads();
+            int here = 0;
+            if constexpr (SUB == 2 && S::BUFFERS == 2) f[0].read(lds, 0);
+            for (int t0 = 0; t0 < steps; t0 += D) {
+#pragma unroll
+                for (int k = 0; k < D; ++k) {
+                    const int t = t0 + k, set = (k + 1) % D;
+                    if (k > 0 && t >= steps) break;
+                    if constexpr (S::BUFFERS == 1) {
+#pragma unroll
+                        for (int s = 0; s < SUB; ++s) {
+                            f[0].read(lds, s);
+                            f[0].multiply(acc);
+                        }
+                        __syncthreads();
+                        store(set, t + 1, lds);
+                        load(set, t + 1 + D);
+                        __syncthreads();
+                    } else {
+                        const int there = HALF - here;
+                        f[1].read(lds + here, SUB - 1);
+                        store(set, t + 1, lds + there);
+                        load(set, t + 1 + D);
+                        if constexpr (SUB == 2) {
+                            f[0].multiply(acc);
+                            interleave<Fragments<S>::N_MFMA, Fragments<S>::N_READS, LA::N_STORES + LB::N_STORES, LA::N_LOADS + LB::N_LOADS>();
+                            __syncthreads();
+                            f[0].read(lds + there, 0);
+                            f[1].multiply(acc);
+                            interleave<Fragments<S>::N_MFMA, Fragments<S>::N_READS, 0, 0>();
+                        } else {
+                            f[1].multiply(acc);
+                            __syncthreads();
+                        }
+                        here = there;
+                    }
+                }
             }
-            here = there;
+            __syncthreads();
         }
-        __syncthreads();
+        if (tail) {                          // every set of registers holds it by now
+            a.trim(ra[0], last * STEP);
+            b.trim(rb[0], last * STEP);
+        }
     }
-    for (int c0 = full; c0 < count; c0 += STEP) {
+    // what is left of the last step, from where the loads above ended or through the guarded loads
+    for (int c0 = steps * STEP; c0 < count; c0 += STEP) {
         Fragments<S> f;
-        a.load_guarded(c0);
-        b.load_guarded(c0);
+        if (!tail) {
+            a.load_guarded(ra[0], c0);
+            b.load_guarded(rb[0], c0);
+        }
         if constexpr (SUMS)
-            if (sums) summed(a, b).add_up();
-        a.store(lds);
-        b.store(lds + S::A_BYTES);
+            if (sums) add_up(a, ra[0], b, rb[0]);
+        a.store(ra[0], lds);
+        b.store(rb[0], lds + S::A_BYTES);
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
