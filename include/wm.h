@@ -465,7 +465,7 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
  * gb.  Any values of offsets are safe: those outside 0 .. M count as the nearest inside, one below its
  * predecessor counts as that.  Results are bitwise reproducible.  float32 products are formed from three
  * bf16 pieces of each factor, with float32 accuracy; infinities and NaN come out as in float32 arithmetic.
- * N, K <= 2^20, M <= 2^30, G <= 2^16. */
+ * N, K <= 2^20, M <= 2^30, G < 2^16. */
 int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, const int64_t *offsets,
                          int G, int M, int N, int K, int dtype, int relu, void *stream);
 int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx,

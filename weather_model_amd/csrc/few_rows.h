@@ -26,42 +26,65 @@ template <class T> __device__ __forceinline__ typename T::acc piece(u32x4 a, u32
     }
 }
 
-// this wave's share of the products of matrix row w (i = lane & 15: four consecutive rows of the result per lane)
-// with row x; rows that do not exist are given as any that do
-template <class T>
-__device__ __forceinline__ typename T::acc dot(const typename T::elem *w, const typename T::elem *wend, const typename T::elem *x,
-                                               const typename T::elem *xend, int K)
-{
+// This wave's share of the products of matrix row w (i = lane & 15: four consecutive rows of the result per lane) with a row of x;
+// rows that do not exist are given as any that do.  x(c, left) gives the piece of the row from value c on, of which `left` count.
+// begin() may be called long before multiply(): the first loads of the weights are then under way.
+template <class T> struct Dot {
     typedef typename T::elem E;
-    constexpr int ROUND = 128 / sizeof(E), PIECE = 16 / sizeof(E);
-    const int g = (threadIdx.x & 63) >> 4, wave = threadIdx.x >> 6;
-    typename T::acc acc = {0, 0, 0, 0};
-    const int rounds = K / ROUND;
-    w += g * 2 * PIECE;
-    x += g * 2 * PIECE;
-    int r = wave;
-    for (; r + (UNROLL - 1) * WAVES < rounds; r += UNROLL * WAVES) {
-        u32x4 a[UNROLL][2], b[UNROLL][2];
+    static constexpr int ROUND = 128 / sizeof(E), PIECE = 16 / sizeof(E);
+    const E *w, *end;
+    int K, rounds;
+    u32x4 a[UNROLL][2];
+    static __device__ __forceinline__ int at() { return (int)((threadIdx.x & 63) >> 4) * 2 * PIECE; }      // of this lane in a round
+    __device__ __forceinline__ void load(int r)
+    {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) a[u][h] = *reinterpret_cast<const u32x4u *>(w + (r + u * WAVES) * ROUND + h * PIECE);
+    }
+    __device__ __forceinline__ bool batch(int r) const { return r + (UNROLL - 1) * WAVES < rounds; }
+    __device__ __forceinline__ void begin(const E *row, const E *tensor_end, int K_)
+    {
+        w = row + at();
+        end = tensor_end;
+        K = K_;
+        rounds = K / ROUND;
+        if (batch(threadIdx.x >> 6)) load(threadIdx.x >> 6);
+    }
+    template <class X> __device__ __forceinline__ typename T::acc multiply(X x)
+    {
+        typename T::acc acc = {0, 0, 0, 0};
+        int r = threadIdx.x >> 6;
+        for (bool there = true; batch(r); r += UNROLL * WAVES, there = false) {
+            u32x4 b[UNROLL][2];
+            if (!there) load(r);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) b[u][h] = x((r + u * WAVES) * ROUND + h * PIECE + at(), PIECE);
+#pragma unroll
+            for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) acc = piece<T>(a[u][h], b[u][h], acc);
+        }
+        for (; r * ROUND < K; r += WAVES)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                a[u][h] = *reinterpret_cast<const u32x4u *>(w + (r + u * WAVES) * ROUND + h * PIECE);
-                b[u][h] = *reinterpret_cast<const u32x4u *>(x + (r + u * WAVES) * ROUND + h * PIECE);
+                const int c = r * ROUND + h * PIECE, left = K - c - at();
+                acc = piece<T>(load16_guarded<E>(w + c, end, left), x(c + at(), left), acc);
             }
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) acc = piece<T>(a[u][h], b[u][h], acc);
+        return acc;
     }
-    for (; r * ROUND < K; r += WAVES) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c = r * ROUND + h * PIECE, left = K - c - g * 2 * PIECE;
-            acc = piece<T>(load16_guarded<E>(w + c, wend, left), load16_guarded<E>(x + c, xend, left), acc);
-        }
+};
+// x as a row in memory
+template <class T> struct RowOf {
+    const typename T::elem *x, *end;
+    __device__ __forceinline__ u32x4 operator()(int c, int left) const
+    {
+        if (left >= (int)(16 / sizeof(typename T::elem))) return *reinterpret_cast<const u32x4u *>(x + c);
+        return load16_guarded<typename T::elem>(x + c, end, left);
     }
-    return acc;
-}
+};
 
 }  // namespace few

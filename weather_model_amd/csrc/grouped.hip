@@ -255,7 +255,9 @@ __global__ __launch_bounds__(few::THREADS) void grouped_few_kernel(const typenam
     const E *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
     for (int r0 = 0; r0 < rows; r0 += 16) {
         const int r = min(r0 + (lane & 15), rows - 1);
-        const f32x4 acc = few::dot<T>(wrow, W + (long long)G * N * K, x + (long long)(row0 + r) * K, x + (long long)M * K, K);
+        few::Dot<T> dot;
+        dot.begin(wrow, W + (long long)G * N * K, K);
+        const f32x4 acc = dot.multiply(few::RowOf<T>{x + (long long)(row0 + r) * K, x + (long long)M * K});
         if (wave > 0) part[wave][lane] = acc;
         __syncthreads();
         if (wave == 0) {
@@ -283,8 +285,8 @@ __global__ __launch_bounds__(few::THREADS) void grouped_few_kernel(const typenam
 int check(const char *who, int M, int N, int K, int G, int dtype)
 {
     WM_REQUIRE(M >= 0 && N > 0 && K > 0 && G > 0, WM_ERR_INVALID, "%s: bad sizes M=%d N=%d K=%d groups=%d", who, M, N, K, G);
-    WM_REQUIRE(N <= 1 << 20 && K <= 1 << 20 && G <= 1 << 16 && M <= 1 << 30, WM_ERR_UNSUPPORTED,
-               "%s: M=%d N=%d K=%d groups=%d is beyond 2^30 rows, 2^20 columns or 2^16 groups", who, M, N, K, G);
+    WM_REQUIRE(N <= 1 << 20 && K <= 1 << 20 && G < 1 << 16 && M <= 1 << 30, WM_ERR_UNSUPPORTED,
+               "%s: M=%d N=%d K=%d groups=%d is beyond 2^30 rows, 2^20 columns or 2^16 - 1 groups", who, M, N, K, G);
     WM_REQUIRE(dtype == WM_F32 || dtype == WM_BF16 || dtype == WM_F16, WM_ERR_INVALID, "%s: bad dtype %d", who, dtype);
     WM_REQUIRE(wm_num_cus() > 0, WM_ERR_NO_DEVICE, "%s: no HIP device", who);
     return WM_OK;
@@ -425,7 +427,7 @@ extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b,
     if (int rc = check("wm_dense_grouped_fwd", M, N, K, G, dtype)) return rc;
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
-    if (few_rows(G, M) && G < 65535) {
+    if (few_rows(G, M)) {
         hipStream_t st = (hipStream_t)stream;
         switch (dtype) {
         case WM_F32: return few_launch<F32>(x, W, b, y, offsets, G, M, N, K, relu, st);

@@ -11,8 +11,6 @@ namespace {
 
 using namespace tile;
 
-constexpr int THREADS = 256;                 // of the kernels without tiles
-
 // x / s rounded to even, as float32 division gives it.  x times the reciprocal is within 2^-22 of the quotient, relatively:
 // only next to a tie (within 2^-15, |x / s| <= 128) can that round to another integer, and there it divides.
 __device__ __forceinline__ float code_of(float x, float s, float r)
@@ -24,16 +22,13 @@ __device__ __forceinline__ float code_of(float x, float s, float r)
 
 // `LANES` threads a row, each NV vectors of 8 values in registers between the two passes; what does not fit (K > 8 LANES
 // NV) is read again.  Codes go to q with row stride ldq >= K, zeros behind K.
-template <class E, int LANES, int NV>
-__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restrict__ x, int M, int K, int8_t *__restrict__ q, long long ldq,
-                                                                float *__restrict__ scale)
+template <class E, int LANES, int NV, int THREADS>
+__device__ __forceinline__ void quantize_row(const E *__restrict__ row, int K, int8_t *to, long long ldq, float *scale)
 {
     typedef E vec __attribute__((ext_vector_type(8), aligned(sizeof(E))));
     typedef uint32_t codes __attribute__((ext_vector_type(2), aligned(1)));
     __shared__ float part[THREADS / 64];
-    const int m = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES, t = threadIdx.x % LANES;
-    if (LANES == 64 && m >= M) return;       // whole waves
-    const E *row = x + (long long)m * K;
+    const int t = threadIdx.x % LANES;
     auto load = [&](int k, float (&v)[8]) {
         if (k + 8 <= K) {
             const vec u = *reinterpret_cast<const vec *>(row + k);
@@ -75,7 +70,6 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restr
     const float s = top > 3.4028235e38f ? __builtin_nanf("") : top / 127.0f;
     const float r = s > 0.0f ? 1.0f / s : 0.0f;
     const bool near = r > 3.4028235e38f;     // a subnormal scale has no reciprocal
-    int8_t *to = q + m * ldq;
     auto put = [&](int k, const float (&u)[8]) {
         uint32_t w[2] = {0u, 0u};
 #pragma unroll
@@ -97,7 +91,16 @@ __global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restr
         load(k, u);
         put(k, u);
     }
-    if (t == 0) scale[m] = s;
+    if (t == 0) *scale = s;
+}
+
+template <class E, int LANES, int NV, int THREADS>
+__global__ __launch_bounds__(THREADS) void quantize_rows_kernel(const E *__restrict__ x, int M, int K, int8_t *__restrict__ q, long long ldq,
+                                                                float *__restrict__ scale)
+{
+    const int m = blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
+    if (LANES == 64 && m >= M) return;       // whole waves
+    quantize_row<E, LANES, NV, THREADS>(x + (long long)m * K, K, q + m * ldq, ldq, scale + m);
 }
 
 template <class E, class S, bool DIRECT>
@@ -183,6 +186,48 @@ __global__ __launch_bounds__(S::THREADS, 2) void dense_i8_kernel(const int8_t *_
 }
 
 // ---- few rows: one read of the weights (few_rows.h)
+// joins the waves' sums; wave 0 scales and writes columns n0 .. n0 + 15 of row y (lane & 15), if `there`
+template <class E>
+__device__ __forceinline__ void few_out(i32x4 acc, i32x4 (&part)[few::WAVES][64], E *y, bool there, float qs, const float *wscale, const float *bias,
+                                        int n0, int N, int relu)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (wave > 0) part[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+        for (int w = 1; w < few::WAVES; ++w) acc += part[w][lane];
+        const int n = n0 + 4 * (lane >> 4), have = min(4, N - n);
+        if (there && have > 0) {
+            f32x4 v;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int kk = n + min(k, have - 1);
+                v[k] = (float)acc[k] * qs * wscale[kk] + (bias ? bias[kk] : 0.0f);
+                if (relu) v[k] = relu_of(v[k]);
+            }
+            if (have == 4) store4(y + n, v);
+            else
+                for (int k = 0; k < have; ++k) y[n + k] = from_float<E>(v[k]);
+        }
+    }
+    __syncthreads();
+}
+
+// zeros in columns n0 .. n0 + 15 of the rows of no expert
+template <class E> __device__ __forceinline__ void few_zeros(E *y, const long long *offsets, int G, int M, int N, int n0)
+{
+    int row0, rows, end;
+    group_rows(offsets, G, M, 0, row0, rows);
+    group_rows(offsets, G, M, G - 1, end, rows);
+    end += rows;
+    const int cols = min(16, N - n0);
+    for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += few::THREADS) {
+        const int r = e / cols;
+        y[(long long)(r < row0 ? r : r - row0 + end) * N + n0 + e % cols] = (E)0.0f;
+    }
+}
+
 template <class E>
 __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
                                                                     const int8_t *__restrict__ W, const float *__restrict__ wscale,
@@ -190,51 +235,48 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
                                                                     const long long *__restrict__ offsets, int G, int M, int N, int K, int relu)
 {
     __shared__ i32x4 part[few::WAVES][64];
-    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63;
+    if (g == G) return few_zeros(y, offsets, G, M, N, n0);
     int row0 = 0, rows = M;
-    if (g == G) {                                    // rows of no expert: zeros
-        int end;
-        group_rows(offsets, G, M, 0, row0, rows);
-        group_rows(offsets, G, M, G - 1, end, rows);
-        end += rows;
-        const int cols = min(16, N - n0);
-        for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += few::THREADS) {
-            const int r = e / cols;
-            y[(long long)(r < row0 ? r : r - row0 + end) * N + n0 + e % cols] = (E)0.0f;
-        }
-        return;
-    }
     if (offsets) group_rows(offsets, G, M, g, row0, rows);
     const int8_t *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
     for (int r0 = 0; r0 < rows; r0 += 16) {
-        const int r = min(r0 + (lane & 15), rows - 1);
-        const i32x4 acc = few::dot<I8>(wrow, W + (long long)G * N * K, q + (row0 + r) * ldq, q + M * ldq, K);
-        if (wave > 0) part[wave][lane] = acc;
-        __syncthreads();
-        if (wave == 0) {
-            i32x4 s = acc;
-#pragma unroll
-            for (int w = 1; w < few::WAVES; ++w) s += part[w][lane];
-            const int n = n0 + 4 * (lane >> 4), have = min(4, N - n);
-            if (r0 + (lane & 15) < rows && have > 0) {
-                E *at = y + (long long)(row0 + r) * N + n;
-                const float qs = qscale[row0 + r];
-                const long long c = (long long)g * N + n;
-                f32x4 v;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int kk = min(k, have - 1);
-                    v[k] = (float)s[k] * qs * wscale[c + kk] + (bias ? bias[c + kk] : 0.0f);
-                    if (relu) v[k] = relu_of(v[k]);
-                }
-                if (have == 4) store4(at, v);
-                else
-                    for (int k = 0; k < have; ++k) at[k] = from_float<E>(v[k]);
-            }
-        }
-        __syncthreads();
+        const int r = row0 + min(r0 + (lane & 15), rows - 1);
+        few::Dot<I8> dot;
+        dot.begin(wrow, W + (long long)G * N * K, K);
+        const i32x4 acc = dot.multiply(few::RowOf<I8>{q + r * ldq, q + M * ldq});
+        few_out(acc, part, y + (long long)r * N, r0 + (lane & 15) < rows, qscale[r], wscale + (long long)g * N, bias ? bias + (long long)g * N : nullptr,
+                n0, N, relu);
     }
 }
+
+// One row: every workgroup makes the row's codes itself, in LDS, while its first weights are on their way -- the same codes as
+// quantize_rows_kernel's.  A launch of its own for one row took as long as the product (1 x 640 x 8000: 14.9 -> 10.5 us a call).
+constexpr int ONE_ROW_K = 8192;
+
+template <class E>
+__global__ __launch_bounds__(few::THREADS) void dense_i8_one_kernel(const E *__restrict__ x, const int8_t *__restrict__ W,
+                                                                    const float *__restrict__ wscale, const float *__restrict__ bias,
+                                                                    E *__restrict__ y, const long long *__restrict__ offsets, int G, int N, int K,
+                                                                    int relu)
+{
+    __shared__ i32x4 part[few::WAVES][64];
+    __shared__ __attribute__((aligned(16))) int8_t codes[ONE_ROW_K];
+    __shared__ float s_shared;
+    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63;
+    if (g == G) return few_zeros(y, offsets, G, 1, N, n0);
+    int row0 = 0, rows = 1;
+    if (offsets) group_rows(offsets, G, 1, g, row0, rows);
+    if (rows == 0) return;
+    few::Dot<I8> dot;
+    dot.begin(W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K, W + (long long)G * N * K, K);
+    quantize_row<E, few::THREADS, ONE_ROW_K / 8 / few::THREADS, few::THREADS>(x, K, codes, (K + 127) / 128 * 128, &s_shared);
+    __syncthreads();
+    const i32x4 acc = dot.multiply([&](int c, int) { return *reinterpret_cast<const u32x4 *>(codes + c); });
+    few_out(acc, part, y, (lane & 15) == 0, s_shared, wscale + (long long)g * N, bias ? bias + (long long)g * N : nullptr, n0, N, relu);
+}
+
+bool one_row(int M, int K) { return M == 1 && K <= ONE_ROW_K; }
 
 size_t padded(int K) { return wm_align_up((size_t)K, 128); }
 
@@ -248,17 +290,19 @@ int check(const char *who, int M, int K, int dtype)
     return WM_OK;
 }
 
-// A wave a row up to 1024 values, a workgroup beyond (8192 rows of 4096 bf16: 54 us by single values, 2 passes; see DESIGN).
+// A wave a row up to 1024 values, a workgroup beyond (8192 rows of 4096 bf16: 25 us = 4.1 TB/s; by single values 54 us).  With
+// fewer rows than CUs the time is one row's chain of load, maximum and codes: more threads a row.
 template <class E> int quantize(const void *x, int M, int K, int8_t *q, long long ldq, float *scale, hipStream_t st)
 {
-#define WM_QUANTIZE(LANES, NV)                                                                                                       \
-    hipLaunchKernelGGL((quantize_rows_kernel<E, LANES, NV>), dim3((M + THREADS / LANES - 1) / (THREADS / LANES)), dim3(THREADS), 0, \
-                       st, (const E *)x, M, K, q, ldq, scale)
-    if (K <= 512) WM_QUANTIZE(64, 1);
-    else if (K <= 1024) WM_QUANTIZE(64, 2);
-    else if (K <= 2048) WM_QUANTIZE(THREADS, 1);
-    else if (K <= 4096) WM_QUANTIZE(THREADS, 2);
-    else WM_QUANTIZE(THREADS, 4);
+#define WM_QUANTIZE(LANES, NV, THREADS)                                                                                                 \
+    hipLaunchKernelGGL((quantize_rows_kernel<E, LANES, NV, THREADS>), dim3((M + THREADS / LANES - 1) / (THREADS / LANES)), dim3(THREADS), \
+                       0, st, (const E *)x, M, K, q, ldq, scale)
+    if (K <= 512) WM_QUANTIZE(64, 1, 256);
+    else if (M < wm_num_cus()) WM_QUANTIZE(1024, 1, 1024);
+    else if (K <= 1024) WM_QUANTIZE(64, 2, 256);
+    else if (K <= 2048) WM_QUANTIZE(256, 1, 256);
+    else if (K <= 4096) WM_QUANTIZE(256, 2, 256);
+    else WM_QUANTIZE(256, 4, 256);
 #undef WM_QUANTIZE
     WM_LAUNCH_CHECK("quantize_rows_kernel");
     return WM_OK;
@@ -281,11 +325,17 @@ template <class E>
 int dense(const void *x, const int8_t *W, const float *wscale, const float *b, void *y, const int64_t *offsets, int G, int M, int N, int K, int relu,
           void *workspace, hipStream_t st)
 {
+    if (one_row(M, K)) {
+        hipLaunchKernelGGL(dense_i8_one_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, (const E *)x, W, wscale, b,
+                           (E *)y, (const long long *)offsets, G, N, K, relu);
+        WM_LAUNCH_CHECK("dense_i8_one_kernel");
+        return WM_OK;
+    }
     float *scale = (float *)workspace;
     int8_t *q = (int8_t *)workspace + wm_align_up((size_t)M * sizeof(float), 256);
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
-    if ((M <= 64 || M / G <= 8) && G < 65535) {
+    if (M <= 64 || M / G <= 8) {
         hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, q, ldq, scale, W, wscale, b,
                            (E *)y, (const long long *)offsets, G, M, N, K, relu);
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
@@ -316,7 +366,7 @@ extern "C" int wm_quantize_rows_i8(const void *x, int M, int K, int dtype, int8_
 
 extern "C" size_t wm_dense_i8_workspace_bytes(int M, int K)
 {
-    if (M <= 0 || K <= 0) return 0;
+    if (M <= 0 || K <= 0 || one_row(M, K)) return 0;
     return wm_align_up((size_t)M * sizeof(float), 256) + (size_t)M * padded(K);
 }
 
@@ -326,11 +376,11 @@ extern "C" int wm_dense_i8(const void *x, const int8_t *W, const float *wscale, 
     if (int rc = check("wm_dense_i8", M, K, dtype)) return rc;
     WM_REQUIRE(N > 0 && G > 0, WM_ERR_INVALID, "wm_dense_i8: bad sizes N=%d groups=%d", N, G);
     WM_REQUIRE(offsets || G == 1, WM_ERR_INVALID, "wm_dense_i8: %d groups need offsets", G);
-    WM_REQUIRE(N <= 1 << 20 && G <= 1 << 16, WM_ERR_UNSUPPORTED, "wm_dense_i8: N=%d groups=%d is beyond 2^20 columns or 2^16 groups", N, G);
+    WM_REQUIRE(N <= 1 << 20 && G < 1 << 16, WM_ERR_UNSUPPORTED, "wm_dense_i8: N=%d groups=%d is beyond 2^20 columns or 2^16 - 1 groups", N, G);
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && wscale && y, WM_ERR_INVALID, "wm_dense_i8: null pointer");
     const size_t need = wm_dense_i8_workspace_bytes(M, K);
-    WM_REQUIRE(workspace && workspace_bytes >= need, WM_ERR_WORKSPACE, "wm_dense_i8: workspace of %zu bytes needed, %zu given", need,
+    WM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), WM_ERR_WORKSPACE, "wm_dense_i8: workspace of %zu bytes needed, %zu given", need,
                workspace_bytes);
     WM_REQUIRE(((uintptr_t)workspace & 15) == 0, WM_ERR_INVALID, "wm_dense_i8: workspace must be 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;

@@ -625,6 +625,22 @@ struct Segment {
     int g, row0, rows;                       // group, first row and rows of a tile
 };
 
+// a lane's value, in a scalar register
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// Scans over the wave in data-parallel moves: 1, 2, 4 and 8 lanes up within rows of 16, then the rows' ends to the next row and the
+// upper half (lanes without a source see `none`).
+template <class F> __device__ __forceinline__ int wave_scan(int v, int none, F join)
+{
+    v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x111, 0xF, 0xF, false));
+    v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x112, 0xF, 0xF, false));
+    v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x114, 0xF, 0xF, false));
+    v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x118, 0xF, 0xF, false));
+    v = join(v, __builtin_amdgcn_update_dpp(none, v, 0x142, 0xA, 0xF, false));
+    return join(v, __builtin_amdgcn_update_dpp(none, v, 0x143, 0xC, 0xF, false));
+}
+__device__ __forceinline__ int wave_scan(int v) { return wave_scan(v, 0, [](int a, int b) { return a + b; }); }
+
 // Bounds of 64 segments s0 .. s0 + 63 in the lanes (segment s is group s - 1); `carry` is the bound before s0.
 __device__ __forceinline__ void segment_bounds(const long long *offsets, int G, int M, int s0, int carry, int &lo, int &hi)
 {
@@ -632,28 +648,8 @@ __device__ __forceinline__ void segment_bounds(const long long *offsets, int G, 
     // the bound at the END of segment s: offsets[s] for s <= G, M behind
     long long v = s <= G ? (offsets ? offsets[s] : (s ? M : 0)) : M;
     int e = v < 0 ? 0 : v > M ? M : (int)v;
-    e = max(e, carry);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(e, o, 64);
-        if ((int)(threadIdx.x & 63) >= o) e = max(e, up);
-    }
-    hi = e;
-    lo = __shfl_up(e, 1, 64);
-    if ((threadIdx.x & 63) == 0) lo = carry;
-}
-
-// a lane's value, in a scalar register
-__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-
-__device__ __forceinline__ int wave_scan(int v)          // inclusive
-{
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(v, o, 64);
-        if ((int)(threadIdx.x & 63) >= o) v += up;
-    }
-    return v;
+    hi = wave_scan(max(e, carry), 0, [](int a, int b) { return max(a, b); });
+    lo = __builtin_amdgcn_update_dpp(carry, hi, 0x138, 0xF, 0xF, false);         // one lane up
 }
 
 // The map from a tile's number to its rows, built once a workgroup; what up to 62 groups need stays in the lanes.

@@ -1202,10 +1202,10 @@ def dense_i8(x, weight, scale, bias=None, relu=False, offsets=None, out=None):
     y = _out_any(out, (M, N), x, "out")
     L = _lib.lib()
     need = L.wm_dense_i8_workspace_bytes(M, K)
-    ws = torch.empty((need,), device=x.device, dtype=torch.uint8)
+    ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
     _call(x.device, L.wm_dense_i8, x.data_ptr(), weight.data_ptr(), scale.data_ptr(),
           0 if bias is None else bias.data_ptr(), y.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
-          G, M, N, K, _DTYPES[x.dtype], 1 if relu else 0, ws.data_ptr(), need)
+          G, M, N, K, _DTYPES[x.dtype], 1 if relu else 0, 0 if ws is None else ws.data_ptr(), need)
     return y
 
 
