@@ -27,52 +27,67 @@ template <class T> __device__ __forceinline__ typename T::acc piece(u32x4 a, u32
 }
 
 // This wave's share of the products of matrix row w (i = lane & 15: four consecutive rows of the result per lane) with a row of x;
-// rows that do not exist are given as any that do.  x(c, left) gives the piece of the row from value c on, of which `left` count.
-// begin() may be called long before multiply(): the first loads of the weights are then under way.
-template <class T> struct Dot {
+// rows that do not exist are given as any that do.  x gives the pieces of its row: whole(c) from value c on, part(c, left) of which
+// only `left` values count.
+// EARLY: begin() is called long before multiply(), and the first loads of the weights go out there.
+template <class T, bool EARLY = false> struct Dot {
     typedef typename T::elem E;
     static constexpr int ROUND = 128 / sizeof(E), PIECE = 16 / sizeof(E);
+    typedef u32x4 Batch[UNROLL][2];
     const E *w, *end;
-    int K, rounds;
-    u32x4 a[UNROLL][2];
+    int K, rounds;                           // rounds: whole ones
+    Batch first;
+    static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
     static __device__ __forceinline__ int at() { return (int)((threadIdx.x & 63) >> 4) * 2 * PIECE; }      // of this lane in a round
-    __device__ __forceinline__ void load(int r)
+    // UNROLL rounds from r on, WAVES apart; behind the last whole one that one again
+    __device__ __forceinline__ int round(int r, int u) const { return min(r + u * WAVES, rounds - 1) * ROUND; }
+    __device__ __forceinline__ void load(int r, Batch &to) const
     {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) a[u][h] = *reinterpret_cast<const u32x4u *>(w + (r + u * WAVES) * ROUND + h * PIECE);
+            for (int h = 0; h < 2; ++h) to[u][h] = *reinterpret_cast<const u32x4u *>(w + round(r, u) + h * PIECE);
     }
-    __device__ __forceinline__ bool batch(int r) const { return r + (UNROLL - 1) * WAVES < rounds; }
+    template <class X> __device__ __forceinline__ void add(int r, const Batch &a, const X &x, typename T::acc &acc) const
+    {
+        Batch b;
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) b[u][h] = x.whole(round(r, u) + h * PIECE + at());
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+            if (r + u * WAVES < rounds)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) acc = piece<T>(a[u][h], b[u][h], acc);
+    }
     __device__ __forceinline__ void begin(const E *row, const E *tensor_end, int K_)
     {
         w = row + at();
         end = tensor_end;
         K = K_;
         rounds = K / ROUND;
-        if (batch(threadIdx.x >> 6)) load(threadIdx.x >> 6);
+        if constexpr (EARLY)
+            if (wave() < rounds) load(wave(), first);
     }
-    template <class X> __device__ __forceinline__ typename T::acc multiply(X x)
+    template <class X> __device__ __forceinline__ typename T::acc multiply(const X &x) const
     {
         typename T::acc acc = {0, 0, 0, 0};
-        int r = threadIdx.x >> 6;
-        for (bool there = true; batch(r); r += UNROLL * WAVES, there = false) {
-            u32x4 b[UNROLL][2];
-            if (!there) load(r);
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) b[u][h] = x((r + u * WAVES) * ROUND + h * PIECE + at(), PIECE);
-#pragma unroll
-            for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) acc = piece<T>(a[u][h], b[u][h], acc);
+        int r = wave();
+        if constexpr (EARLY) {
+            if (r < rounds) add(r, first, x, acc);
+            r += UNROLL * WAVES;
         }
-        for (; r * ROUND < K; r += WAVES)
+        for (; r < rounds; r += UNROLL * WAVES) {
+            Batch a;
+            load(r, a);
+            add(r, a, x, acc);
+        }
+        if (rounds * ROUND < K && rounds % WAVES == wave())
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int c = r * ROUND + h * PIECE, left = K - c - at();
-                acc = piece<T>(load16_guarded<E>(w + c, end, left), x(c + at(), left), acc);
+                const int c = rounds * ROUND + h * PIECE, left = K - c - at();
+                acc = piece<T>(load16_guarded<E>(w + c, end, left), x.part(c + at(), left), acc);
             }
         return acc;
     }
@@ -80,11 +95,8 @@ template <class T> struct Dot {
 // x as a row in memory
 template <class T> struct RowOf {
     const typename T::elem *x, *end;
-    __device__ __forceinline__ u32x4 operator()(int c, int left) const
-    {
-        if (left >= (int)(16 / sizeof(typename T::elem))) return *reinterpret_cast<const u32x4u *>(x + c);
-        return load16_guarded<typename T::elem>(x + c, end, left);
-    }
+    __device__ __forceinline__ u32x4 whole(int c) const { return *reinterpret_cast<const u32x4u *>(x + c); }
+    __device__ __forceinline__ u32x4 part(int c, int left) const { return load16_guarded<typename T::elem>(x + c, end, left); }
 };
 
 }  // namespace few

@@ -253,6 +253,11 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
 // One row: every workgroup makes the row's codes itself, in LDS, while its first weights are on their way -- the same codes as
 // quantize_rows_kernel's.  A launch of its own for one row took as long as the product (1 x 640 x 8000: 14.9 -> 10.5 us a call).
 constexpr int ONE_ROW_K = 8192;
+struct Codes {                               // in LDS, zeros behind the row
+    const int8_t *q;
+    __device__ __forceinline__ u32x4 whole(int c) const { return *reinterpret_cast<const u32x4 *>(q + c); }
+    __device__ __forceinline__ u32x4 part(int c, int) const { return whole(c); }
+};
 
 template <class E>
 __global__ __launch_bounds__(few::THREADS) void dense_i8_one_kernel(const E *__restrict__ x, const int8_t *__restrict__ W,
@@ -268,11 +273,11 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_one_kernel(const E *__r
     int row0 = 0, rows = 1;
     if (offsets) group_rows(offsets, G, 1, g, row0, rows);
     if (rows == 0) return;
-    few::Dot<I8> dot;
+    few::Dot<I8, true> dot;
     dot.begin(W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K, W + (long long)G * N * K, K);
     quantize_row<E, few::THREADS, ONE_ROW_K / 8 / few::THREADS, few::THREADS>(x, K, codes, (K + 127) / 128 * 128, &s_shared);
     __syncthreads();
-    const i32x4 acc = dot.multiply([&](int c, int) { return *reinterpret_cast<const u32x4 *>(codes + c); });
+    const i32x4 acc = dot.multiply(Codes{codes});
     few_out(acc, part, y, (lane & 15) == 0, s_shared, wscale + (long long)g * N, bias ? bias + (long long)g * N : nullptr, n0, N, relu);
 }
 

@@ -97,14 +97,19 @@ template <class E> __device__ __forceinline__ u32x4 load16_guarded(const E *p, c
         }
         return v;
     }
+    // one value after the other: the last bytes of a tensor, and no registers for it
+    constexpr int PER_WORD = 4 / sizeof(E);
 #pragma unroll
-    for (int e = 0; e < N; ++e)
-        if (e < avail && p + e < end) {
+    for (int d = 0; d < 4; ++d)
+#pragma unroll 1
+        for (int i = 0; i < PER_WORD; ++i) {
+            const int e = d * PER_WORD + i;
+            if (e >= avail || p + e >= end) break;
             uint32_t bits;
             if constexpr (sizeof(E) == 4) bits = __builtin_bit_cast(uint32_t, p[e]);
             else if constexpr (sizeof(E) == 2) bits = __builtin_bit_cast(uint16_t, p[e]);
             else bits = (uint8_t)p[e];
-            v[e * (int)sizeof(E) / 4] |= bits << (8 * (e * (int)sizeof(E) % 4));
+            v[d] |= bits << (8 * (int)sizeof(E) * i);
         }
     return v;
 }
