@@ -242,7 +242,7 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
     const int8_t *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
     for (int r0 = 0; r0 < rows; r0 += 16) {
         const int r = row0 + min(r0 + (lane & 15), rows - 1);
-        few::Dot<I8> dot;
+        few::Dot<I8, 4> dot;
         dot.begin(wrow, W + (long long)G * N * K, K);
         const i32x4 acc = dot.multiply(few::RowOf<I8>{q + r * ldq, q + M * ldq});
         few_out(acc, part, y + (long long)r * N, r0 + (lane & 15) < rows, qscale[r], wscale + (long long)g * N, bias ? bias + (long long)g * N : nullptr,
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_one_kernel(const E *__r
     int row0 = 0, rows = 1;
     if (offsets) group_rows(offsets, G, 1, g, row0, rows);
     if (rows == 0) return;
-    few::Dot<I8, true> dot;
+    few::Dot<I8, 4, true> dot;
     dot.begin(W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K, W + (long long)G * N * K, K);
     quantize_row<E, few::THREADS, ONE_ROW_K / 8 / few::THREADS, few::THREADS>(x, K, codes, (K + 127) / 128 * 128, &s_shared);
     __syncthreads();
