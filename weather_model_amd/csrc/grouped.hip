@@ -96,7 +96,7 @@ __device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__re
     }
 }
 
-template <class S, class Sub, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
+template <class S, class Half, class Quarter, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
 __global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
                                                                   const E *__restrict__ mask, E *__restrict__ out,
                                                                   const long long *__restrict__ offsets, int G, int M, int NO, int C, int relu,
@@ -105,19 +105,17 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_kernel(const E *__
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     const RowTiles<S::BM> tiles(offsets, G, M);
     const int across = (NO + S::BN - 1) / S::BN;
-    const Cut<S, Sub> cut(blockIdx.x, tiles.total * across, slots);
+    const Cut<S, Half, Quarter> cut(blockIdx.x, tiles.total * across, slots);
     if (cut.tile < 0) return;
     int rt, ct;
     place_of_tile(cut.tile, tiles.total, across, 8, rt, ct);
     Segment s = tiles.tile(rt);
     const int n0 = min(ct * S::BN, max(0, NO - S::BN));      // the last tile moves back over its neighbour
-    if (!cut.part) {
-        rows_tile<S, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0, G, M, NO, C, relu);
-    } else {
-        s.row0 += cut.row;
-        s.rows -= cut.row;
-        rows_tile<Sub, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
-    }
+    s.row0 += cut.row;
+    s.rows -= cut.row;
+    if (cut.parts == 1) rows_tile<S, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0, G, M, NO, C, relu);
+    else if (cut.parts == 4) rows_tile<Quarter, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
+    else if constexpr (S::ALONE) rows_tile<Half, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
 }
 
 // ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
@@ -300,17 +298,15 @@ int blocks_ok(const char *who, long long blocks)
     return WM_OK;
 }
 
-constexpr int LDS_PER_CU = 160 << 10;
-
-template <class S, class Sub, bool BACKWARD, bool DIRECT>
+template <class S, class Half, class Quarter, bool BACKWARD, bool DIRECT>
 int rows_launch(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                 int C, int relu, hipStream_t st)
 {
     typedef typename S::T::elem E;
-    const int slots = wm_num_cus() * (S::LDS <= LDS_PER_CU / 2 ? 2 : 1);
-    const long long blocks = Cut<S, Sub>::blocks(row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN), slots);
+    const int slots = wm_num_cus() * (S::ALONE ? 1 : 2);
+    const long long blocks = Cut<S, Half, Quarter>::blocks(row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN), slots);
     if (int rc = blocks_ok("wm_dense_grouped", blocks)) return rc;
-    hipLaunchKernelGGL((grouped_rows_kernel<S, Sub, BACKWARD, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x,
+    hipLaunchKernelGGL((grouped_rows_kernel<S, Half, Quarter, BACKWARD, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)x,
                        (const E *)W, (const E *)bias, (const E *)mask, (E *)out, (const long long *)offsets, G, M, NO, C, relu, slots);
     WM_LAUNCH_CHECK("grouped_rows_kernel");
     return WM_OK;
@@ -318,13 +314,14 @@ int rows_launch(const void *x, const void *W, const void *bias, const void *mask
 
 template <class T> struct Tiles {                       // 16-bit types
     typedef Shape<T, 256, 256, 2, 4> Large;
-    typedef Shape<T, 128, 256, 2, 4> LargePart;
+    typedef Shape<T, 128, 256, 2, 4> LargeHalf;
+    typedef Shape<T, 128, 128, 2, 4> LargeQuarter;
     typedef Shape<T, 128, 128, 2, 2> Medium;
-    typedef Shape<T, 64, 64, 2, 2, 2, 2> MediumPart;
+    typedef Shape<T, 64, 64, 2, 2, 2, 2> MediumQuarter;
 };
 template <> struct Tiles<F32> {
     typedef Shape<F32, 128, 128, 2, 2, 1> Medium;
-    typedef Shape<F32, 64, 64, 2, 2, 1, 2> MediumPart;
+    typedef Shape<F32, 64, 64, 2, 2, 1, 2> MediumQuarter;
 };
 
 bool large(int G, int M, int N) { return M / G >= 512 && N >= 512; }
@@ -337,11 +334,11 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
     if constexpr (T::PLANES == 1) {
         if (direct_ok(x, 2ll * C) && direct_ok(W, BACKWARD ? 2ll * NO : 2ll * C)) {
             if (large(G, M, NO))
-                return rows_launch<typename Z::Large, typename Z::LargePart, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-            return rows_launch<typename Z::Medium, typename Z::MediumPart, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+                return rows_launch<typename Z::Large, typename Z::LargeHalf, typename Z::LargeQuarter, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+            return rows_launch<typename Z::Medium, void, typename Z::MediumQuarter, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
         }
     }
-    return rows_launch<typename Z::Medium, typename Z::MediumPart, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    return rows_launch<typename Z::Medium, void, typename Z::MediumQuarter, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows.
@@ -386,7 +383,7 @@ int weights_launch(const void *x, const void *gy, void *gW, void *gb, float *par
     const long long blocks = (long long)splits * G * ((N + S::BM - 1) / S::BM) * ((K + S::BN - 1) / S::BN);
     if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
     // groups begun on empty CUs, where all workgroups run at once
-    const long long first = blocks <= 2ll * wm_num_cus() && S::LDS <= LDS_PER_CU / 2 ? wm_num_cus() / (blocks / G) : G;
+    const long long first = blocks <= 2ll * wm_num_cus() && !S::ALONE ? wm_num_cus() / (blocks / G) : G;
     hipLaunchKernelGGL((grouped_weights_kernel<S, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)gy, (const E *)x, (E *)gW,
                        (E *)gb, partial, (const long long *)offsets, G, M, N, K, splits, (int)first);
     WM_LAUNCH_CHECK("grouped_weights_kernel");

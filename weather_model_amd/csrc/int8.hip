@@ -161,7 +161,7 @@ __device__ __forceinline__ void i8_tile(const int8_t *__restrict__ q, long long 
     }
 }
 
-template <class E, class S, class Sub, bool DIRECT>
+template <class E, class S, class Half, class Quarter, bool DIRECT>
 __global__ __launch_bounds__(S::THREADS, 2) void dense_i8_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
                                                               const int8_t *__restrict__ W, const float *__restrict__ wscale,
                                                               const float *__restrict__ bias, E *__restrict__ y,
@@ -170,19 +170,17 @@ __global__ __launch_bounds__(S::THREADS, 2) void dense_i8_kernel(const int8_t *_
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     const RowTiles<S::BM> tiles(offsets, G, M);
     const int across = (N + S::BN - 1) / S::BN;
-    const Cut<S, Sub> cut(blockIdx.x, tiles.total * across, slots);
+    const Cut<S, Half, Quarter> cut(blockIdx.x, tiles.total * across, slots);
     if (cut.tile < 0) return;
     int rt, ct;
     place_of_tile(cut.tile, tiles.total, across, 8, rt, ct);
     Segment s = tiles.tile(rt);
     const int n0 = min(ct * S::BN, max(0, N - S::BN));       // the last tile moves back over its neighbour
-    if (!cut.part) {
-        i8_tile<E, S, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0, G, M, N, K, relu);
-    } else {
-        s.row0 += cut.row;
-        s.rows -= cut.row;
-        i8_tile<E, Sub, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0 + cut.col, G, M, N, K, relu);
-    }
+    s.row0 += cut.row;
+    s.rows -= cut.row;
+    if (cut.parts == 1) i8_tile<E, S, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0, G, M, N, K, relu);
+    else if (cut.parts == 4) i8_tile<E, Quarter, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0 + cut.col, G, M, N, K, relu);
+    else if constexpr (S::ALONE) i8_tile<E, Half, DIRECT>(q, ldq, qscale, W, wscale, bias, y, lds, s, n0 + cut.col, G, M, N, K, relu);
 }
 
 // ---- few rows: one read of the weights (few_rows.h)
@@ -313,14 +311,14 @@ template <class E> int quantize(const void *x, int M, int K, int8_t *q, long lon
     return WM_OK;
 }
 
-template <class E, class S, class Sub, bool DIRECT>
+template <class E, class S, class Half, class Quarter, bool DIRECT>
 int dense_tiles(const int8_t *q, long long ldq, const float *scale, const int8_t *W, const float *wscale, const float *b, void *y,
                 const int64_t *offsets, int G, int M, int N, int K, int relu, hipStream_t st)
 {
-    const int slots = wm_num_cus() * (S::LDS <= 80 << 10 ? 2 : 1);
-    const long long blocks = Cut<S, Sub>::blocks(row_tiles_most(G, M, S::BM) * ((N + S::BN - 1) / S::BN), slots);
+    const int slots = wm_num_cus() * (S::ALONE ? 1 : 2);
+    const long long blocks = Cut<S, Half, Quarter>::blocks(row_tiles_most(G, M, S::BM) * ((N + S::BN - 1) / S::BN), slots);
     WM_REQUIRE(blocks <= (1ll << 32) / 512 - 1, WM_ERR_UNSUPPORTED, "wm_dense_i8: %lld tiles are too many for one launch", blocks);
-    hipLaunchKernelGGL((dense_i8_kernel<E, S, Sub, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
+    hipLaunchKernelGGL((dense_i8_kernel<E, S, Half, Quarter, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, q, ldq, scale, W, wscale, b, (E *)y,
                        (const long long *)offsets, G, M, N, K, relu, slots);
     WM_LAUNCH_CHECK("dense_i8_kernel");
     return WM_OK;
@@ -346,12 +344,15 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
         return WM_OK;
     }
+    typedef Shape<I8, 128, 128, 2, 2> Medium;
+    typedef Shape<I8, 64, 64, 2, 2, 2, 2> MediumQuarter;
     if (direct_ok(W, K)) {
         if (M / G >= 512 && N >= 512)
-            return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, Shape<I8, 128, 256, 2, 4>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
-        return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2, 2, 2>, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+            return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, Shape<I8, 128, 256, 2, 4>, Shape<I8, 128, 128, 2, 4>, true>(
+                q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+        return dense_tiles<E, Medium, void, MediumQuarter, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
     }
-    return dense_tiles<E, Shape<I8, 128, 128, 2, 2>, Shape<I8, 64, 64, 2, 2, 2, 2>, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
+    return dense_tiles<E, Medium, void, MediumQuarter, false>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
 }
 
 }  // namespace

@@ -389,6 +389,7 @@ template <class T_, int BM_, int BN_, int WM_, int WN_, int BUFFERS_ = 2, int DE
     static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;             // 16 x 16 results a wave
     static constexpr int A_BYTES = BN * T::BKC * 16 * T::PLANES, B_BYTES = BM * T::BKC * 16 * T::PLANES;
     static constexpr int RING = BM * BN == 65536 ? 5 : 4, LDS = T::PLANES == 1 ? RING * (A_BYTES + B_BYTES) / 2 : BUFFERS * (A_BYTES + B_BYTES);
+    static constexpr bool ALONE = LDS > 80 << 10;                          // one workgroup a CU
     typedef typename T::acc Acc[MI][NI];
     // where a lane's results lie: rows row() + 16 m, columns col() + 16 n .. + 3
     static __device__ __forceinline__ int row() { return (int)(threadIdx.x >> 6) / WN * (BM / WM) + (int)(threadIdx.x & 15); }
@@ -723,24 +724,28 @@ __device__ __forceinline__ void place_of_tile(int t, int row_tiles, int col_tile
 }
 
 // The work of a workgroup: a tile of S, or part of one.  `slots` workgroups run at once; the tiles that are left when they
-// have been filled a whole number of times are cut into tiles of Sub where those find room at once, so that a
-// launch ends after a part of a tile's time instead of a whole one.
-template <class S, class Sub> struct Cut {
-    static constexpr int ACROSS = S::BN / Sub::BN, PARTS = S::BM / Sub::BM * ACROSS;
-    static_assert(S::THREADS == Sub::THREADS && Sub::LDS <= S::LDS, "one launch");
-    int tile, row, col;                      // tile < 0: nothing; row and col of the part in it
-    bool part;
+// have been filled a whole number of times are cut into tiles of Quarter or of Half where those find room at once, so that a
+// launch ends after a part of a tile's time instead of a whole one.  Halves only where a tile has a CU to itself: two tiles to a
+// CU leave one each for half of the slots, which is as fast (45001 x 216 x 432 float32 71 us whole, 76 in halves).
+template <class S, class Half, class Quarter> struct Cut {
+    typedef typename std::conditional<S::ALONE, Half, S>::type H;
+    static_assert(S::THREADS == H::THREADS && H::LDS <= S::LDS && (!S::ALONE || S::BM * S::BN == 2 * H::BM * H::BN), "one launch");
+    static_assert(S::THREADS == Quarter::THREADS && Quarter::LDS <= S::LDS && S::BM * S::BN == 4 * Quarter::BM * Quarter::BN, "one launch");
+    int tile, row, col, parts;               // tile < 0: nothing; row and col of the part in it
     __device__ __forceinline__ Cut(int block, int total, int slots)
     {
-        const int left = total % slots, whole = left * PARTS <= slots ? total - left : total;
-        part = block >= whole;
-        const int k = part ? block - whole : 0;
-        tile = part ? whole + k / PARTS : block;
-        row = k % PARTS / ACROSS * Sub::BM;
-        col = k % PARTS % ACROSS * Sub::BN;
+        const int left = total % slots;
+        parts = left * 4 <= slots ? 4 : S::ALONE && left * 2 <= slots ? 2 : 1;
+        const int whole = parts > 1 ? total - left : total;
+        if (block < whole) parts = 1;
+        const int k = block < whole ? 0 : block - whole;
+        tile = block < whole ? block : whole + k / parts;
+        const int i = k % parts, across = parts == 4 ? S::BN / Quarter::BN : S::BN / H::BN;
+        row = i / across * (parts == 4 ? Quarter::BM : H::BM);
+        col = i % across * (parts == 4 ? Quarter::BN : H::BN);
         if (tile >= total) tile = -1;
     }
-    static long long blocks(long long total_most, int slots) { return total_most + (long long)slots / PARTS * (PARTS - 1); }
+    static long long blocks(long long total_most, int slots) { return total_most + (long long)slots / 4 * 3; }
 };
 
 // The order in which the groups' products over rows are taken up: the longest first, so that a launch does not end on one of
