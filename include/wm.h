@@ -465,7 +465,7 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
  * gb.  Any values of offsets are safe: those outside 0 .. M count as the nearest inside, one below its
  * predecessor counts as that.  Results are bitwise reproducible.  float32 products are formed from three
  * bf16 pieces of each factor, with float32 accuracy; infinities and NaN come out as in float32 arithmetic.
- * N, K <= 2^20, M <= 2^30, G < 2^16. */
+ * N, K <= 2^20, M <= 2^30, G <= 4096.  Outputs may not overlap inputs. */
 int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, const int64_t *offsets,
                          int G, int M, int N, int K, int dtype, int relu, void *stream);
 int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx,
@@ -482,7 +482,8 @@ int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, v
  * a captured graph whose replays draw anew) and u(e) 32 bits: with z = the framework's hash of (seed, e / 4)
  * -- the one of wm_synth_uniform_f32 -- bits 16 (e % 4) .. + 15 of z above the same bits of the hash of
  * (seed, z).  The backward pass is the same call on the gradient, without residual.  A dropped element is an exact 0
- * whatever x holds; p = 1 drops all.  n elements of `dtype`; y may be x or residual. */
+ * whatever x holds; p = 1 drops all.  n elements of `dtype`; y may be x or residual; seed counts
+ * modulo 2^32. */
 int wm_dropout(const void *x, const void *residual, void *y, int64_t n, int dtype, double p,
                uint64_t seed, uint64_t offset, const int64_t *offset_dev, void *stream);
 
@@ -494,7 +495,7 @@ int wm_dropout(const void *x, const void *residual, void *y, int64_t n, int dtyp
  * what serves a trained Dense layer (convolution.py:175-176, model.predict) from weights of a byte each.
  * W (G, N, K) int8, wscale and b (G, N) float32 (b may be NULL), y (M, N) of `dtype`; offsets as in
  * wm_dense_grouped_fwd, or NULL with G = 1: all rows use the one W.  The sums are exact integers (K <= 2^17).
- * The workspace (16-byte aligned) holds the codes and scales of x. */
+ * The workspace (16-byte aligned) holds the codes and scales of x; one row of K <= 8192 needs none. */
 int wm_quantize_rows_i8(const void *x, int M, int K, int dtype, int8_t *q, float *scale, void *stream);
 size_t wm_dense_i8_workspace_bytes(int M, int K);
 int wm_dense_i8(const void *x, const int8_t *W, const float *wscale, const float *b, void *y,

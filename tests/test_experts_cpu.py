@@ -54,6 +54,7 @@ def test_c_abi_refusals():
     refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 0, 4, 4, 4, 0, 0, 0), -1, b"bad sizes")
     refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 1, -1, 4, 4, 0, 0, 0), -1, b"bad sizes")
     refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 1, 4, 4, (1 << 20) + 1, 0, 0, 0), -2, b"beyond")
+    refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 4097, 4, 4, 4, 0, 0, 0), -2, b"4096 groups")
     refused(L.wm_dense_grouped_bwd_data(p, p, 0, p, p, 1, 4, 4, 4, 1, 0), -1, b"dtype")
     refused(L.wm_dense_grouped_bwd_wb(p, p, p, 0, 0, 0, p, 1, 4, 0, 4, 0, 0), -1, b"bad sizes")
     refused(L.wm_quantize_rows_i8(p, 4, (1 << 17) + 1, 0, p, p, 0), -2, b"32 bits")
@@ -66,5 +67,6 @@ def test_c_abi_refusals():
 def test_product_sizes_do_not_overflow_the_workspace_query():
     from weather_model_amd import _lib
     L = _lib.lib()
+    assert L.wm_dense_i8_workspace_bytes(1, 8192) == 0 and L.wm_dense_i8_workspace_bytes(1, 8193) > 0
     assert L.wm_dense_i8_workspace_bytes(1 << 24, 1 << 17) >= (1 << 24) * (1 << 17)
     assert L.wm_dense_grouped_bwd_wb_workspace_bytes(1, 1 << 30, 8, 8) >= 8 * 8 * 4

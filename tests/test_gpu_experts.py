@@ -71,6 +71,11 @@ SHAPES = [
     (list(range(80)), 33, 40, 1, 0),
     ([700, 900], 300, 520, 0, 0),
     ([17, 2], 1, 1, 0, 0),
+    ([600, 0, 1100], 520, 136, 2, 1),              # tiles of 256 x 256 and what is left behind them; K no multiple of a stage
+    ([513, 700], 771, 88, 0, 0),                   # the same with columns that are no multiple of 16 bytes
+    ([900], 1032, 1000, 0, 9),
+    ([40] * 21, 72, 96, 0, 0),                     # quarters of small tiles
+    ([3] * 30, 260, 64, 0, 4),
 ]
 
 
@@ -243,6 +248,164 @@ def test_grouped_autograd_against_differences():
             assert abs(float(leaf.grad.reshape(-1)[at]) - d) <= 1e-5 * max(1.0, abs(d)), (k, at)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grouped_results_do_not_depend_on_where_the_tensors_lie(dtype):
+    """The same rows in 16-byte rows (memory to LDS directly) and moved by one element (through registers): each within
+    the bound of the other's sum; and run to run bit for bit."""
+    from weather_model_amd import ops
+    sizes, N, K = [130, 0, 300, 77], 144, 200
+    M, G = sum(sizes), len(sizes)
+    x, w, gy = rows(1, (M, K), dtype), rows(2, (G, N, K), dtype, K ** -0.5), rows(3, (M, N), dtype)
+
+    def moved(t):
+        flat = torch.zeros((t.numel() + 1,), dtype=dtype, device="cuda")
+        flat[1:] = t.cuda().reshape(-1)
+        return flat[1:].view(t.shape)
+    off = offsets_of(sizes)
+    outs = []
+    for f in (lambda t: t.cuda(), moved, lambda t: t.cuda()):
+        a = [f(t) for t in (x, w, gy)]
+        outs.append([ops.dense_grouped_forward(a[0], a[1], off), *ops.dense_grouped_backward(a[0], a[1], off, a[2])])
+    ref, S = grouped_ref(x, w, None, sizes, 0, False)
+    close(outs[0][0], ref, S, K, "aligned")
+    close(outs[1][0], ref, S, K, "moved")
+    for a, b in zip(outs[0], outs[2]):
+        assert torch.equal(a, b)
+
+
+def test_grouped_offsets_and_storage_beyond_32_bits():
+    """More than 2^31 elements of rows, and of weights: the last ones, and the first, against float64."""
+    from weather_model_amd import ops
+    M, K, N = 36000, 65536, 24
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty((M, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    w = torch.empty((2, N, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen) * K ** -0.5
+    off = torch.tensor([0, 35990, M - 1], device="cuda")
+    y = ops.dense_grouped_forward(x, w, off)
+    some = [0, 17999, 35989, 35990, M - 2]
+    for r in some:
+        a, c = x[r].double().cpu(), w[int(r >= 35990)].double().cpu()
+        close(y[r], c @ a, c.abs() @ a.abs(), K, r)
+    assert not bool(y[M - 1].any())
+    gy = torch.empty((M, N), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    _, gw, _ = ops.dense_grouped_backward(x, w, off, gy, need_gx=False, need_bias=False)
+    for k in (0, K - 1):
+        a, c = gy[35990:M - 1].double().cpu(), x[35990:M - 1, k].double().cpu()
+        close(gw[1, :, k], a.t() @ c, a.abs().t() @ c.abs(), M, k)
+    gx, _, _ = ops.dense_grouped_backward(x, w, off, gy, need_gw=False)
+    a, c = gy[M - 2].double().cpu(), w[1].double().cpu()
+    close(gx[M - 2], a @ c, a.abs() @ c.abs(), N, "gx")
+    del x, y, gx, gw
+    G, N, K = 3, 24000, 32000                       # 2.3e9 weights
+    w = torch.empty((G, N, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen) * K ** -0.5
+    for M in (5, 200):                              # few rows, tiles
+        x = torch.empty((M, K), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+        y = ops.dense_grouped_forward(x, w, torch.tensor([0, 1, 2, M], device="cuda"))
+        a, c = x[M - 1].double().cpu(), w[2, -40:].double().cpu()
+        close(y[M - 1, -40:], c @ a, c.abs() @ a.abs(), K, M)
+    q = torch.randint(-127, 128, (G, N, K), device="cuda", generator=gen, dtype=torch.int8)
+    t = torch.ones((G, N), device="cuda")
+    for M in (3, 200):
+        x = torch.empty((M, K), dtype=torch.float32, device="cuda").normal_(generator=gen)
+        y = ops.dense_i8(x, q, t, offsets=torch.tensor([0, 1, 2, M], device="cuda"))
+        xq, xs = codes_ref(x[M - 1:].cpu())
+        ref = (xq @ q[2, -40:].double().cpu().t()) * xs[:, None]
+        assert bool(((y[M - 1:, -40:].cpu().double() - ref).abs() <= 4 * U * ref.abs()).all()), M
+
+
+def test_refusals():
+    from weather_model_amd import ops
+    x, w, off = rows(1, (6, 8), torch.float32).cuda(), rows(2, (2, 4, 8), torch.float32).cuda(), offsets_of([4, 2])
+    bad = [
+        (ValueError, "expects", lambda: ops.dense_grouped_forward(x, w[0], off)),
+        (ValueError, "expects", lambda: ops.dense_grouped_forward(x[:, :7], w, off)),
+        (TypeError, "like the rows", lambda: ops.dense_grouped_forward(x, w.half(), off)),
+        (TypeError, "float32, bfloat16 or float16", lambda: ops.dense_grouped_forward(x.double(), w, off)),
+        (TypeError, "int64", lambda: ops.dense_grouped_forward(x, w, off.int())),
+        (ValueError, "offsets", lambda: ops.dense_grouped_forward(x, w, off[:2])),
+        (RuntimeError, "no CPU fallback", lambda: ops.dense_grouped_forward(x, w, off.cpu())),
+        (ValueError, "bias", lambda: ops.dense_grouped_forward(x, w, off, torch.zeros(4, device="cuda"))),
+        (ValueError, "contiguous", lambda: ops.dense_grouped_forward(x, w, off, out=torch.zeros(6, 8, device="cuda")[:, :4])),
+        (ValueError, "shares memory", lambda: ops.dense_grouped_forward(x, rows(2, (2, 8, 8), torch.float32).cuda(), off, out=x)),
+        (ValueError, "grad_output", lambda: ops.dense_grouped_backward(x, w, off, x)),
+        (ValueError, "mask", lambda: ops.dense_grouped_backward(x, w, off, x[:, :4], mask_below=x[:, :4])),
+        (ValueError, "residual", lambda: ops.dropout_forward(x, 0.1, 1, residual=x[:3])),
+        (ValueError, "shares memory", lambda: ops.dropout_forward(x[:3], 0.1, 1, out=x.view(-1)[8:32].view(3, 8))),
+        (ValueError, "expects", lambda: ops.quantize_rows(x[0])),
+        (ValueError, "expects", lambda: ops.quantize_rows(x[:, :0])),
+        (TypeError, "int8", lambda: ops.dense_i8(x, w[0], torch.ones(4, device="cuda"))),
+        (ValueError, "scale", lambda: ops.dense_i8(x, w[0].to(torch.int8), torch.ones(3, device="cuda"))),
+        (ValueError, "expects", lambda: ops.dense_i8(x, w.to(torch.int8), torch.ones(2, 4, device="cuda"))),
+        (TypeError, "float32", lambda: ops.dense_i8(x, w[0].to(torch.int8), torch.ones(4, device="cuda"), torch.ones(4, device="cuda").half())),
+    ]
+    for k, (error, text, call) in enumerate(bad):
+        with pytest.raises(error, match=text):
+            call()
+            raise AssertionError(f"case {k} was taken")
+    from weather_model_amd._lib import WmError
+    with pytest.raises(WmError, match="beyond"):
+        ops.dense_grouped_forward(x, torch.zeros((4097, 4, 8), device="cuda"), torch.zeros(4098, dtype=torch.int64, device="cuda"))
+
+
+def test_nothing_to_do():
+    """No rows at all: empty results, gradients of zeros."""
+    from weather_model_amd import ops
+    x, w, off = torch.zeros((0, 8), device="cuda"), torch.ones((2, 4, 8), device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    assert ops.dense_grouped_forward(x, w, off).shape == (0, 4)
+    gx, gw, gb = ops.dense_grouped_backward(x, w, off, torch.zeros((0, 4), device="cuda"))
+    assert gx.shape == (0, 8) and not bool(gw.any()) and not bool(gb.any())
+    assert ops.dropout_forward(x, 0.5, 1).shape == (0, 8)
+    assert ops.quantize_rows(x)[0].shape == (0, 8)
+    assert ops.dense_i8(x, torch.ones((4, 8), dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")).shape == (0, 4)
+    # rows, but none owned
+    y = ops.dense_grouped_forward(torch.ones((70, 8), device="cuda"), w, off)
+    assert not bool(y.any())
+
+
+def test_operators_in_two_streams_and_in_graphs():
+    """Two calls at once on two streams, then each captured into a graph of its own and replayed in turn with eager work in
+    between: every result equals the eager one."""
+    from weather_model_amd import ops
+    sizes, N, K = [300, 0, 261, 40], 136, 264
+    off = offsets_of(sizes)
+    sets = []
+    for k in range(2):
+        x, w = rows(5 + k, (sum(sizes), K), torch.bfloat16).cuda(), rows(7 + k, (len(sizes), N, K), torch.bfloat16, 0.1).cuda()
+        q, t = ops.quantize_rows(w.reshape(-1, K))
+        sets.append((x, w, rows(9 + k, (sum(sizes), N), torch.bfloat16).cuda(), q.view(w.shape), t.view(len(sizes), N)))
+
+    def work(k):
+        x, w, gy, q, t = sets[k]
+        return [ops.dense_grouped_forward(x, w, off), *ops.dense_grouped_backward(x, w, off, gy), ops.dropout_forward(x, 0.3, k),
+                ops.dense_i8(x, q, t, offsets=off), ops.dense_grouped_forward(x[:20], w, off)]
+    want = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(3):
+        got = []
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got.append(work(k))
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+    graphs, outs = [], []
+    for k in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(work(k))
+        graphs.append(g)
+    for turn in range(4):
+        for k in (0, 1) if turn % 2 else (1, 0):
+            for o in outs[k]:
+                o.fill_(float("nan"))
+            graphs[k].replay()
+        work(turn % 2)
+        torch.cuda.synchronize()
+        for a, b in zip(want, outs):
+            assert all(torch.equal(u, v) for u, v in zip(a, b)), turn
+
+
 # ------------------------------------------------------------------ dropout
 
 def kept(n, p, seed, offset):
@@ -293,6 +456,16 @@ def test_dropout_drops_infinities_works_in_place_and_in_pieces():
     assert torch.equal(z, whole)
     share = float(kept(1 << 20, 0.1, 3, 0).double().mean())
     assert abs(share - 0.9) < 5 * (0.09 / 2 ** 20) ** 0.5
+
+
+def test_dropout_of_more_than_2_32_elements():
+    from weather_model_amd import ops
+    n, p = 2 ** 32 + 1027, 0.2
+    x = torch.ones((n,), dtype=torch.bfloat16, device="cuda")
+    ops.dropout_forward(x, p, 6, offset=3, out=x)
+    for at in (0, 2 ** 31 - 500, 2 ** 32 - 500):
+        m = min(1500, n - at)
+        assert torch.equal(x[at:at + m].cpu() != 0, kept(m, p, 6, 3 + at)), at
 
 
 def test_dropout_autograd_and_graph_replays_with_a_device_offset():
@@ -364,7 +537,8 @@ def test_quantize_ties_extremes_and_bad_rows():
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8000, 640), (3, 37, 19), (16, 64, 128), (17, 130, 257), (128, 128, 64), (200, 301, 515),
-                                   (130, 260, 2049), (48, 129, 33), (300, 50, 127)])
+                                   (130, 260, 2049), (48, 129, 33), (300, 50, 127), (600, 520, 272), (700, 1040, 1040), (1, 40, 8192),
+                                   (1, 33, 8200), (1, 17, 4099), (20, 300, 640)])
 def test_dense_i8(M, N, K, dtype):
     from weather_model_amd import ops
     x, b = rows(M, (M, K), dtype), rows(N, (N,), torch.float32)

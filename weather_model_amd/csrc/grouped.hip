@@ -285,8 +285,8 @@ __global__ __launch_bounds__(few::THREADS, 6) void grouped_few_kernel(const type
 int check(const char *who, int M, int N, int K, int G, int dtype)
 {
     WM_REQUIRE(M >= 0 && N > 0 && K > 0 && G > 0, WM_ERR_INVALID, "%s: bad sizes M=%d N=%d K=%d groups=%d", who, M, N, K, G);
-    WM_REQUIRE(N <= 1 << 20 && K <= 1 << 20 && G < 1 << 16 && M <= 1 << 30, WM_ERR_UNSUPPORTED,
-               "%s: M=%d N=%d K=%d groups=%d is beyond 2^30 rows, 2^20 columns or 2^16 - 1 groups", who, M, N, K, G);
+    WM_REQUIRE(N <= 1 << 20 && K <= 1 << 20 && G <= 4096 && M <= 1 << 30, WM_ERR_UNSUPPORTED,
+               "%s: M=%d N=%d K=%d groups=%d is beyond 2^30 rows, 2^20 columns or 4096 groups", who, M, N, K, G);
     WM_REQUIRE(dtype == WM_F32 || dtype == WM_BF16 || dtype == WM_F16, WM_ERR_INVALID, "%s: bad dtype %d", who, dtype);
     WM_REQUIRE(wm_num_cus() > 0, WM_ERR_NO_DEVICE, "%s: no HIP device", who);
     return WM_OK;

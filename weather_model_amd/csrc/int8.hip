@@ -69,13 +69,13 @@ __device__ __forceinline__ void quantize_row(const E *__restrict__ row, int K, i
     }
     const float s = top > 3.4028235e38f ? __builtin_nanf("") : top / 127.0f;
     const float r = s > 0.0f ? 1.0f / s : 0.0f;
-    const bool near = r > 3.4028235e38f;     // a subnormal scale has no reciprocal
+    const bool far = r > 3.4028235e38f;      // a subnormal scale has no reciprocal
     auto put = [&](int k, const float (&u)[8]) {
         uint32_t w[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float c = 0.0f;
-            if (s > 0.0f) c = near ? rintf(u[e] / s) : code_of(u[e], s, r);
+            if (s > 0.0f) c = far ? rintf(u[e] / s) : code_of(u[e], s, r);
             c = fminf(fmaxf(c, -127.0f), 127.0f);
             w[e / 4] |= (uint32_t)(uint8_t)(int8_t)c << (8 * (e % 4));
         }
@@ -382,7 +382,7 @@ extern "C" int wm_dense_i8(const void *x, const int8_t *W, const float *wscale, 
     if (int rc = check("wm_dense_i8", M, K, dtype)) return rc;
     WM_REQUIRE(N > 0 && G > 0, WM_ERR_INVALID, "wm_dense_i8: bad sizes N=%d groups=%d", N, G);
     WM_REQUIRE(offsets || G == 1, WM_ERR_INVALID, "wm_dense_i8: %d groups need offsets", G);
-    WM_REQUIRE(N <= 1 << 20 && G < 1 << 16, WM_ERR_UNSUPPORTED, "wm_dense_i8: N=%d groups=%d is beyond 2^20 columns or 2^16 - 1 groups", N, G);
+    WM_REQUIRE(N <= 1 << 20 && G <= 4096, WM_ERR_UNSUPPORTED, "wm_dense_i8: N=%d groups=%d is beyond 2^20 columns or 4096 groups", N, G);
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && wscale && y, WM_ERR_INVALID, "wm_dense_i8: null pointer");
     const size_t need = wm_dense_i8_workspace_bytes(M, K);

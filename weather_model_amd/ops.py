@@ -976,13 +976,23 @@ def _same_device(t, name, like):
     return t
 
 
-def _out_any(out, shape, like, name):
+def _out_any(out, shape, like, name, *inputs):
+    """``out`` checked, or a new tensor; it may not share memory with any of ``inputs``."""
     if out is None:
         return torch.empty(shape, device=like.device, dtype=like.dtype)
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device or \
             not out.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {like.dtype} {tuple(shape)} tensor on {like.device}")
+    for t in inputs:
+        if t is not None and _overlap(out, t):
+            raise ValueError(f"{name} shares memory with an input that the call still reads")
     return out
+
+
+def _overlap(a, b):
+    """Whether two contiguous tensors share memory."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    return pa < pb + b.numel() * b.element_size() and pb < pa + a.numel() * a.element_size()
 
 
 def _call(device, fn, *args):
@@ -1031,7 +1041,7 @@ def dense_grouped_forward(x, weight, offsets, bias=None, relu=False, out=None):
         bias = _req_any(bias, "bias", x)
         if tuple(bias.shape) != (G, N):
             raise ValueError(f"bias must be {(G, N)}, got {tuple(bias.shape)}")
-    y = _out_any(out, (M, N), x, "out")
+    y = _out_any(out, (M, N), x, "out", x, weight, bias, offsets)
     _call(x.device, _lib.lib().wm_dense_grouped_fwd, x.data_ptr(), weight.data_ptr(),
           0 if bias is None else bias.data_ptr(), y.data_ptr(), offsets.data_ptr(), G, M, N, K,
           _DTYPES[x.dtype], 1 if relu else 0)
@@ -1061,8 +1071,8 @@ def dense_grouped_backward(x, weight, offsets, gy, mask_below=None, need_gx=True
               0 if mask_below is None else mask_below.data_ptr(), gx.data_ptr(), offsets.data_ptr(), G, M,
               N, K, dt)
     if need_gw:
-        gw = _out_any(out_w, (G, N, K), x, "out_w")
-        gb = _out_any(out_b, (G, N), x, "out_b") if need_bias else None
+        gw = _out_any(out_w, (G, N, K), x, "out_w", x, gy, offsets)
+        gb = _out_any(out_b, (G, N), x, "out_b", x, gy, gw, offsets) if need_bias else None
         need = L.wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K)
         ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
         _call(x.device, L.wm_dense_grouped_bwd_wb, x.data_ptr(), gy.data_ptr(), gw.data_ptr(),
@@ -1128,7 +1138,11 @@ def dropout_forward(x, p, seed, offset=0, residual=None, out=None):
         residual = _req_any(residual, "residual", x)
         if residual.shape != x.shape:
             raise ValueError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
-    y = torch.empty_like(x) if out is None else _out_any(out, x.shape, x, "out")
+    if out is None:
+        y = torch.empty_like(x)
+    else:                                         # in place, element for element, or apart
+        y = _out_any(out, x.shape, x, "out", *(t for t in (x, residual) if t is not None and
+                                                t.data_ptr() != out.data_ptr()))
     _call(x.device, _lib.lib().wm_dropout, x.data_ptr(), 0 if residual is None else residual.data_ptr(),
           y.data_ptr(), x.numel(), _DTYPES[x.dtype], p, seed, off, off_dev)
     return y
@@ -1199,7 +1213,7 @@ def dense_i8(x, weight, scale, bias=None, relu=False, offsets=None, out=None):
         bias = _same_device(_req(bias, "bias"), "bias", x)
         if bias.shape != scale.shape:
             raise ValueError(f"bias must be {tuple(scale.shape)}, got {tuple(bias.shape)}")
-    y = _out_any(out, (M, N), x, "out")
+    y = _out_any(out, (M, N), x, "out", x, weight, scale, bias, offsets)
     L = _lib.lib()
     need = L.wm_dense_i8_workspace_bytes(M, K)
     ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
