@@ -471,7 +471,7 @@ int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, c
 int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx,
                               const int64_t *offsets, int G, int M, int N, int K, int dtype,
                               void *stream);
-size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K);
+size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K, int dtype);
 int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, void *workspace,
                             size_t workspace_bytes, const int64_t *offsets, int G, int M, int N, int K,
                             int dtype, void *stream);

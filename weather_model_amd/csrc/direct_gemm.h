@@ -19,7 +19,8 @@ namespace tile {
 typedef __attribute__((address_space(3))) const char *lds_ptr;
 __device__ __forceinline__ uint32_t lds_address(const void *p) { return (uint32_t)(uintptr_t)(lds_ptr)p; }
 
-// a raw buffer of `bytes` (at most 2^31 - 1 count) from p
+// a raw buffer of `bytes` (at most 2^31 - 1 count) from p.  A word whose voffset + soffset lies beyond them reads as zero, also where
+// soffset alone does; the sum does not wrap.
 __device__ __forceinline__ u32x4 descriptor(const char *p, long long bytes)
 {
     const uint64_t a = (uint64_t)p;

@@ -14,11 +14,6 @@ using namespace tile;
 
 constexpr int THREADS = 256;                 // of the kernels without tiles
 
-template <class T> __device__ __forceinline__ f32x4 load4_f32(const T *p)
-{
-    return __builtin_convertvector(*reinterpret_cast<const typename Vec4<T>::type *>(p), f32x4);
-}
-
 // ---- rows: out (M, NO) = x (M, C) times W[g], forward (W[g] is (NO, C), its c along memory) or backward
 // (W[g] is (C, NO)).  bias and relu are the forward's, mask the backward's.
 template <class S, bool BACKWARD, bool DIRECT, class E>
@@ -37,7 +32,7 @@ __device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__re
     const E *wg = W + (long long)s.g * NO * C;
     const E *xr = x + (long long)s.row0 * C;
     const E *wt = BACKWARD ? wg + n0 : wg + (long long)n0 * C;
-    constexpr int MI = S::MI, NI = S::NI;
+    constexpr int MI = S::MI;
     typename S::Acc acc = {};
     if constexpr (DIRECT) {
         typename std::conditional<BACKWARD, DirectCols<T, BN, THREADS>, DirectRows<T, BN, THREADS>>::type a;
@@ -53,20 +48,7 @@ __device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__re
         product<S>(a, b, C, lds, acc);
     }
 
-    if constexpr (T::PLANES == 3) {                  // what the split made a NaN of
-        const int ni0 = S::col(), mi0 = S::row();
-#pragma unroll
-        for (int m = 0; m < MI; ++m)
-#pragma unroll
-            for (int n = 0; n < NI; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i = ni0 + 16 * n + k, r = mi0 + 16 * m;
-                    if (acc[m][n][k] != acc[m][n][k] && i < cols && r < s.rows)
-                        acc[m][n][k] = BACKWARD ? dot_again(wt + i, NO, xr + (long long)r * C, 1, C)
-                                                : dot_again(wt + (long long)i * C, 1, xr + (long long)r * C, 1, C);
-                }
-    }
+    if constexpr (T::PLANES == 3) not_finite_again<S>(acc, wt, BACKWARD ? 1 : C, BACKWARD ? NO : 1, xr, C, 1, cols, s.rows, C);
     typedef Out<S, E> O;
     const int col = O::col(), have = min(O::V, cols - col);
     if (S::wave_col() * O::COLS >= cols) return;
@@ -143,7 +125,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
     const int share = ((rows + splits - 1) / splits + STEP - 1) / STEP * STEP;
     row0 += min(rows, split * share);
     rows = min(share, max(0, rows - split * share));
-    constexpr int MI = S::MI, NI = S::NI;
+    constexpr int MI = S::MI;
     typename S::Acc acc = {};
     const int ks = min(BN, K), ns = min(BM, N);
     const E *xt = x + (long long)row0 * K + k0, *yt = gy + (long long)row0 * N + n0;
@@ -179,18 +161,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
         }
         if (sums && (int)threadIdx.x < BM) bias(threadIdx.x, total);
     }
-    if constexpr (T::PLANES == 3) {
-        const int ni0 = S::col(), mi0 = S::row();
-#pragma unroll
-        for (int m = 0; m < MI; ++m)
-#pragma unroll
-            for (int n = 0; n < NI; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int i = ni0 + 16 * n + k, j = mi0 + 16 * m;
-                    if (acc[m][n][k] != acc[m][n][k] && i < ks && j < ns) acc[m][n][k] = dot_again(xt + i, K, yt + j, N, rows);
-                }
-    }
+    if constexpr (T::PLANES == 3) not_finite_again<S>(acc, xt, 1, K, yt, 1, N, ks, ns, rows);
     const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
     auto leave = [&](auto *to) {
         typedef Out<S, typename std::remove_pointer<decltype(to)>::type> O;
@@ -324,7 +295,10 @@ template <> struct Tiles<F32> {
     typedef Shape<F32, 64, 64, 2, 2, 1, 2> MediumQuarter;
 };
 
-bool large(int G, int M, int N) { return M / G >= 512 && N >= 512; }
+// Tiles of 256 x 256 where an average expert has two of them a column and they are at least a quarter of the CUs (in quarters they then
+// fill the card).  bf16 forward, us, 128 x 128 | 256 x 256: 8 experts, 16384 rows of 1024 -> 1024 43 | 36, of 1024 -> 512 25 | 23;
+// 4096 rows of 1024 -> 1024 15 | 16; backward, 512 rows of 8192 -> 2048 46 | 73.
+bool large(int G, int M, int N) { return M / G >= 512 && N >= 512 && (long long)(M / 256) * (N / 256) * 4 >= wm_num_cus(); }
 
 template <class T, bool BACKWARD>
 int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
@@ -341,8 +315,10 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
     return rows_launch<typename Z::Medium, void, typename Z::MediumQuarter, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
-// The few-rows kernel reads an expert's weights once for every 16 of its rows.
-bool few_rows(int G, int M) { return M <= 64 || M / G <= 8; }
+// The few-rows kernel reads an expert's weights once for every 16 of its rows: it is for rows that are few even where one expert has
+// them all.  us, few rows | tiles, 1024 -> 1024: 1 expert bf16 32 rows 8.5 | 8.6, 64 rows 11 | 9.0, float32 64 rows 21 | 24, 96 rows
+// 30 | 24; 16 experts of as many rows bf16 64 rows 9.0 | 12, float32 128 rows 17 | 34; all 128 in one of them 20 | 9.1, 38 | 24.
+bool few_rows(int G, int M, int dtype) { return M <= (G == 1 ? 32 : 64) * (dtype == WM_F32 ? 2 : 1); }
 
 template <class T> int few_launch(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
                                   int relu, hipStream_t st)
@@ -365,12 +341,15 @@ int rows_any(int dtype, const void *x, const void *W, const void *bias, const vo
     }
 }
 
-// Shares of the rows of an expert, whatever tile is taken: enough workgroups of 128 x 128 for two rounds of 256 CUs, at
-// least 256 rows of an average expert each.
-int weight_splits(int M, int N, int K, int G)
+// Shares of the rows of an expert: enough workgroups of 128 x 128 for two rounds of 256 CUs in float32, where a share is long, and one in
+// 16 bits, and so many rows of an average expert each that the sums of the shares cost less.  432 -> 216, us with 1, 2, 4, 8, 16, 32
+// shares: bf16, 8 experts, 45000 rows 76 47 46 51 62 84 (taken: 4), 4096 rows 12 16 17 21 30 46 (1); float32 329 174 98 84 98 126 (8),
+// 37 28 24 27 41 59 (2).
+int weight_splits(int M, int N, int K, int G, int dtype)
 {
+    const int round = dtype == WM_F32 ? 512 : 256, least = dtype == WM_F32 ? 256 : 512;
     const long long tiles = (long long)G * ((N + 127) / 128) * ((K + 127) / 128);
-    const long long want = (512 + tiles - 1) / tiles, most = M / ((long long)G * 256);
+    const long long want = (round + tiles - 1) / tiles, most = M / ((long long)G * least);
     const long long s = want < most ? want : most;
     return s < 1 ? 1 : s > 64 ? 64 : (int)s;
 }
@@ -392,16 +371,17 @@ int weights_launch(const void *x, const void *gy, void *gW, void *gb, float *par
 
 template <class T>
 int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *workspace, const int64_t *offsets, int G, int M, int N, int K,
-                  hipStream_t st)
+                  int splits, hipStream_t st)
 {
     typedef typename T::elem E;
     typedef typename Tiles<T>::Medium Md;
-    const int splits = weight_splits(M, N, K, G);
     float *partial = splits > 1 ? (float *)workspace : nullptr;
     int rc;
     if constexpr (T::PLANES == 1) {
         typedef typename Tiles<T>::Large L;
-        const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N), big = large(1, N, K) && splits == 1;
+        // 256 x 256 where they fill the CUs: 512 rows of 2048 -> 8192 31 -> 25 us, 45000 rows of 8 x 1024 -> 1024 (128 tiles) 53 -> 57
+        const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N),
+                   big = N >= 512 && K >= 512 && splits == 1 && (long long)G * (N / 256) * (K / 256) >= wm_num_cus();
         rc = direct && big ? weights_launch<L, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
              : direct      ? weights_launch<Md, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
                            : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
@@ -426,7 +406,7 @@ extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b,
     if (int rc = check("wm_dense_grouped_fwd", M, N, K, G, dtype)) return rc;
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
-    if (few_rows(G, M)) {
+    if (few_rows(G, M, dtype)) {
         hipStream_t st = (hipStream_t)stream;
         switch (dtype) {
         case WM_F32: return few_launch<F32>(x, W, b, y, offsets, G, M, N, K, relu, st);
@@ -446,10 +426,10 @@ extern "C" int wm_dense_grouped_bwd_data(const void *gy, const void *W, const vo
     return rows_any<true>(dtype, gy, W, nullptr, mask_below, gx, offsets, G, M, K, N, 0, (hipStream_t)stream);
 }
 
-extern "C" size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K)
+extern "C" size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K, int dtype)
 {
     if (M < 0 || N <= 0 || K <= 0 || G <= 0) return 0;
-    const int S = weight_splits(M, N, K, G);
+    const int S = weight_splits(M, N, K, G, dtype);
     return S > 1 ? wm_align_up((size_t)S * G * N * (K + 1) * sizeof(float), 256) : 0;
 }
 
@@ -458,13 +438,14 @@ extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, 
 {
     if (int rc = check("wm_dense_grouped_bwd_wb", M, N, K, G, dtype)) return rc;
     WM_REQUIRE((x && gy || M == 0) && gW && offsets, WM_ERR_INVALID, "wm_dense_grouped_bwd_wb: null pointer");
-    const size_t need = wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K);
+    const size_t need = wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K, dtype);
     WM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), WM_ERR_WORKSPACE,
                "wm_dense_grouped_bwd_wb: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    const int splits = weight_splits(M, N, K, G, dtype);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case WM_F32: return weights_typed<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
-    case WM_BF16: return weights_typed<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
-    default: return weights_typed<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, st);
+    case WM_F32: return weights_typed<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, splits, st);
+    case WM_BF16: return weights_typed<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, splits, st);
+    default: return weights_typed<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, splits, st);
     }
 }

@@ -8,7 +8,6 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
 template <class T> struct Vec4 { typedef T type __attribute__((ext_vector_type(4), aligned(sizeof(T)))); };
-template <class T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T)))); };
 
 template <class T> __device__ __forceinline__ float to_float(T v) { return (float)v; }
 template <class T> __device__ __forceinline__ T from_float(float v) { return (T)v; }

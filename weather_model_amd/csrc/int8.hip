@@ -249,7 +249,7 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
 }
 
 // One row: every workgroup makes the row's codes itself, in LDS, while its first weights are on their way -- the same codes as
-// quantize_rows_kernel's.  A launch of its own for one row took as long as the product (1 x 640 x 8000: 14.9 -> 10.5 us a call).
+// quantize_rows_kernel's.  A launch of its own for one row took as long as the product (1 x 640 x 8000: 14.9 -> 9.3 us a call).
 constexpr int ONE_ROW_K = 8192;
 struct Codes {                               // in LDS, zeros behind the row
     const int8_t *q;
@@ -293,17 +293,22 @@ int check(const char *who, int M, int K, int dtype)
     return WM_OK;
 }
 
-// A wave a row up to 1024 values, a workgroup beyond (8192 rows of 4096 bf16: 25 us = 4.1 TB/s; by single values 54 us).  With
-// fewer rows than CUs the time is one row's chain of load, maximum and codes: more threads a row.
+// A wave a row up to 2048 values, a workgroup beyond.  With few rows the time is one row's chain of load, maximum and codes, and a row
+// is spread over as many threads as leave each a vector.  us, bf16: 8192 rows of 4096 22 (4.7 TB/s; by single values 54); a
+// wave | a workgroup a row: 16384 x 640 12 | 22, 16384 x 2048 24 | 28, 1000 x 640 4.2 | 3.6, 2000 x 2048 6.8 | 5.7; 200 x 8192 by
+// 256 | 1024 threads 6.2 | 4.2.
 template <class E> int quantize(const void *x, int M, int K, int8_t *q, long long ldq, float *scale, hipStream_t st)
 {
 #define WM_QUANTIZE(LANES, NV, THREADS)                                                                                                 \
     hipLaunchKernelGGL((quantize_rows_kernel<E, LANES, NV, THREADS>), dim3((M + THREADS / LANES - 1) / (THREADS / LANES)), dim3(THREADS), \
                        0, st, (const E *)x, M, K, q, ldq, scale)
-    if (K <= 512) WM_QUANTIZE(64, 1, 256);
-    else if (M < wm_num_cus()) WM_QUANTIZE(1024, 1, 1024);
+    const int cus = wm_num_cus();
+    if (M < 4 * cus && K > 4096) WM_QUANTIZE(1024, 1, 1024);
+    else if (M < 4 * cus && K > 2048) WM_QUANTIZE(512, 1, 512);
+    else if (M < (K > 1024 ? 16 : 4) * cus && K <= 2048) WM_QUANTIZE(256, 1, 256);
+    else if (K <= 512) WM_QUANTIZE(64, 1, 256);
     else if (K <= 1024) WM_QUANTIZE(64, 2, 256);
-    else if (K <= 2048) WM_QUANTIZE(256, 1, 256);
+    else if (K <= 2048) WM_QUANTIZE(64, 4, 256);
     else if (K <= 4096) WM_QUANTIZE(256, 2, 256);
     else WM_QUANTIZE(256, 4, 256);
 #undef WM_QUANTIZE
@@ -338,7 +343,7 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     int8_t *q = (int8_t *)workspace + wm_align_up((size_t)M * sizeof(float), 256);
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
-    if (M <= 64 || M / G <= 8) {
+    if (M <= (G == 1 ? 32 : 64)) {               // as in grouped.hip (1024 -> 1024, 16 experts, 128 rows 15 us either way, 256 rows 16 | 15)
         hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, q, ldq, scale, W, wscale, b,
                            (E *)y, (const long long *)offsets, G, M, N, K, relu);
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
@@ -347,7 +352,8 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     typedef Shape<I8, 128, 128, 2, 2> Medium;
     typedef Shape<I8, 64, 64, 2, 2, 2, 2> MediumQuarter;
     if (direct_ok(W, K)) {
-        if (M / G >= 512 && N >= 512)
+        // as in grouped.hip: 8 experts, 16384 rows of 1024 -> 1024 46 | 42 us, 4096 rows 19 | 21
+        if (M / G >= 512 && N >= 512 && (long long)(M / 256) * (N / 256) * 4 >= wm_num_cus())
             return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, Shape<I8, 128, 256, 2, 4>, Shape<I8, 128, 128, 2, 4>, true>(
                 q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
         return dense_tiles<E, Medium, void, MediumQuarter, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);

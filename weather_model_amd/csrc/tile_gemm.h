@@ -12,7 +12,8 @@
 // product is the six piece products that are not below 2^-24 of it: hh, hm, mh, hl, lh, mm, each exact in the
 // float32 accumulator.  That is float32 accuracy (what is left out is 3 2^-26 of |a||b| at most) at 2500 / 6
 // TFLOP/s of matrix rate where the float32 MFMA has 157.  An infinity, a NaN or a value that rounds up to
-// infinity in bf16 makes a NaN of its products; such elements of C are then summed again in float32 (dot_again).
+// infinity in bf16 makes a NaN of its products, and a product next to the largest float32 may overflow in its first
+// piece; elements of C that are not finite are summed again in float32 (not_finite_again).
 #pragma once
 
 #include <type_traits>
@@ -616,12 +617,46 @@ template <class S, class E> struct Out {
     }
 };
 
-// C[i][j] once more in float32, for elements that the split made a NaN of
-__device__ __forceinline__ float dot_again(const float *a, long long sa, const float *b, long long sb, int count)
+// The elements of C that are not finite once more, on the float32 MFMA from memory, by the wave that holds one (`cols` of i and `rows`
+// of j count; element (i, c) of A at a + i ai + c ac).  Where all of them are NaN a launch takes 11 times as long; by a
+// loop over c for each element it took 40 to 150 times as long.
+template <class S>
+__device__ __forceinline__ void not_finite_again(typename S::Acc &acc, const float *a, long long ai, long long ac, const float *b, long long bj,
+                                                 long long bc, int cols, int rows, int count)
 {
-    float s = 0.0f;
-    for (int c = 0; c < count; ++c) s = fmaf(a[c * sa], b[c * sb], s);
-    return s;
+    const auto bad = [&](int m, int n, int k) {
+        return !(fabsf(acc[m][n][k]) <= 3.4028235e38f) && S::col() + 16 * n + k < cols && S::row() + 16 * m < rows;
+    };
+    bool any = false;
+#pragma unroll
+    for (int m = 0; m < S::MI; ++m)
+#pragma unroll
+        for (int n = 0; n < S::NI; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) any |= bad(m, n, k);
+    if (__ballot(any) == 0) return;
+    const int lane = threadIdx.x & 63, i0 = S::wave_col() * (S::BN / S::WN) + (lane & 15), j0 = S::row();
+    // a row of blocks at a time, for the registers' sake
+#pragma unroll
+    for (int m = 0; m < S::MI; ++m) {
+        f32x4 again[S::NI] = {};
+        const float *bp = b + (long long)min(j0 + 16 * m, rows - 1) * bj;
+#pragma unroll 2
+        for (int c0 = 0; c0 < count; c0 += 4) {
+            const int c = c0 + (lane >> 4), have = min(c, count - 1);
+            const float y = c < count ? bp[have * bc] : 0.0f;
+#pragma unroll
+            for (int n = 0; n < S::NI; ++n) {
+                const float x = a[min(i0 + 16 * n, cols - 1) * ai + have * ac];
+                again[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(c < count ? x : 0.0f, y, again[n], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < S::NI; ++n)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (bad(m, n, k)) acc[m][n][k] = again[n][k];
+    }
 }
 
 // ---- ragged rows: group g owns rows offsets[g] .. offsets[g+1] - 1 of M.  Offsets outside 0 .. M are read as
