@@ -34,7 +34,9 @@ class ExpertStack:
                     (l and w.shape[2] != self.w[l - 1].shape[1]):
                 raise ValueError(f"layer {l}: weight {tuple(w.shape)} and bias {tuple(b.shape)} do not fit")
         self.p, self.seed = float(p), int(seed)
-        self.drawn = 0                            # elements of the dropout stream used so far
+        # where each layer's dropout last drew, on the device: the replays of a captured step move on as eager steps do
+        self.drawn = torch.arange(len(weights) - 1, device=self.w[0].device, dtype=torch.int64) << 48
+        self.h = None
         sizes = [t.numel() for t in self.w + self.b]
         self.flat_grads = torch.zeros((sum(sizes),), device=self.w[0].device, dtype=self.w[0].dtype)
         views = self.flat_grads.split(sizes)
@@ -44,28 +46,31 @@ class ExpertStack:
 
     def forward(self, x, offsets, train=False):
         """h_L (M, N_L); with ``train`` dropout is drawn and every activation stays for ``backward``."""
-        h, keep, L = [x], [], len(self.w)
+        h, L = [x], len(self.w)
+        drop = train and L > 1 and self.p > 0
+        if drop:
+            self.drawn.add_(x.shape[0] * max(w.shape[1] for w in self.w[:-1]))
         for l, (w, b) in enumerate(zip(self.w, self.b)):
             y = ops.dense_grouped_forward(h[-1], w, offsets, b, relu=l + 1 < L)
-            if train and l + 1 < L and self.p > 0:
-                ops.dropout_forward(y, self.p, self.seed, offset=self.drawn, out=y)
-                keep.append(self.drawn)
-                self.drawn += y.numel()
+            if drop and l + 1 < L:
+                ops.dropout_forward(y, self.p, self.seed, offset=self.drawn[l:l + 1], out=y)
             h.append(y)
         if train:
-            self.h, self.offsets, self.draws = h, offsets, keep
+            self.h, self.offsets, self.dropped = h, offsets, drop
         return h[-1]
 
     def backward(self, gout):
         """Gradients of every layer from dL/dh_L of the last ``forward(train=True)``.  Returns the flat
         buffer [dW_1..dW_L, db_1..db_L]."""
+        if self.h is None:
+            raise RuntimeError("ExpertStack.backward: call forward(train=True) first")
         g = gout
         for l in range(len(self.w), 0, -1):
             g, _, _ = ops.dense_grouped_backward(self.h[l - 1], self.w[l - 1], self.offsets, g,
                                                  mask_below=self.h[l - 1] if l > 1 else None, need_gx=l > 1,
                                                  out_w=self.gw[l - 1], out_b=self.gb[l - 1])
-            if l > 1 and self.draws:
-                ops.dropout_backward(g, self.p, self.seed, offset=self.draws[l - 2], out=g)
+            if l > 1 and self.dropped:
+                ops.dropout_backward(g, self.p, self.seed, offset=self.drawn[l - 2:l - 1], out=g)
         return self.flat_grads
 
     def step_grads(self, x, offsets, gout):

@@ -1073,12 +1073,20 @@ def dense_grouped_backward(x, weight, offsets, gy, mask_below=None, need_gx=True
     if need_gw:
         gw = _out_any(out_w, (G, N, K), x, "out_w", x, gy, offsets)
         gb = _out_any(out_b, (G, N), x, "out_b", x, gy, gw, offsets) if need_bias else None
-        need = L.wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K)
+        need = L.wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K, dt)
         ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
         _call(x.device, L.wm_dense_grouped_bwd_wb, x.data_ptr(), gy.data_ptr(), gw.data_ptr(),
               0 if gb is None else gb.data_ptr(), 0 if ws is None else ws.data_ptr(), need,
               offsets.data_ptr(), G, M, N, K, dt)
     return gx, gw, gb
+
+
+def _no_capture(name):
+    # A leaf's node that adds up gradients lives as long as any graph of the leaf, on the stream of its first use: a
+    # captured backward pass that meets one of an earlier eager graph works on two streams, and the process ends.
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name}: autograd's backward pass cannot be captured into a graph; capture "
+                           f"{name}_forward and {name}_backward")
 
 
 class DenseGroupedFunction(torch.autograd.Function):
@@ -1094,7 +1102,9 @@ class DenseGroupedFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
+        _no_capture("dense_grouped")
         x, weight, offsets, y = ctx.saved_tensors
         if ctx.own_mask:
             gy = torch.where(y > 0, gy, 0.0)          # stand-alone mask (no fusing consumer), any type
@@ -1106,7 +1116,8 @@ class DenseGroupedFunction(torch.autograd.Function):
 
 
 def dense_grouped(x, weight, offsets, bias=None, relu=False, relu_input=False, relu_bwd_fused=False):
-    """act(weight[g] @ x[r] + bias[g]) for the rows r of each expert g, with gradients."""
+    """act(weight[g] @ x[r] + bias[g]) for the rows r of each expert g, with gradients (of first order; a captured graph
+    takes ``dense_grouped_forward`` and ``dense_grouped_backward``)."""
     return DenseGroupedFunction.apply(x, weight, offsets, bias, relu, relu_input, relu_bwd_fused)
 
 
@@ -1164,7 +1175,9 @@ class DropoutFunction(torch.autograd.Function):
         return dropout_forward(x, p, seed, offset, residual)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
+        _no_capture("dropout")
         offset, = ctx.saved_tensors
         gx = dropout_backward(gy, ctx.p, ctx.seed, ctx.offset if offset is None else offset) \
             if ctx.needs_input_grad[0] else None
@@ -1172,7 +1185,8 @@ class DropoutFunction(torch.autograd.Function):
 
 
 def dropout(x, p, seed, offset=0, residual=None):
-    """``dropout_forward`` with gradients.  A device ``offset`` may be advanced after the backward pass, not
+    """``dropout_forward`` with gradients (of first order; a captured graph takes ``dropout_forward`` and
+    ``dropout_backward``).  A device ``offset`` may be advanced after the backward pass, not
     between the two (autograd notices and refuses)."""
     return DropoutFunction.apply(x, residual, p, seed, offset)
 
