@@ -85,7 +85,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_kernel(const E *__
                                                                   int slots)
 {
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    const RowTiles<S::BM> tiles(offsets, G, M);
+    const RowTiles tiles(offsets, G, M, S::BM);
     const int across = (NO + S::BN - 1) / S::BN;
     const Cut<S, Half, Quarter> cut(blockIdx.x, tiles.total * across, slots);
     if (cut.tile < 0) return;
@@ -100,13 +100,14 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_kernel(const E *__
     else if constexpr (S::ALONE) rows_tile<Half, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
 }
 
-// ---- weights: gW[g] (N, K) = gy^T x over the rows of g.  Split s of S takes its share of each expert's rows;
-// with S > 1 the shares go to `partial` (S, G, N, K), and to (S, G, N) behind it, and grouped_weights_sum_kernel adds
-// them in order.  gb is summed by the workgroups of the first columns from the registers that feed LDS.
+// ---- weights: gW[g] (N, K) = gy^T x over the rows of g: a workgroup takes a tile of one expert's, or with chunk > 0 of `chunk` rows of it.
+// An expert of more than one chunk has them in `partial`, (N, K) each and (N) behind all of them, and
+// grouped_weights_sum_kernel adds them in order.  gb is summed by the workgroups of the first columns from what is in LDS or in the
+// registers that feed it.
 template <class S, bool DIRECT, class E = typename S::T::elem>
 __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E *__restrict__ gy, const E *__restrict__ x, E *__restrict__ gW,
                                                                      E *__restrict__ gb, float *__restrict__ partial, const long long *__restrict__ offsets, int G,
-                                                                     int M, int N, int K, int splits, int first)
+                                                                     int M, int N, int K, int chunk, int chunks, int first)
 {
     typedef typename S::T T;
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
@@ -118,13 +119,21 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
     id /= kt;
     const int n0 = min(id % nt * BM, max(0, N - BM));
     id /= nt;
-    const int split = id % splits, turn = id / splits;
     int g, row0, rows;
-    group_in_turn(offsets, G, M, turn, first, g, row0, rows);
-    constexpr int STEP = T::BKC * 8;
-    const int share = ((rows + splits - 1) / splits + STEP - 1) / STEP * STEP;
-    row0 += min(rows, split * share);
-    rows = min(share, max(0, rows - split * share));
+    float *own = nullptr, *own_bias = nullptr;               // where a part of an expert's sums goes
+    if (chunk > 0) {
+        const RowTiles map(offsets, G, M, chunk);
+        if (id >= map.total) return;
+        const Segment s = map.tile(id);
+        if (s.g < 0 || s.g >= G) return;
+        g = s.g, row0 = s.row0, rows = s.rows;
+        if (s.parts > 1) {
+            own = partial + (long long)id * N * K;
+            own_bias = partial + (long long)chunks * N * K + (long long)id * N;
+        }
+    } else {
+        group_in_turn(offsets, G, M, id, first, g, row0, rows);
+    }
     constexpr int MI = S::MI;
     typename S::Acc acc = {};
     const int ks = min(BN, K), ns = min(BM, N);
@@ -132,7 +141,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
     const bool sums = gb && k0 == 0;
     auto bias = [&](int j, float v) {
         if (j >= ns) return;
-        if (partial) partial[(long long)splits * G * N * K + ((long long)split * G + g) * N + n0 + j] = v;
+        if (own) own_bias[n0 + j] = v;
         else gb[(long long)g * N + n0 + j] = from_float<E>(v);
     };
     if constexpr (DIRECT) {
@@ -162,7 +171,6 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
         if (sums && (int)threadIdx.x < BM) bias(threadIdx.x, total);
     }
     if constexpr (T::PLANES == 3) not_finite_again<S>(acc, xt, 1, K, yt, 1, N, ks, ns, rows);
-    const long long at = (((long long)(partial ? split * G + g : g) * N + n0) * K) + k0;
     auto leave = [&](auto *to) {
         typedef Out<S, typename std::remove_pointer<decltype(to)>::type> O;
         const int col = O::col(), have = min(O::V, ks - col);
@@ -177,24 +185,38 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
         }
     };
     __syncthreads();                                 // the bias sums have left LDS
-    if (partial) leave(partial + at);
-    else leave(gW + at);
+    if (own) leave(own + (long long)n0 * K + k0);
+    else leave(gW + ((long long)g * N + n0) * K + k0);
 }
 
+// gW and gb of the experts that are in `partial` or have no rows; blockIdx.y is the expert.
 template <class E>
-__global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const float *__restrict__ partial, E *__restrict__ gW, long long count,
-                                                                      E *__restrict__ gb, long long bcount, int S)
+__global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const float *__restrict__ partial, E *__restrict__ gW, E *__restrict__ gb,
+                                                                      const long long *__restrict__ offsets, int G, int M, int N, long long count,
+                                                                      int chunk, int chunks)
 {
-    const float *bias = partial + S * count;
-    for (long long e = (long long)blockIdx.x * THREADS + threadIdx.x; e < count + (gb ? bcount : 0); e += (long long)gridDim.x * THREADS) {
-        const bool w = e < count;
-        const float *p = w ? partial + e : bias + (e - count);
-        const long long step = w ? count : bcount;
-        float s = p[0];
-        for (int k = 1; k < S; ++k) s += p[k * step];
-        if (w) gW[e] = from_float<E>(s);
-        else gb[e - count] = from_float<E>(s);
-    }
+    const int g = blockIdx.y;
+    int first, parts;
+    RowTiles(offsets, G, M, chunk).tiles_of(g, first, parts);
+    if (parts == 1) return;
+    // `n` sums from p, `step` apart, four at a time
+    const auto add = [&](const float *p, long long step, E *to, long long n) {
+        for (long long e = 4 * ((long long)blockIdx.x * THREADS + threadIdx.x); e < n; e += 4ll * gridDim.x * THREADS) {
+            const int have = n - e < 4 ? (int)(n - e) : 4;
+            f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (have == 4) {
+#pragma unroll 4
+                for (int k = 0; k < parts; ++k) s += *reinterpret_cast<const Vec4<float>::type *>(p + k * step + e);
+                store4(to + e, s);
+            } else {
+                for (int k = 0; k < parts; ++k)
+                    for (int i = 0; i < have; ++i) s[i] += p[k * step + e + i];
+                for (int i = 0; i < have; ++i) to[e + i] = from_float<E>(s[i]);
+            }
+        }
+    };
+    add(partial + first * count, count, gW + g * count, count);
+    if (gb) add(partial + chunks * count + (long long)first * N, N, gb + (long long)g * N, N);
 }
 
 // ---- few rows: y (M, N) for groups of a handful of rows.  One read of the weights is the cost, so a workgroup takes 16
@@ -341,59 +363,63 @@ int rows_any(int dtype, const void *x, const void *W, const void *bias, const vo
     }
 }
 
-// Shares of the rows of an expert: enough workgroups of 128 x 128 for two rounds of 256 CUs in float32, where a share is long, and one in
-// 16 bits, and so many rows of an average expert each that the sums of the shares cost less.  432 -> 216, us with 1, 2, 4, 8, 16, 32
-// shares: bf16, 8 experts, 45000 rows 76 47 46 51 62 84 (taken: 4), 4096 rows 12 16 17 21 30 46 (1); float32 329 174 98 84 98 126 (8),
-// 37 28 24 27 41 59 (2).
-int weight_splits(int M, int N, int K, int G, int dtype)
+// Rows of a chunk, or 0 for whole experts: workgroups of 128 x 128 for two rounds of 256 CUs in float32, where a chunk takes long, and for
+// one in 16 bits, and so many rows each that the sums of the chunks cost less.  Chunks are counted in rows and not in experts, as
+// one expert may have most of the rows.  432 -> 216, us with 1, 2, 4, 8, 16, 32 chunks an expert: bf16, 8 experts, 45000 rows 76 47 46 51
+// 62 84 (taken: 4), 4096 rows 12 16 17 21 30 46 (1); float32 329 174 98 84 98 126 (8), 37 28 24 27 41 59 (2).  Where the experts are
+// enough, but one alone would be far from filling the card, those of more than twice the average are cut: 64 experts, 45000 rows in one of
+// them 2500 us whole in float32, 570 in bf16; evenly spread it costs the launch that finds nothing to add.
+int weight_chunk(int M, int N, int K, int G, int dtype)
 {
     const int round = dtype == WM_F32 ? 512 : 256, least = dtype == WM_F32 ? 256 : 512;
-    const long long tiles = (long long)G * ((N + 127) / 128) * ((K + 127) / 128);
-    const long long want = (round + tiles - 1) / tiles, most = M / ((long long)G * least);
-    const long long s = want < most ? want : most;
-    return s < 1 ? 1 : s > 64 ? 64 : (int)s;
+    const long long tiles = (long long)((N + 127) / 128) * ((K + 127) / 128), want = (round + tiles - 1) / tiles;
+    const bool enough = want <= G;
+    if (M <= least || (enough && (tiles * 8 >= round || M < 16 * least))) return 0;
+    const int rows = (int)wm_align_up((size_t)(enough ? 2ll * M / G : (M + want - 1) / want), 64);
+    return rows < least ? least : rows;
 }
+long long chunks_most(int G, int M, int chunk) { return chunk ? row_tiles_most(G, M, chunk) : 0; }
 
 template <class S, bool DIRECT>
 int weights_launch(const void *x, const void *gy, void *gW, void *gb, float *partial, const int64_t *offsets, int G, int M, int N, int K,
-                   int splits, hipStream_t st)
+                   int chunk, hipStream_t st)
 {
     typedef typename S::T::elem E;
-    const long long blocks = (long long)splits * G * ((N + S::BM - 1) / S::BM) * ((K + S::BN - 1) / S::BN);
+    const long long chunks = chunks_most(G, M, chunk), blocks = (chunk ? chunks : G) * ((N + S::BM - 1) / S::BM) * ((K + S::BN - 1) / S::BN);
     if (int rc = blocks_ok("wm_dense_grouped_bwd_wb", blocks)) return rc;
-    // groups begun on empty CUs, where all workgroups run at once
-    const long long first = blocks <= 2ll * wm_num_cus() && !S::ALONE ? wm_num_cus() / (blocks / G) : G;
+    // experts begun on empty CUs, where all workgroups run at once
+    const long long first = !chunk && blocks <= 2ll * wm_num_cus() && !S::ALONE ? wm_num_cus() / (blocks / G) : G;
     hipLaunchKernelGGL((grouped_weights_kernel<S, DIRECT>), dim3((unsigned)blocks), dim3(S::THREADS), 0, st, (const E *)gy, (const E *)x, (E *)gW,
-                       (E *)gb, partial, (const long long *)offsets, G, M, N, K, splits, (int)first);
+                       (E *)gb, partial, (const long long *)offsets, G, M, N, K, chunk, (int)chunks, (int)first);
     WM_LAUNCH_CHECK("grouped_weights_kernel");
     return WM_OK;
 }
 
 template <class T>
 int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *workspace, const int64_t *offsets, int G, int M, int N, int K,
-                  int splits, hipStream_t st)
+                  int chunk, hipStream_t st)
 {
     typedef typename T::elem E;
     typedef typename Tiles<T>::Medium Md;
-    float *partial = splits > 1 ? (float *)workspace : nullptr;
+    float *partial = (float *)workspace;
     int rc;
     if constexpr (T::PLANES == 1) {
         typedef typename Tiles<T>::Large L;
-        // 256 x 256 where they fill the CUs: 512 rows of 2048 -> 8192 31 -> 25 us, 45000 rows of 8 x 1024 -> 1024 (128 tiles) 53 -> 57
+        // 256 x 256 where they fill the CUs: 512 rows of 2048 -> 8192 31 -> 25 us, 16384 rows of 8 x 1024 -> 1024 (128 tiles) 53 -> 57
         const bool direct = direct_ok(x, 2ll * K) && direct_ok(gy, 2ll * N),
-                   big = N >= 512 && K >= 512 && splits == 1 && (long long)G * (N / 256) * (K / 256) >= wm_num_cus();
-        rc = direct && big ? weights_launch<L, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
-             : direct      ? weights_launch<Md, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st)
-                           : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
+                   big = N >= 512 && K >= 512 && !chunk && (long long)G * (N / 256) * (K / 256) >= wm_num_cus();
+        rc = direct && big ? weights_launch<L, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, chunk, st)
+             : direct      ? weights_launch<Md, true>(x, gy, gW, gb, partial, offsets, G, M, N, K, chunk, st)
+                           : weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, chunk, st);
     } else {
-        rc = weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, splits, st);
+        rc = weights_launch<Md, false>(x, gy, gW, gb, partial, offsets, G, M, N, K, chunk, st);
     }
-    if (rc != WM_OK || splits == 1) return rc;
-    const long long count = (long long)G * N * K;
-    long long grid = (count + THREADS - 1) / THREADS;
-    if (grid > 4096) grid = 4096;
-    hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid), dim3(THREADS), 0, st, (const float *)workspace, (E *)gW, count, (E *)gb,
-                       (long long)G * N, splits);
+    if (rc != WM_OK || !chunk) return rc;
+    const long long count = (long long)N * K;
+    long long grid = (count + 4 * THREADS - 1) / (4 * THREADS);
+    if (grid > 1024) grid = 1024;
+    hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid, G), dim3(THREADS), 0, st, (const float *)partial, (E *)gW, (E *)gb,
+                       (const long long *)offsets, G, M, N, count, chunk, (int)chunks_most(G, M, chunk));
     WM_LAUNCH_CHECK("grouped_weights_sum_kernel");
     return WM_OK;
 }
@@ -429,8 +455,8 @@ extern "C" int wm_dense_grouped_bwd_data(const void *gy, const void *W, const vo
 extern "C" size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K, int dtype)
 {
     if (M < 0 || N <= 0 || K <= 0 || G <= 0) return 0;
-    const int S = weight_splits(M, N, K, G, dtype);
-    return S > 1 ? wm_align_up((size_t)S * G * N * (K + 1) * sizeof(float), 256) : 0;
+    const int chunk = weight_chunk(M, N, K, G, dtype);
+    return chunk ? wm_align_up((size_t)chunks_most(G, M, chunk) * N * (K + 1) * sizeof(float), 256) : 0;
 }
 
 extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, void *workspace, size_t workspace_bytes,
@@ -441,11 +467,11 @@ extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, 
     const size_t need = wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K, dtype);
     WM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), WM_ERR_WORKSPACE,
                "wm_dense_grouped_bwd_wb: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
-    const int splits = weight_splits(M, N, K, G, dtype);
+    const int chunk = weight_chunk(M, N, K, G, dtype);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-    case WM_F32: return weights_typed<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, splits, st);
-    case WM_BF16: return weights_typed<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, splits, st);
-    default: return weights_typed<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, splits, st);
+    case WM_F32: return weights_typed<F32>(x, gy, gW, gb, workspace, offsets, G, M, N, K, chunk, st);
+    case WM_BF16: return weights_typed<BF16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, chunk, st);
+    default: return weights_typed<F16>(x, gy, gW, gb, workspace, offsets, G, M, N, K, chunk, st);
     }
 }

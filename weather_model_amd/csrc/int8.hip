@@ -168,7 +168,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void dense_i8_kernel(const int8_t *_
                                                               const long long *__restrict__ offsets, int G, int M, int N, int K, int relu, int slots)
 {
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    const RowTiles<S::BM> tiles(offsets, G, M);
+    const RowTiles tiles(offsets, G, M, S::BM);
     const int across = (N + S::BN - 1) / S::BN;
     const Cut<S, Half, Quarter> cut(blockIdx.x, tiles.total * across, slots);
     if (cut.tile < 0) return;

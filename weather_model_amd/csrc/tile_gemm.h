@@ -664,6 +664,7 @@ __device__ __forceinline__ void not_finite_again(typename S::Acc &acc, const flo
 // Rows that no group owns are the segments -1 (before offsets[0]) and G (behind offsets[G]).
 struct Segment {
     int g, row0, rows;                       // group, first row and rows of a tile
+    int parts;                               // tiles of the group
 };
 
 // a lane's value, in a scalar register
@@ -693,12 +694,12 @@ __device__ __forceinline__ void segment_bounds(const long long *offsets, int G, 
     lo = __builtin_amdgcn_update_dpp(carry, hi, 0x138, 0xF, 0xF, false);         // one lane up
 }
 
-// The map from a tile's number to its rows, built once a workgroup; what up to 62 groups need stays in the lanes.
-template <int BM> struct RowTiles {
+// The map from the number of a tile of BM rows to its rows, built once a workgroup; what up to 62 groups need stays in the lanes.
+struct RowTiles {
     const long long *offsets;
-    int G, M, lo, hi, total;                 // bounds of the first 64 segments
+    int G, M, BM, lo, hi, total;             // bounds of the first 64 segments
 
-    __device__ __forceinline__ RowTiles(const long long *offsets_, int G_, int M_) : offsets(offsets_), G(G_), M(M_), total(0)
+    __device__ __forceinline__ RowTiles(const long long *offsets_, int G_, int M_, int BM_) : offsets(offsets_), G(G_), M(M_), BM(BM_), total(0)
     {
         int carry = 0;
         for (int s0 = 0; s0 < G + 2; s0 += 64) {
@@ -719,12 +720,28 @@ template <int BM> struct RowTiles {
             if (holds) {
                 const int k = __builtin_ctzll(holds);
                 const int row0 = lane_value(l, k) + (t - lane_value(upto - n, k)) * BM;
-                return {s0 + k - 1, row0, min(lane_value(h, k) - row0, BM)};
+                return {s0 + k - 1, row0, min(lane_value(h, k) - row0, BM), lane_value(n, k)};
             }
             before = lane_value(upto, 63);
             carry = lane_value(h, 63);
         }
-        return {0, 0, 0};
+        return {0, 0, 0, 0};
+    }
+    // the first tile of group g and how many it has
+    __device__ __forceinline__ void tiles_of(int g, int &first, int &count) const
+    {
+        int before = 0, carry = 0, l = lo, h = hi;
+        for (int s0 = 0;; s0 += 64) {
+            if (s0 > 0) segment_bounds(offsets, G, M, s0, carry, l, h);
+            const int n = (h - l + BM - 1) / BM, upto = before + wave_scan(n);
+            if (g + 1 < s0 + 64) {
+                count = lane_value(n, g + 1 - s0);
+                first = lane_value(upto, g + 1 - s0) - count;
+                return;
+            }
+            before = lane_value(upto, 63);
+            carry = lane_value(h, 63);
+        }
     }
 };
 
