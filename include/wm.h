@@ -465,12 +465,16 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
  * gb.  Any values of offsets are safe: those outside 0 .. M count as the nearest inside, one below its
  * predecessor counts as that.  Results are bitwise reproducible.  float32 products are formed from three
  * bf16 pieces of each factor, with float32 accuracy; infinities and NaN come out as in float32 arithmetic.
- * N, K <= 2^20, M <= 2^30, G <= 4096.  Outputs may not overlap inputs. */
-int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, const int64_t *offsets,
-                         int G, int M, int N, int K, int dtype, int relu, void *stream);
+ * N, K <= 2^20, M <= 2^30, G <= 4096.  Outputs may not overlap inputs;
+ * workspaces (0 bytes: none is needed) are 16-byte aligned. */
+size_t wm_dense_grouped_fwd_workspace_bytes(int G, int M, int N, int K, int dtype);
+int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, void *workspace,
+                         size_t workspace_bytes, const int64_t *offsets, int G, int M, int N, int K,
+                         int dtype, int relu, void *stream);
+size_t wm_dense_grouped_bwd_data_workspace_bytes(int G, int M, int N, int K, int dtype);
 int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx,
-                              const int64_t *offsets, int G, int M, int N, int K, int dtype,
-                              void *stream);
+                              void *workspace, size_t workspace_bytes, const int64_t *offsets, int G, int M,
+                              int N, int K, int dtype, void *stream);
 size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K, int dtype);
 int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, void *gb, void *workspace,
                             size_t workspace_bytes, const int64_t *offsets, int G, int M, int N, int K,

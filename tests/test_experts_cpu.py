@@ -51,17 +51,21 @@ def test_c_abi_refusals():
     refused(L.wm_dropout(p, 0, p, 4, 0, float("nan"), 0, 0, 0, 0), -1, b"probability")
     refused(L.wm_dropout(p, 0, p, 4, 1, 0.1, 0, 0, 0, 0), -1, b"dtype")
     refused(L.wm_dropout(0, 0, p, 4, 0, 0.1, 0, 0, 0, 0), -1, b"null pointer")
-    refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 0, 4, 4, 4, 0, 0, 0), -1, b"bad sizes")
-    refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 1, -1, 4, 4, 0, 0, 0), -1, b"bad sizes")
-    refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 1, 4, 4, (1 << 20) + 1, 0, 0, 0), -2, b"beyond")
-    refused(L.wm_dense_grouped_fwd(p, p, 0, p, p, 4097, 4, 4, 4, 0, 0, 0), -2, b"4096 groups")
-    refused(L.wm_dense_grouped_bwd_data(p, p, 0, p, p, 1, 4, 4, 4, 1, 0), -1, b"dtype")
+    refused(L.wm_dense_grouped_fwd(p, p, 0, p, 0, 0, p, 0, 4, 4, 4, 0, 0, 0), -1, b"bad sizes")
+    refused(L.wm_dense_grouped_fwd(p, p, 0, p, 0, 0, p, 1, -1, 4, 4, 0, 0, 0), -1, b"bad sizes")
+    refused(L.wm_dense_grouped_fwd(p, p, 0, p, 0, 0, p, 1, 4, 4, (1 << 20) + 1, 0, 0, 0), -2, b"beyond")
+    refused(L.wm_dense_grouped_fwd(p, p, 0, p, 0, 0, p, 4097, 4, 4, 4, 0, 0, 0), -2, b"4096 groups")
+    refused(L.wm_dense_grouped_bwd_data(p, p, 0, p, 0, 0, p, 1, 4, 4, 4, 1, 0), -1, b"dtype")
     refused(L.wm_dense_grouped_bwd_wb(p, p, p, 0, 0, 0, p, 1, 4, 0, 4, 0, 0), -1, b"bad sizes")
     refused(L.wm_quantize_rows_i8(p, 4, (1 << 17) + 1, 0, p, p, 0), -2, b"32 bits")
     refused(L.wm_quantize_rows_i8(p, 4, 0, 0, p, p, 0), -1, b"bad sizes")
     refused(L.wm_dense_i8(p, p, p, 0, p, 0, 1, 4, 4, 4, 7, 0, p, 64, 0), -1, b"dtype")
     assert L.wm_dense_i8_workspace_bytes(0, 4) == 0 and L.wm_dense_i8_workspace_bytes(3, 0) == 0
     assert L.wm_dense_grouped_bwd_wb_workspace_bytes(0, 4, 4, 4, 0) == 0
+    assert L.wm_dense_grouped_fwd_workspace_bytes(1, 16, 64, 8192, 0) == 0          # few rows
+    assert L.wm_dense_grouped_fwd_workspace_bytes(1, 200, 64, 500, 0) == 0          # no long contraction
+    assert L.wm_dense_grouped_fwd_workspace_bytes(1, 200, 64, 8192, 0) >= 200 * 64 * 4 * 2
+    assert L.wm_dense_grouped_bwd_data_workspace_bytes(1, 16, 8192, 64, 2) >= 16 * 64 * 4 * 2
 
 
 def test_product_sizes_do_not_overflow_the_workspace_query():

@@ -80,6 +80,10 @@ SHAPES = [
     ([1100, 1000], 136, 2056, 0, 2),               # and backward
     ([2048], 2048, 72, 0, 0),                      # quarters
     ([33, 40], 2064, 4104, 0, 0),                  # gradients of weights in tiles of 256 x 256
+    ([70, 0, 131], 40, 3000, 2, 1),                # few tiles and a long contraction: in parts, forward
+    ([70, 0, 131], 3001, 41, 2, 1),                # and backward
+    ([3], 1100, 96, 0, 0),
+    ([300] * 3, 24, 1096, 0, 0),
 ]
 
 

@@ -79,8 +79,10 @@ SIGNATURES = {
     "wm_dense_bwd_f32": (c_int, [vp, vp, vp, vp, vp, vp, vp, vp, c_sz, c_int, c_int, c_int, vp]),
     "wm_mse_metrics_workspace_bytes": (c_sz, [c_i64]),
     "wm_mse_metrics_f32": (c_int, [vp, vp, c_int, c_i64, c_int, c_f32, vp, vp, vp, c_sz, vp]),
-    "wm_dense_grouped_fwd": (c_int, [vp] * 5 + [c_int] * 6 + [vp]),
-    "wm_dense_grouped_bwd_data": (c_int, [vp] * 5 + [c_int] * 5 + [vp]),
+    "wm_dense_grouped_fwd_workspace_bytes": (c_sz, [c_int] * 5),
+    "wm_dense_grouped_fwd": (c_int, [vp] * 5 + [c_sz, vp] + [c_int] * 6 + [vp]),
+    "wm_dense_grouped_bwd_data_workspace_bytes": (c_sz, [c_int] * 5),
+    "wm_dense_grouped_bwd_data": (c_int, [vp] * 5 + [c_sz, vp] + [c_int] * 5 + [vp]),
     "wm_dense_grouped_bwd_wb_workspace_bytes": (c_sz, [c_int] * 5),
     "wm_dense_grouped_bwd_wb": (c_int, [vp] * 5 + [c_sz, vp] + [c_int] * 5 + [vp]),
     "wm_dropout": (c_int, [vp, vp, vp, c_i64, c_int, c_f64, c_u64, c_u64, vp, vp]),

@@ -219,6 +219,20 @@ __device__ __forceinline__ void product_direct(DA &a, DB &b, int count, int rows
     product_direct<S, RING, false>(a, b, count, rows, lds, acc, none);
 }
 
+// Whether tiles of 256 x 256, one a CU, end before those of 128 x 128, two a CU: by the rounds that each makes, the last of them cut (Cut).
+// A round of the larger takes 1.5 times as long (1024 deep in bf16: 34 | 22 us); parts of a round as measured.  bf16, us, 128 | 256:
+// 8 experts, 16384 rows of 1024 -> 1024 45 | 37, 12 experts, 20000 rows of 1000 -> 1000 81 | 63, 22 experts, 14612 rows of 2976 -> 1320
+// 215 | 207 and backward 211 | 169, 2 experts, 30000 rows of 512 -> 640 33 | 36; 512 rows of 8192 -> 2048 37 | 59.
+inline bool tiles_of_256(int G, int M, int N, int cus)
+{
+    if (M / G < 256 || N < 256) return false;
+    const auto time = [&](int size, long long slots, int whole, int half, int quarter) {
+        const long long t = ((long long)M / size + G / 2) * ((N + size - 1) / size), left = t % slots;
+        return t / slots * whole + (left == 0 ? 0 : left * 4 <= slots ? quarter : left * 2 <= slots ? half : whole);
+    };
+    return time(256, cus, 100, 60, 38) < time(128, 2ll * cus, 68, 44, 36);
+}
+
 inline bool direct_ok(const void *p, long long ld_bytes) { return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0; }
 
 }  // namespace tile

@@ -16,9 +16,11 @@ constexpr int THREADS = 256;                 // of the kernels without tiles
 
 // ---- rows: out (M, NO) = x (M, C) times W[g], forward (W[g] is (NO, C), its c along memory) or backward
 // (W[g] is (C, NO)).  bias and relu are the forward's, mask the backward's.
-template <class S, bool BACKWARD, bool DIRECT, class E>
+// Of the contraction the C values from c0 on, of `depth`; out is of the type of x, or float32 for a part of the sums.
+template <class S, bool BACKWARD, bool DIRECT, class E, class OUT>
 __device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias, const E *__restrict__ mask,
-                                          E *__restrict__ out, char *lds, Segment s, int n0, int G, int M, int NO, int C, int relu)
+                                          OUT *__restrict__ out, char *lds, Segment s, int n0, int G, int M, int NO, int depth, int c0, int C,
+                                          int relu)
 {
     typedef typename S::T T;
     constexpr int BM = S::BM, BN = S::BN, THREADS = S::THREADS;
@@ -26,35 +28,35 @@ __device__ __forceinline__ void rows_tile(const E *__restrict__ x, const E *__re
     const int cols = min(BN, NO - n0);
     if (s.rows <= 0 || cols <= 0) return;
     if (s.g < 0 || s.g >= G) {                       // rows of no expert: zeros
-        for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) out[(long long)(s.row0 + e / cols) * NO + n0 + e % cols] = (E)0.0f;
+        for (int e = threadIdx.x; e < s.rows * cols; e += THREADS) out[(long long)(s.row0 + e / cols) * NO + n0 + e % cols] = (OUT)0.0f;
         return;
     }
-    const E *wg = W + (long long)s.g * NO * C;
-    const E *xr = x + (long long)s.row0 * C;
-    const E *wt = BACKWARD ? wg + n0 : wg + (long long)n0 * C;
+    const E *wg = W + (long long)s.g * NO * depth;
+    const E *xr = x + (long long)s.row0 * depth + c0;
+    const E *wt = BACKWARD ? wg + (long long)c0 * NO + n0 : wg + (long long)n0 * depth + c0;
     constexpr int MI = S::MI;
     typename S::Acc acc = {};
     if constexpr (DIRECT) {
         typename std::conditional<BACKWARD, DirectCols<T, BN, THREADS>, DirectRows<T, BN, THREADS>>::type a;
         DirectRows<T, BM, THREADS> b;
-        a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
-        b.init(xr, C, s.rows, C, x + (long long)M * C);
+        a.init(wt, BACKWARD ? NO : depth, cols, C, W + (long long)G * NO * depth);
+        b.init(xr, depth, s.rows, C, x + (long long)M * depth);
         product_direct<S, S::RING>(a, b, C, s.rows, lds, acc);
     } else {
         typename std::conditional<BACKWARD, Strided<T, BN, THREADS>, Contiguous<T, BN, THREADS>>::type a;
         Contiguous<T, BM, THREADS> b;
-        a.init(wt, BACKWARD ? NO : C, cols, C, W + (long long)G * NO * C);
-        b.init(xr, C, s.rows, C, x + (long long)M * C);
+        a.init(wt, BACKWARD ? NO : depth, cols, C, W + (long long)G * NO * depth);
+        b.init(xr, depth, s.rows, C, x + (long long)M * depth);
         product<S>(a, b, C, lds, acc);
     }
 
-    if constexpr (T::PLANES == 3) not_finite_again<S>(acc, wt, BACKWARD ? 1 : C, BACKWARD ? NO : 1, xr, C, 1, cols, s.rows, C);
-    typedef Out<S, E> O;
+    if constexpr (T::PLANES == 3) not_finite_again<S>(acc, wt, BACKWARD ? 1 : depth, BACKWARD ? NO : 1, xr, depth, 1, cols, s.rows, C);
+    typedef Out<S, OUT> O;
     const int col = O::col(), have = min(O::V, cols - col);
     if (S::wave_col() * O::COLS >= cols) return;
     float add[O::V] = {};
     if (!BACKWARD && bias) O::load(bias + (long long)s.g * NO + n0 + col, have, add);
-    E *to = out + (long long)s.row0 * NO + n0 + col;
+    OUT *to = out + (long long)s.row0 * NO + n0 + col;
     const E *mk = mask ? mask + (long long)s.row0 * NO + n0 + col : nullptr;
 #pragma unroll
     for (int m = 0; m < MI; ++m) {
@@ -95,9 +97,47 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_kernel(const E *__
     const int n0 = min(ct * S::BN, max(0, NO - S::BN));      // the last tile moves back over its neighbour
     s.row0 += cut.row;
     s.rows -= cut.row;
-    if (cut.parts == 1) rows_tile<S, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0, G, M, NO, C, relu);
-    else if (cut.parts == 4) rows_tile<Quarter, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
-    else if constexpr (S::ALONE) rows_tile<Half, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, relu);
+    if (cut.parts == 1) rows_tile<S, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0, G, M, NO, C, 0, C, relu);
+    else if (cut.parts == 4) rows_tile<Quarter, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, 0, C, relu);
+    else if constexpr (S::ALONE) rows_tile<Half, BACKWARD, DIRECT>(x, W, bias, mask, out, lds, s, n0 + cut.col, G, M, NO, C, 0, C, relu);
+}
+
+// Few tiles and a long contraction: blockIdx.y is a part of `depth` values of it, whose sums go to `partial`, (M, NO) each.
+template <class S, bool BACKWARD, bool DIRECT, class E = typename S::T::elem>
+__global__ __launch_bounds__(S::THREADS, 2) void grouped_rows_part_kernel(const E *__restrict__ x, const E *__restrict__ W, const E *__restrict__ bias,
+                                                                       float *__restrict__ partial, const long long *__restrict__ offsets, int G, int M,
+                                                                       int NO, int C, int depth)
+{
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+    const RowTiles tiles(offsets, G, M, S::BM);
+    const int across = (NO + S::BN - 1) / S::BN, c0 = blockIdx.y * depth;
+    if ((int)blockIdx.x >= tiles.total * across) return;
+    const int n0 = min((int)blockIdx.x % across * S::BN, max(0, NO - S::BN));      // the last tile moves back over its neighbour
+    rows_tile<S, BACKWARD, DIRECT>(x, W, c0 == 0 ? bias : nullptr, (const E *)nullptr, partial + (long long)blockIdx.y * M * NO, lds,
+                                   tiles.tile(blockIdx.x / across), n0, G, M, NO, C, c0, min(depth, C - c0), 0);
+}
+template <class E>
+__global__ __launch_bounds__(THREADS) void grouped_rows_sum_kernel(const float *__restrict__ partial, const E *__restrict__ mask, E *__restrict__ out,
+                                                                   long long count, int parts, int relu)
+{
+    const long long e = 4 * ((long long)blockIdx.x * THREADS + threadIdx.x);
+    const int have = count - e < 4 ? (int)(count - e) : 4;
+    if (have <= 0) return;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = 0; k < parts; ++k) {
+        const float *p = partial + k * count + e;
+        if (have == 4) s += *reinterpret_cast<const Vec4<float>::type *>(p);
+        else
+            for (int i = 0; i < have; ++i) s[i] += p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (relu) s[i] = relu_of(s[i]);
+        if (mask && i < have) s[i] = to_float(mask[e + i]) > 0.0f ? s[i] : 0.0f;
+    }
+    if (have == 4) store4(out + e, s);
+    else
+        for (int i = 0; i < have; ++i) out[e + i] = from_float<E>(s[i]);
 }
 
 // ---- weights: gW[g] (N, K) = gy^T x over the rows of g: a workgroup takes a tile of one expert's, or with chunk > 0 of `chunk` rows of it.
@@ -291,6 +331,13 @@ int blocks_ok(const char *who, long long blocks)
     return WM_OK;
 }
 
+int workspace_ok(const char *who, size_t need, const void *workspace, size_t bytes)
+{
+    WM_REQUIRE(need == 0 || (workspace && bytes >= need), WM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", who, need, bytes);
+    WM_REQUIRE(need == 0 || ((uintptr_t)workspace & 15) == 0, WM_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
+    return WM_OK;
+}
+
 template <class S, class Half, class Quarter, bool BACKWARD, bool DIRECT>
 int rows_launch(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
                 int C, int relu, hipStream_t st)
@@ -317,23 +364,59 @@ template <> struct Tiles<F32> {
     typedef Shape<F32, 64, 64, 2, 2, 1, 2> MediumQuarter;
 };
 
-// Tiles of 256 x 256 where an average expert has two of them a column and they are at least a quarter of the CUs (in quarters they then
-// fill the card).  bf16 forward, us, 128 x 128 | 256 x 256: 8 experts, 16384 rows of 1024 -> 1024 43 | 36, of 1024 -> 512 25 | 23;
-// 4096 rows of 1024 -> 1024 15 | 16; backward, 512 rows of 8192 -> 2048 46 | 73.
-bool large(int G, int M, int N) { return M / G >= 512 && N >= 512 && (long long)(M / 256) * (N / 256) * 4 >= wm_num_cus(); }
+// Values of the contraction that a workgroup takes where tiles of 64 x 64 are too few to hide a long one, or 0: whole.  us, whole | in parts,
+// forward and backward: float32 1 expert, 100 rows of 1024 -> 1024 24 29 | 14 15, of 4096 82 99 | 25 28, 1024 rows of 4096 -> 1024 83
+// 100 | 65 72, 16 experts, 200 rows of 2048 -> 256 43 52 | 20 22, 128 rows of 640 -> 8000 18 22 | 21 22 (not taken); 16 bits are
+// quicker through a contraction: 6 experts, 1579 rows of 3599 -> 247 29 39 | 22 27, 100 rows of 4096 -> 1024 19 25 | 14 15, of 1024 10
+// 11 | 13 15, 512 rows of 2048 -> 1024 11 15 | 14 15 (not taken).
+int rows_depth(int G, int M, int NO, int C, int dtype)
+{
+    const bool f32 = dtype == WM_F32;
+    const long long tiles = ((long long)M / 64 + (G < M ? G : M) / 2 + 1) * ((NO + 63) / 64);      // about
+    if (C < (!f32 ? 2304 : tiles <= 256 ? 512 : 2048) || tiles > (f32 ? 512 : 256)) return 0;
+    long long parts = tiles <= 256 ? 512 / tiles : 1024 / tiles;
+    if (parts > (f32 ? 10 : 4)) parts = f32 ? 10 : 4;
+    if (parts > C / (f32 ? 128 : 512)) parts = C / (f32 ? 128 : 512);
+    return (int)wm_align_up((size_t)((C + parts - 1) / parts), 64);
+}
+size_t rows_bytes(int G, int M, int NO, int C, int dtype)
+{
+    const int depth = rows_depth(G, M, NO, C, dtype);
+    return depth ? wm_align_up((size_t)((C + depth - 1) / depth) * M * NO * sizeof(float), 256) : 0;
+}
+
+template <class S, bool BACKWARD, bool DIRECT>
+int rows_parts(const void *x, const void *W, const void *bias, const void *mask, void *out, float *partial, const int64_t *offsets, int G, int M,
+               int NO, int C, int relu, int depth, hipStream_t st)
+{
+    typedef typename S::T::elem E;
+    const long long blocks = row_tiles_most(G, M, S::BM) * ((NO + S::BN - 1) / S::BN), count = (long long)M * NO;
+    const int parts = (C + depth - 1) / depth;
+    if (int rc = blocks_ok("wm_dense_grouped", blocks * parts)) return rc;
+    hipLaunchKernelGGL((grouped_rows_part_kernel<S, BACKWARD, DIRECT>), dim3((unsigned)blocks, parts), dim3(S::THREADS), 0, st, (const E *)x, (const E *)W,
+                       (const E *)bias, partial, (const long long *)offsets, G, M, NO, C, depth);
+    WM_LAUNCH_CHECK("grouped_rows_part_kernel");
+    hipLaunchKernelGGL(grouped_rows_sum_kernel<E>, dim3((unsigned)((count + 4 * THREADS - 1) / (4 * THREADS))), dim3(THREADS), 0, st, (const float *)partial,
+                       (const E *)mask, (E *)out, count, parts, relu);
+    WM_LAUNCH_CHECK("grouped_rows_sum_kernel");
+    return WM_OK;
+}
 
 template <class T, bool BACKWARD>
-int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
-               int C, int relu, hipStream_t st)
+int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, void *workspace, const int64_t *offsets, int G, int M,
+               int NO, int C, int relu, hipStream_t st)
 {
     typedef Tiles<T> Z;
+    const int depth = rows_depth(G, M, NO, C, std::is_same<T, F32>::value ? WM_F32 : WM_BF16);
     if constexpr (T::PLANES == 1) {
         if (direct_ok(x, 2ll * C) && direct_ok(W, BACKWARD ? 2ll * NO : 2ll * C)) {
-            if (large(G, M, NO))
+            if (depth) return rows_parts<typename Z::MediumQuarter, BACKWARD, true>(x, W, bias, mask, out, (float *)workspace, offsets, G, M, NO, C, relu, depth, st);
+            if (tiles_of_256(G, M, NO, wm_num_cus()))
                 return rows_launch<typename Z::Large, typename Z::LargeHalf, typename Z::LargeQuarter, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
             return rows_launch<typename Z::Medium, void, typename Z::MediumQuarter, BACKWARD, true>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
         }
     }
+    if (depth) return rows_parts<typename Z::MediumQuarter, BACKWARD, false>(x, W, bias, mask, out, (float *)workspace, offsets, G, M, NO, C, relu, depth, st);
     return rows_launch<typename Z::Medium, void, typename Z::MediumQuarter, BACKWARD, false>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
 }
 
@@ -353,13 +436,13 @@ template <class T> int few_launch(const void *x, const void *W, const void *b, v
 }
 
 template <bool BACKWARD>
-int rows_any(int dtype, const void *x, const void *W, const void *bias, const void *mask, void *out, const int64_t *offsets, int G, int M, int NO,
-             int C, int relu, hipStream_t st)
+int rows_any(int dtype, const void *x, const void *W, const void *bias, const void *mask, void *out, void *workspace, const int64_t *offsets, int G,
+             int M, int NO, int C, int relu, hipStream_t st)
 {
     switch (dtype) {
-    case WM_F32: return rows_typed<F32, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-    case WM_BF16: return rows_typed<BF16, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
-    default: return rows_typed<F16, BACKWARD>(x, W, bias, mask, out, offsets, G, M, NO, C, relu, st);
+    case WM_F32: return rows_typed<F32, BACKWARD>(x, W, bias, mask, out, workspace, offsets, G, M, NO, C, relu, st);
+    case WM_BF16: return rows_typed<BF16, BACKWARD>(x, W, bias, mask, out, workspace, offsets, G, M, NO, C, relu, st);
+    default: return rows_typed<F16, BACKWARD>(x, W, bias, mask, out, workspace, offsets, G, M, NO, C, relu, st);
     }
 }
 
@@ -426,12 +509,18 @@ int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *works
 
 }  // namespace
 
-extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
-                                    int dtype, int relu, void *stream)
+extern "C" size_t wm_dense_grouped_fwd_workspace_bytes(int G, int M, int N, int K, int dtype)
+{
+    return M > 0 && N > 0 && K > 0 && G > 0 && !few_rows(G, M, dtype) ? rows_bytes(G, M, N, K, dtype) : 0;
+}
+
+extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, void *workspace, size_t workspace_bytes,
+                                    const int64_t *offsets, int G, int M, int N, int K, int dtype, int relu, void *stream)
 {
     if (int rc = check("wm_dense_grouped_fwd", M, N, K, G, dtype)) return rc;
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
+    if (int rc = workspace_ok("wm_dense_grouped_fwd", wm_dense_grouped_fwd_workspace_bytes(G, M, N, K, dtype), workspace, workspace_bytes)) return rc;
     if (few_rows(G, M, dtype)) {
         hipStream_t st = (hipStream_t)stream;
         switch (dtype) {
@@ -440,16 +529,23 @@ extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b,
         default: return few_launch<F16>(x, W, b, y, offsets, G, M, N, K, relu, st);
         }
     }
-    return rows_any<false>(dtype, x, W, b, nullptr, y, offsets, G, M, N, K, relu, (hipStream_t)stream);
+    return rows_any<false>(dtype, x, W, b, nullptr, y, workspace, offsets, G, M, N, K, relu, (hipStream_t)stream);
 }
 
-extern "C" int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx, const int64_t *offsets, int G, int M,
-                                         int N, int K, int dtype, void *stream)
+extern "C" size_t wm_dense_grouped_bwd_data_workspace_bytes(int G, int M, int N, int K, int dtype)
+{
+    return M > 0 && N > 0 && K > 0 && G > 0 ? rows_bytes(G, M, K, N, dtype) : 0;
+}
+
+extern "C" int wm_dense_grouped_bwd_data(const void *gy, const void *W, const void *mask_below, void *gx, void *workspace, size_t workspace_bytes,
+                                         const int64_t *offsets, int G, int M, int N, int K, int dtype, void *stream)
 {
     if (int rc = check("wm_dense_grouped_bwd_data", M, N, K, G, dtype)) return rc;
     if (M == 0) return WM_OK;
     WM_REQUIRE(gy && W && gx && offsets, WM_ERR_INVALID, "wm_dense_grouped_bwd_data: null pointer");
-    return rows_any<true>(dtype, gy, W, nullptr, mask_below, gx, offsets, G, M, K, N, 0, (hipStream_t)stream);
+    if (int rc = workspace_ok("wm_dense_grouped_bwd_data", wm_dense_grouped_bwd_data_workspace_bytes(G, M, N, K, dtype), workspace, workspace_bytes))
+        return rc;
+    return rows_any<true>(dtype, gy, W, nullptr, mask_below, gx, workspace, offsets, G, M, K, N, 0, (hipStream_t)stream);
 }
 
 extern "C" size_t wm_dense_grouped_bwd_wb_workspace_bytes(int G, int M, int N, int K, int dtype)
@@ -464,9 +560,7 @@ extern "C" int wm_dense_grouped_bwd_wb(const void *x, const void *gy, void *gW, 
 {
     if (int rc = check("wm_dense_grouped_bwd_wb", M, N, K, G, dtype)) return rc;
     WM_REQUIRE((x && gy || M == 0) && gW && offsets, WM_ERR_INVALID, "wm_dense_grouped_bwd_wb: null pointer");
-    const size_t need = wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K, dtype);
-    WM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), WM_ERR_WORKSPACE,
-               "wm_dense_grouped_bwd_wb: workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+    if (int rc = workspace_ok("wm_dense_grouped_bwd_wb", wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K, dtype), workspace, workspace_bytes)) return rc;
     const int chunk = weight_chunk(M, N, K, G, dtype);
     hipStream_t st = (hipStream_t)stream;
     switch (dtype) {

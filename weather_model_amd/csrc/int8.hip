@@ -352,8 +352,7 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     typedef Shape<I8, 128, 128, 2, 2> Medium;
     typedef Shape<I8, 64, 64, 2, 2, 2, 2> MediumQuarter;
     if (direct_ok(W, K)) {
-        // as in grouped.hip: 8 experts, 16384 rows of 1024 -> 1024 46 | 42 us, 4096 rows 19 | 21
-        if (M / G >= 512 && N >= 512 && (long long)(M / 256) * (N / 256) * 4 >= wm_num_cus())
+        if (tiles_of_256(G, M, N, wm_num_cus()))
             return dense_tiles<E, Shape<I8, 256, 256, 2, 4>, Shape<I8, 128, 256, 2, 4>, Shape<I8, 128, 128, 2, 4>, true>(
                 q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);
         return dense_tiles<E, Medium, void, MediumQuarter, true>(q, ldq, scale, W, wscale, b, y, offsets, G, M, N, K, relu, st);

@@ -589,13 +589,13 @@ template <class S, class E> struct Out {
         __builtin_amdgcn_wave_barrier();
     }
     // up to V consecutive elements
-    static __device__ __forceinline__ void load(const E *p, int have, float (&v)[V])
+    template <class F> static __device__ __forceinline__ void load(const F *p, int have, float (&v)[V])
     {
-        typedef E vec __attribute__((ext_vector_type(V), aligned(sizeof(E))));
+        typedef F vec __attribute__((ext_vector_type(V), aligned(sizeof(F))));
         if (have >= V) {
             const vec x = *reinterpret_cast<const vec *>(p);
 #pragma unroll
-            for (int k = 0; k < V; ++k) v[k] = to_float((E)x[k]);
+            for (int k = 0; k < V; ++k) v[k] = to_float((F)x[k]);
         } else {
 #pragma unroll
             for (int k = 0; k < V; ++k) v[k] = k < have ? to_float(p[k]) : 0.0f;
@@ -762,7 +762,11 @@ __device__ __forceinline__ void group_rows(const long long *offsets, int G, int 
     row0 = rows = 0;
 }
 
-inline long long row_tiles_most(int G, int M, int BM) { return (M + (long long)(G + 2) * (BM - 1)) / BM; }
+inline long long row_tiles_most(int G, int M, int BM)
+{
+    const long long n = (M + (long long)(G + 2) * (BM - 1)) / BM;
+    return n < M ? n : M;                    // none is empty
+}
 
 // Workgroups go round the eight XCDs in turn: logical tiles are dealt out so that an XCD works on a run of
 // them, and a run keeps to `band` row tiles and walks the columns, so that its operands stay in its L2.

@@ -12,6 +12,7 @@ raises otherwise -- there is no CPU path in the product.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import numpy as np
@@ -1006,6 +1007,20 @@ def _call(device, fn, *args):
             _lib.check(fn(*args, stream))
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(name, *sizes):
+    return getattr(_lib.lib(), name + "_workspace_bytes")(*sizes)
+
+
+def _workspace(device, name, *sizes):
+    """(tensor, address, bytes) of the workspace of one call"""
+    need = _workspace_bytes(name, *sizes)
+    if need == 0:
+        return None, 0, 0
+    ws = torch.empty((need,), device=device, dtype=torch.uint8)
+    return ws, ws.data_ptr(), need
+
+
 def _grouped_args(x, weight, offsets):
     x = _req_any(x, "input")
     weight = _req_any(weight, "weight", x)
@@ -1042,9 +1057,11 @@ def dense_grouped_forward(x, weight, offsets, bias=None, relu=False, out=None):
         if tuple(bias.shape) != (G, N):
             raise ValueError(f"bias must be {(G, N)}, got {tuple(bias.shape)}")
     y = _out_any(out, (M, N), x, "out", x, weight, bias, offsets)
+    dt = _DTYPES[x.dtype]
+    ws, at, size = _workspace(x.device, "wm_dense_grouped_fwd", G, M, N, K, dt)
     _call(x.device, _lib.lib().wm_dense_grouped_fwd, x.data_ptr(), weight.data_ptr(),
-          0 if bias is None else bias.data_ptr(), y.data_ptr(), offsets.data_ptr(), G, M, N, K,
-          _DTYPES[x.dtype], 1 if relu else 0)
+          0 if bias is None else bias.data_ptr(), y.data_ptr(), at, size, offsets.data_ptr(), G, M, N, K,
+          dt, 1 if relu else 0)
     return y
 
 
@@ -1067,17 +1084,16 @@ def dense_grouped_backward(x, weight, offsets, gy, mask_below=None, need_gx=True
             if tuple(mask_below.shape) != (M, K):
                 raise ValueError(f"mask must be {(M, K)}, got {tuple(mask_below.shape)}")
         gx = torch.empty((M, K), device=x.device, dtype=x.dtype)
+        ws, at, size = _workspace(x.device, "wm_dense_grouped_bwd_data", G, M, N, K, dt)
         _call(x.device, L.wm_dense_grouped_bwd_data, gy.data_ptr(), weight.data_ptr(),
-              0 if mask_below is None else mask_below.data_ptr(), gx.data_ptr(), offsets.data_ptr(), G, M,
-              N, K, dt)
+              0 if mask_below is None else mask_below.data_ptr(), gx.data_ptr(), at, size,
+              offsets.data_ptr(), G, M, N, K, dt)
     if need_gw:
         gw = _out_any(out_w, (G, N, K), x, "out_w", x, gy, offsets)
         gb = _out_any(out_b, (G, N), x, "out_b", x, gy, gw, offsets) if need_bias else None
-        need = L.wm_dense_grouped_bwd_wb_workspace_bytes(G, M, N, K, dt)
-        ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
+        ws, at, size = _workspace(x.device, "wm_dense_grouped_bwd_wb", G, M, N, K, dt)
         _call(x.device, L.wm_dense_grouped_bwd_wb, x.data_ptr(), gy.data_ptr(), gw.data_ptr(),
-              0 if gb is None else gb.data_ptr(), 0 if ws is None else ws.data_ptr(), need,
-              offsets.data_ptr(), G, M, N, K, dt)
+              0 if gb is None else gb.data_ptr(), at, size, offsets.data_ptr(), G, M, N, K, dt)
     return gx, gw, gb
 
 
@@ -1228,12 +1244,10 @@ def dense_i8(x, weight, scale, bias=None, relu=False, offsets=None, out=None):
         if bias.shape != scale.shape:
             raise ValueError(f"bias must be {tuple(scale.shape)}, got {tuple(bias.shape)}")
     y = _out_any(out, (M, N), x, "out", x, weight, scale, bias, offsets)
-    L = _lib.lib()
-    need = L.wm_dense_i8_workspace_bytes(M, K)
-    ws = torch.empty((need,), device=x.device, dtype=torch.uint8) if need else None
-    _call(x.device, L.wm_dense_i8, x.data_ptr(), weight.data_ptr(), scale.data_ptr(),
+    ws, at, size = _workspace(x.device, "wm_dense_i8", M, K)
+    _call(x.device, _lib.lib().wm_dense_i8, x.data_ptr(), weight.data_ptr(), scale.data_ptr(),
           0 if bias is None else bias.data_ptr(), y.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
-          G, M, N, K, _DTYPES[x.dtype], 1 if relu else 0, 0 if ws is None else ws.data_ptr(), need)
+          G, M, N, K, _DTYPES[x.dtype], 1 if relu else 0, at, size)
     return y
 
 
