@@ -88,7 +88,7 @@ template <class T, int UNROLL, bool EARLY = false> struct Dot {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int c = rounds * ROUND + h * PIECE, left = K - c - at();
-                acc = piece<T>(load16_guarded<E>(w + c, end, left), x.part(c + at(), left), acc);
+                acc = piece<T>(load16_of_row<E>(w - at(), c + at(), K, end), x.part(c + at(), left), acc);
             }
         return acc;
     }
@@ -97,7 +97,7 @@ template <class T, int UNROLL, bool EARLY = false> struct Dot {
 template <class T> struct RowOf {
     const typename T::elem *x, *end;
     __device__ __forceinline__ u32x4 whole(int c) const { return *reinterpret_cast<const u32x4u *>(x + c); }
-    __device__ __forceinline__ u32x4 part(int c, int left) const { return load16_guarded<typename T::elem>(x + c, end, left); }
+    __device__ __forceinline__ u32x4 part(int c, int left) const { return load16_of_row<typename T::elem>(x, c, c + left, end); }
 };
 
 }  // namespace few

@@ -115,6 +115,21 @@ template <class E> __device__ __forceinline__ u32x4 load16_guarded(const E *p, c
     return v;
 }
 
+// 16 bytes from value `pos` on of a row of `count` values that lie within a tensor ending at `end`; zeros behind the row.  Whatever would
+// leave the row is read as its last 16 bytes and moved down: value after value, the one tile that meets the end of a tensor held up
+// the launch (33 experts, 2999 rows, float16: 333 -> 515 forward 13.9 -> 11.4 us, gradients of rows 19.9 -> 17.9, of weights 25.4 -> 19.7).
+template <class E> __device__ __forceinline__ u32x4 load16_of_row(const E *row, int pos, int count, const E *end)
+{
+    constexpr int N = 16 / sizeof(E);
+    if (count < N) return load16_guarded<E>(row + pos, end, count - pos);
+    const int at = min(pos, count - N), down = min((pos - at) * (int)sizeof(E), 16) * 8;
+    const u32x4 v = *reinterpret_cast<const u32x4u *>(row + at);
+    const uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+    const uint64_t a = down == 0 ? lo : down < 64 ? lo >> down | hi << (64 - down) : down < 128 ? hi >> (down - 64) : 0,
+                   b = down < 64 ? hi >> down : 0;
+    return u32x4{(uint32_t)a, (uint32_t)(a >> 32), (uint32_t)b, (uint32_t)(b >> 32)};
+}
+
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b)
 {
     typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -191,12 +206,11 @@ template <class T, int ROWS, int THREADS> struct Contiguous {
     }
     __device__ __forceinline__ void load_guarded(Regs &reg, int c0) const
     {
-        const E *at = base + c0;
+        const int pos = c0 + q * T::ECH;
 #pragma unroll
         for (int j = 0; j < PER; ++j)
 #pragma unroll
-            for (int h = 0; h < LOADS; ++h)
-                reg.v[j][h] = load16_guarded<E>(at + off[j] + h * 4, end, count - c0 - q * T::ECH - h * 4);
+            for (int h = 0; h < LOADS; ++h) reg.v[j][h] = load16_of_row<E>(base + off[j] - q * T::ECH, pos + h * 4, count, end);
     }
     __device__ __forceinline__ void store(const Regs &reg, char *lds) const
     {
@@ -281,6 +295,22 @@ template <class T, int ROWS, int THREADS> struct Strided {
     }
     __device__ __forceinline__ void load_guarded(Regs &reg, int c0) const
     {
+        if (!slow) {                         // the last c again for those behind it
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int c = c0 + q * 8 + e;
+                const E *p = base + (long long)min(c, count - 1) * ld + r0;
+                if constexpr (WORDS == 1) {
+                    reg.v[e][0] = *reinterpret_cast<const u32u *>(p);
+                } else {
+                    const words v = *reinterpret_cast<const words *>(p);
+#pragma unroll
+                    for (int w = 0; w < WORDS; ++w) reg.v[e][w] = v[w];
+                }
+            }
+            trim(reg, c0);
+            return;
+        }
         const E *at = base + (long long)c0 * ld;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
