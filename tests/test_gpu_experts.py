@@ -128,10 +128,11 @@ def test_grouped_backward(case, dtype):
         at += n
 
 
-def test_grouped_weight_gradient_split_over_rows():
+@pytest.mark.parametrize("N,K", [(24, 70), (216, 201)])
+def test_grouped_weight_gradient_split_over_rows(N, K):
     """Few small weights and many rows: the rows are split over workgroups and joined in a fixed order."""
     from weather_model_amd import _lib, ops
-    sizes, N, K = [9000, 0, 5001], 24, 70
+    sizes = [9000, 0, 5001]
     assert _lib.lib().wm_dense_grouped_bwd_wb_workspace_bytes(3, sum(sizes), N, K, 0) > 0
     for dtype in TYPES:
         x, gy = rows(1, (sum(sizes), K), dtype), rows(2, (sum(sizes), N), dtype)
@@ -144,6 +145,23 @@ def test_grouped_weight_gradient_split_over_rows():
             a, c = gy[at:at + n].double(), x[at:at + n].double()
             close(runs[0][1][g], a.t() @ c, a.abs().t() @ c.abs(), n, g)
             close(runs[0][2][g], a.sum(0), a.abs().sum(0), n, g, norm=False)
+            at += n
+
+
+def test_grouped_weight_gradient_of_one_expert_with_most_of_the_rows():
+    """Many experts, one of which is cut in chunks; the others are not, or have no rows at all."""
+    from weather_model_amd import ops
+    sizes, N, K = [3] * 20 + [9001] + [0] * 10 + [40] * 9, 40, 72
+    for dtype in TYPES:
+        x, gy = rows(1, (sum(sizes), K), dtype), rows(2, (sum(sizes), N), dtype)
+        w = torch.zeros((len(sizes), N, K), dtype=dtype, device="cuda")
+        _, gw, gb = ops.dense_grouped_backward(x.cuda(), w, offsets_of(sizes), gy.cuda(), need_gx=False,
+                                               out_w=torch.full_like(w, 7), out_b=torch.full((len(sizes), N), 7, dtype=dtype, device="cuda"))
+        at = 0
+        for g, n in enumerate(sizes):
+            a, c = gy[at:at + n].double(), x[at:at + n].double()
+            close(gw[g], a.t() @ c, a.abs().t() @ c.abs(), n, g)
+            close(gb[g], a.sum(0), a.abs().sum(0), n, g, norm=False)
             at += n
 
 

@@ -229,6 +229,7 @@ __global__ __launch_bounds__(S::THREADS, 2) void grouped_weights_kernel(const E 
     else leave(gW + ((long long)g * N + n0) * K + k0);
 }
 
+constexpr long long FEW_SUMS = 1 << 15;
 // gW and gb of the experts that are in `partial` or have no rows; blockIdx.y is the expert.
 template <class E>
 __global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const float *__restrict__ partial, E *__restrict__ gW, E *__restrict__ gb,
@@ -239,19 +240,35 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const floa
     int first, parts;
     RowTiles(offsets, G, M, chunk).tiles_of(g, first, parts);
     if (parts == 1) return;
-    // `n` sums from p, `step` apart, four at a time
+    // `n` sums from p, `step` apart; the parts of small weights are shared out over the waves (100000 rows of 64 x 64 in 391 parts: 87 -> 46
+    // us; 4096 rows of 432 x 216 in 16: 16 -> 21, not taken)
+    __shared__ f32x4 join[4][64];
+    const bool shared = parts > 8 && count <= FEW_SUMS;
+    const int at = shared ? threadIdx.x & 63 : threadIdx.x, wave = shared ? threadIdx.x >> 6 : 0, waves = shared ? 4 : 1;
+    const long long span = shared ? 256 : 4 * THREADS;
     const auto add = [&](const float *p, long long step, E *to, long long n) {
-        for (long long e = 4 * ((long long)blockIdx.x * THREADS + threadIdx.x); e < n; e += 4ll * gridDim.x * THREADS) {
+        for (long long e0 = span * blockIdx.x; e0 < n; e0 += span * gridDim.x) {
+            const long long e = e0 + 4 * at;
             const int have = n - e < 4 ? (int)(n - e) : 4;
             f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
             if (have == 4) {
-#pragma unroll 4
-                for (int k = 0; k < parts; ++k) s += *reinterpret_cast<const Vec4<float>::type *>(p + k * step + e);
-                store4(to + e, s);
+#pragma unroll 8
+                for (int k = wave; k < parts; k += waves) s += *reinterpret_cast<const Vec4<float>::type *>(p + k * step + e);
             } else {
-                for (int k = 0; k < parts; ++k)
+                for (int k = wave; k < parts; k += waves)
                     for (int i = 0; i < have; ++i) s[i] += p[k * step + e + i];
-                for (int i = 0; i < have; ++i) to[e + i] = from_float<E>(s[i]);
+            }
+            if (shared) {
+                join[wave][at] = s;
+                __syncthreads();
+                s = join[0][at];
+                for (int w = 1; w < 4; ++w) s += join[w][at];
+                __syncthreads();
+            }
+            if (wave == 0) {
+                if (have == 4) store4(to + e, s);
+                else
+                    for (int i = 0; i < have; ++i) to[e + i] = from_float<E>(s[i]);
             }
         }
     };
@@ -421,9 +438,9 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows: it is for rows that are few even where one expert has
-// them all.  us, few rows | tiles, 1024 -> 1024: 1 expert bf16 32 rows 8.5 | 8.6, 64 rows 11 | 9.0, float32 64 rows 21 | 24, 96 rows
-// 30 | 24; 16 experts of as many rows bf16 64 rows 9.0 | 12, float32 128 rows 17 | 34; all 128 in one of them 20 | 9.1, 38 | 24.
-bool few_rows(int G, int M, int dtype) { return M <= (G == 1 ? 32 : 64) * (dtype == WM_F32 ? 2 : 1); }
+// them all.  us, few rows | tiles, 1024 -> 1024: 1 expert bf16 32 rows 8.5 | 8.6, 64 rows 11 | 9.0, float32 32 rows 11 | 14, 64 rows
+// 21 | 14; 16 experts, 64 rows, bf16 9.0 | 12, float32 18 | 20; 128 rows, all in one of them, 20 | 9.1, 38 | 24.
+bool few_rows(int G, int M) { return M <= 32 || (M <= 64 && G >= 4); }
 
 template <class T> int few_launch(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
                                   int relu, hipStream_t st)
@@ -448,18 +465,20 @@ int rows_any(int dtype, const void *x, const void *W, const void *bias, const vo
 
 // Rows of a chunk, or 0 for whole experts: workgroups of 128 x 128 for two rounds of 256 CUs in float32, where a chunk takes long, and for
 // one in 16 bits, and so many rows each that the sums of the chunks cost less.  Chunks are counted in rows and not in experts, as
-// one expert may have most of the rows.  432 -> 216, us with 1, 2, 4, 8, 16, 32 chunks an expert: bf16, 8 experts, 45000 rows 76 47 46 51
-// 62 84 (taken: 4), 4096 rows 12 16 17 21 30 46 (1); float32 329 174 98 84 98 126 (8), 37 28 24 27 41 59 (2).  Where the experts are
-// enough, but one alone would be far from filling the card, those of more than twice the average are cut: 64 experts, 45000 rows in one of
-// them 2500 us whole in float32, 570 in bf16; evenly spread it costs the launch that finds nothing to add.
+// one expert may have most of the rows; experts of fewer than two chunks on average are cut only where they have twice the average.
+// 432 -> 216, us with 1, 2, 4, 8, 16, 32 chunks an expert: bf16, 8 experts, 45000 rows 76 47 46 51 62 84 (taken: 4); float32 329 174
+// 98 84 98 126 (8); with at least 128, 256, 512, 1024 rows: bf16, 1 expert, 4096 rows 19 15 16 21 (taken: 256), 17112 rows of 16 x 73 -> 116
+// 15 15 20 28; float32 27 30 43 70 (128), 23 27 40 66.  Where the experts are enough, but one alone would be far from filling the card: 64
+// experts, 45000 rows in one of them 2500 us whole in float32, 570 in bf16; 101 and 52 in chunks; evenly spread it costs the launch that
+// finds nothing to add.
 int weight_chunk(int M, int N, int K, int G, int dtype)
 {
-    const int round = dtype == WM_F32 ? 512 : 256, least = dtype == WM_F32 ? 256 : 512;
+    const int round = dtype == WM_F32 ? 512 : 256, least = dtype == WM_F32 ? 128 : 256;
     const long long tiles = (long long)((N + 127) / 128) * ((K + 127) / 128), want = (round + tiles - 1) / tiles;
     const bool enough = want <= G;
-    if (M <= least || (enough && (tiles * 8 >= round || M < 16 * least))) return 0;
-    const int rows = (int)wm_align_up((size_t)(enough ? 2ll * M / G : (M + want - 1) / want), 64);
-    return rows < least ? least : rows;
+    if (M <= 2 * least || (enough && (tiles * 8 >= round || M < 32 * least))) return 0;
+    const long long rows = enough || M / G < 2 * least ? 2ll * M / G : (M + want - 1) / want;
+    return (int)wm_align_up((size_t)(rows < least ? least : rows), 64);
 }
 long long chunks_most(int G, int M, int chunk) { return chunk ? row_tiles_most(G, M, chunk) : 0; }
 
@@ -499,8 +518,7 @@ int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *works
     }
     if (rc != WM_OK || !chunk) return rc;
     const long long count = (long long)N * K;
-    long long grid = (count + 4 * THREADS - 1) / (4 * THREADS);
-    if (grid > 1024) grid = 1024;
+    const long long many = (count + 1023) / 1024, grid = count <= FEW_SUMS ? (count + 255) / 256 : many > 1024 ? 1024 : many;
     hipLaunchKernelGGL(grouped_weights_sum_kernel<E>, dim3((unsigned)grid, G), dim3(THREADS), 0, st, (const float *)partial, (E *)gW, (E *)gb,
                        (const long long *)offsets, G, M, N, count, chunk, (int)chunks_most(G, M, chunk));
     WM_LAUNCH_CHECK("grouped_weights_sum_kernel");
@@ -511,7 +529,7 @@ int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *works
 
 extern "C" size_t wm_dense_grouped_fwd_workspace_bytes(int G, int M, int N, int K, int dtype)
 {
-    return M > 0 && N > 0 && K > 0 && G > 0 && !few_rows(G, M, dtype) ? rows_bytes(G, M, N, K, dtype) : 0;
+    return M > 0 && N > 0 && K > 0 && G > 0 && !few_rows(G, M) ? rows_bytes(G, M, N, K, dtype) : 0;
 }
 
 extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, void *workspace, size_t workspace_bytes,
@@ -521,7 +539,7 @@ extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b,
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
     if (int rc = workspace_ok("wm_dense_grouped_fwd", wm_dense_grouped_fwd_workspace_bytes(G, M, N, K, dtype), workspace, workspace_bytes)) return rc;
-    if (few_rows(G, M, dtype)) {
+    if (few_rows(G, M)) {
         hipStream_t st = (hipStream_t)stream;
         switch (dtype) {
         case WM_F32: return few_launch<F32>(x, W, b, y, offsets, G, M, N, K, relu, st);

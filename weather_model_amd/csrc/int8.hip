@@ -343,7 +343,7 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     int8_t *q = (int8_t *)workspace + wm_align_up((size_t)M * sizeof(float), 256);
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
-    if (M <= (G == 1 ? 32 : 64)) {               // as in grouped.hip (1024 -> 1024, 16 experts, 128 rows 15 us either way, 256 rows 16 | 15)
+    if (M <= 32 || (M <= 64 && G >= 4)) {        // as in grouped.hip (1024 -> 1024, 16 experts, 128 rows 15 us either way, 256 rows 16 | 15)
         hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, q, ldq, scale, W, wscale, b,
                            (E *)y, (const long long *)offsets, G, M, N, K, relu);
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
