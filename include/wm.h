@@ -499,9 +499,9 @@ int wm_dropout(const void *x, const void *residual, void *y, int64_t n, int dtyp
  * what serves a trained Dense layer (convolution.py:175-176, model.predict) from weights of a byte each.
  * W (G, N, K) int8, wscale and b (G, N) float32 (b may be NULL), y (M, N) of `dtype`; offsets as in
  * wm_dense_grouped_fwd, or NULL with G = 1: all rows use the one W.  The sums are exact integers (K <= 2^17).
- * The workspace (16-byte aligned) holds the codes and scales of x; one row of K <= 8192 needs none. */
+ * The workspace (16-byte aligned) holds the codes and scales of x; a few short rows need none. */
 int wm_quantize_rows_i8(const void *x, int M, int K, int dtype, int8_t *q, float *scale, void *stream);
-size_t wm_dense_i8_workspace_bytes(int M, int K);
+size_t wm_dense_i8_workspace_bytes(int M, int N, int K);
 int wm_dense_i8(const void *x, const int8_t *W, const float *wscale, const float *b, void *y,
                 const int64_t *offsets, int G, int M, int N, int K, int dtype, int relu,
                 void *workspace, size_t workspace_bytes, void *stream);

@@ -60,7 +60,7 @@ def test_c_abi_refusals():
     refused(L.wm_quantize_rows_i8(p, 4, (1 << 17) + 1, 0, p, p, 0), -2, b"32 bits")
     refused(L.wm_quantize_rows_i8(p, 4, 0, 0, p, p, 0), -1, b"bad sizes")
     refused(L.wm_dense_i8(p, p, p, 0, p, 0, 1, 4, 4, 4, 7, 0, p, 64, 0), -1, b"dtype")
-    assert L.wm_dense_i8_workspace_bytes(0, 4) == 0 and L.wm_dense_i8_workspace_bytes(3, 0) == 0
+    assert L.wm_dense_i8_workspace_bytes(0, 4, 4) == 0 and L.wm_dense_i8_workspace_bytes(3, 4, 0) == 0
     assert L.wm_dense_grouped_bwd_wb_workspace_bytes(0, 4, 4, 4, 0) == 0
     assert L.wm_dense_grouped_fwd_workspace_bytes(1, 16, 64, 8192, 0) == 0          # few rows
     assert L.wm_dense_grouped_fwd_workspace_bytes(1, 200, 64, 500, 0) == 0          # no long contraction
@@ -71,6 +71,7 @@ def test_c_abi_refusals():
 def test_product_sizes_do_not_overflow_the_workspace_query():
     from weather_model_amd import _lib
     L = _lib.lib()
-    assert L.wm_dense_i8_workspace_bytes(1, 8192) == 0 and L.wm_dense_i8_workspace_bytes(1, 8193) > 0
-    assert L.wm_dense_i8_workspace_bytes(1 << 24, 1 << 17) >= (1 << 24) * (1 << 17)
+    assert L.wm_dense_i8_workspace_bytes(1, 8, 8192) == 0 and L.wm_dense_i8_workspace_bytes(1, 8, 8193) > 0
+    assert L.wm_dense_i8_workspace_bytes(4, 8, 2048) == 0 and L.wm_dense_i8_workspace_bytes(4, 8000, 2048) > 0
+    assert L.wm_dense_i8_workspace_bytes(1 << 24, 8, 1 << 17) >= (1 << 24) * (1 << 17)
     assert L.wm_dense_grouped_bwd_wb_workspace_bytes(1, 1 << 30, 8, 8, 0) >= 8 * 8 * 4

@@ -602,7 +602,8 @@ def test_quantize_ties_extremes_and_bad_rows():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("M,N,K", [(1, 1, 1), (1, 8000, 640), (3, 37, 19), (16, 64, 128), (17, 130, 257), (128, 128, 64), (200, 301, 515),
                                    (130, 260, 2049), (48, 129, 33), (300, 50, 127), (600, 520, 272), (2048, 2048, 64), (2100, 2056, 272), (1, 40, 8192),
-                                   (1, 33, 8200), (1, 17, 4099), (20, 300, 640)])
+                                   (1, 33, 8200), (1, 17, 4099), (20, 300, 640), (2, 40, 8192), (4, 50, 8100), (5, 60, 2048), (16, 30, 2041), (9, 300, 1001),
+                                   (3, 5000, 999), (2, 20, 9000), (16, 4100, 2048)])
 def test_dense_i8(M, N, K, dtype):
     from weather_model_amd import ops
     x, b = rows(M, (M, K), dtype), rows(N, (N,), torch.float32)
@@ -616,6 +617,26 @@ def test_dense_i8(M, N, K, dtype):
         # the integer, two scalings and the sum are rounded once each in float32
         tol = 4 * U * (exact.abs() + (0 if bias is None else bias.double().abs())) + half_step(dtype) * ref.abs() + torch.finfo(dtype).tiny
         assert bool(((y.double() - ref).abs() <= tol * (1 + 2.0 ** -8)).all())
+
+
+@pytest.mark.parametrize("K", [70, 2100, 8191])
+@pytest.mark.parametrize("sizes", [[1, 0, 3], [0, 2, 0, 0, 1], [9, 0, 4, 0, 2], [40, 0, 0, 3, 20]])
+def test_dense_i8_few_rows_of_experts(sizes, K):
+    from weather_model_amd import ops
+    M, N, G = sum(sizes) + 1, 37, len(sizes)
+    x, b = rows(K, (M, K), torch.bfloat16), rows(2, (G, N), torch.float32)
+    q = torch.randint(-127, 128, (G, N, K), generator=torch.Generator().manual_seed(3)).to(torch.int8).cuda()
+    t = rows(4, (G, N), torch.float32).abs().cuda()
+    y = ops.dense_i8(x.cuda(), q, t, b.cuda(), offsets=offsets_of(sizes)).cpu().double()
+    xq, xs = codes_ref(x)
+    at = 0
+    for g, n in enumerate(sizes):
+        p = slice(at, at + n)
+        e = (xq[p] @ q[g].cpu().double().t()) * xs[p][:, None] * t[g].cpu().double()
+        ref = e + b[g].double()
+        assert bool(((y[p] - ref).abs() <= 4 * U * (e.abs() + b[g].double().abs()) + 2.0 ** -8 * ref.abs()).all()), g
+        at += n
+    assert not bool(y[at:].any())
 
 
 def test_dense_i8_grouped_extreme_codes_and_unaligned_weights():

@@ -87,7 +87,7 @@ SIGNATURES = {
     "wm_dense_grouped_bwd_wb": (c_int, [vp] * 5 + [c_sz, vp] + [c_int] * 5 + [vp]),
     "wm_dropout": (c_int, [vp, vp, vp, c_i64, c_int, c_f64, c_u64, c_u64, vp, vp]),
     "wm_quantize_rows_i8": (c_int, [vp, c_int, c_int, c_int, vp, vp, vp]),
-    "wm_dense_i8_workspace_bytes": (c_sz, [c_int, c_int]),
+    "wm_dense_i8_workspace_bytes": (c_sz, [c_int] * 3),
     "wm_dense_i8": (c_int, [vp] * 6 + [c_int] * 6 + [vp, c_sz, vp]),
     "wm_comm_unique_id": (c_int, [vp]),
     "wm_comm_init": (c_int, [c_int, c_int, vp]),

@@ -248,38 +248,53 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
     }
 }
 
-// One row: every workgroup makes the row's codes itself, in LDS, while its first weights are on their way -- the same codes as
-// quantize_rows_kernel's.  A launch of its own for one row took as long as the product (1 x 640 x 8000: 14.9 -> 9.3 us a call).
-constexpr int ONE_ROW_K = 8192;
+// A few short rows: every workgroup makes their codes itself, in LDS, while its first weights are on their way -- the same codes as
+// quantize_rows_kernel's, without its launch.  ONE: the whole workgroup takes the one row, K <= 8192; otherwise a wave takes a row.
+constexpr int OWN_ROWS = 8, OWN_BYTES = 8192, OWN_LDS = OWN_BYTES + OWN_ROWS * 144;
 struct Codes {                               // in LDS, zeros behind the row
     const int8_t *q;
     __device__ __forceinline__ u32x4 whole(int c) const { return *reinterpret_cast<const u32x4 *>(q + c); }
     __device__ __forceinline__ u32x4 part(int c, int) const { return whole(c); }
 };
 
-template <class E>
-__global__ __launch_bounds__(few::THREADS) void dense_i8_one_kernel(const E *__restrict__ x, const int8_t *__restrict__ W,
+template <class E, bool ONE>
+__global__ __launch_bounds__(few::THREADS) void dense_i8_own_kernel(const E *__restrict__ x, const int8_t *__restrict__ W,
                                                                     const float *__restrict__ wscale, const float *__restrict__ bias,
-                                                                    E *__restrict__ y, const long long *__restrict__ offsets, int G, int N, int K,
-                                                                    int relu)
+                                                                    E *__restrict__ y, const long long *__restrict__ offsets, int G, int M, int N,
+                                                                    int K, int relu)
 {
     __shared__ i32x4 part[few::WAVES][64];
-    __shared__ __attribute__((aligned(16))) int8_t codes[ONE_ROW_K];
-    __shared__ float s_shared;
-    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63;
-    if (g == G) return few_zeros(y, offsets, G, 1, N, n0);
-    int row0 = 0, rows = 1;
-    if (offsets) group_rows(offsets, G, 1, g, row0, rows);
+    __shared__ __attribute__((aligned(16))) int8_t codes[OWN_LDS];
+    __shared__ float scales[OWN_ROWS];
+    const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (g == G) return few_zeros(y, offsets, G, M, N, n0);
+    int row0 = 0, rows = M;
+    if (offsets) group_rows(offsets, G, M, g, row0, rows);
     if (rows == 0) return;
     few::Dot<I8, 4, true> dot;
     dot.begin(W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K, W + (long long)G * N * K, K);
-    quantize_row<E, few::THREADS, ONE_ROW_K / 8 / few::THREADS, few::THREADS>(x, K, codes, (K + 127) / 128 * 128, &s_shared);
+    const int ldq = (K + 127) / 128 * 128, stride = ldq + 16;        // 16: the rows' chunks in different banks
+    if constexpr (ONE) {
+        quantize_row<E, few::THREADS, OWN_BYTES / 8 / few::THREADS, few::THREADS>(x, K, codes, ldq, scales);
+    } else {
+        for (int r = wave; r < rows; r += few::WAVES)
+            quantize_row<E, 64, 2048 / 8 / 64, few::THREADS>(x + (long long)(row0 + r) * K, K, codes + r * stride, ldq, scales + r);
+    }
     __syncthreads();
-    const i32x4 acc = dot.multiply(Codes{codes});
-    few_out(acc, part, y, (lane & 15) == 0, s_shared, wscale + (long long)g * N, bias ? bias + (long long)g * N : nullptr, n0, N, relu);
+    const int r = min(lane & 15, rows - 1);
+    const i32x4 acc = dot.multiply(Codes{codes + r * stride});
+    few_out(acc, part, y + (long long)(row0 + r) * N, (lane & 15) < rows, scales[r], wscale + (long long)g * N,
+            bias ? bias + (long long)g * N : nullptr, n0, N, relu);
 }
 
-bool one_row(int M, int K) { return M == 1 && K <= ONE_ROW_K; }
+// Every 16 columns make the codes again: for rows whose codes take little more than the launch that this saves.  us a call | in a
+// captured graph, codes here / in a launch of their own: 1 x 640 x 8000 8.4 / 12.2 | 6.5 / 6.9, 4 x 1024 x 4096 8.3 / 12.3 | 5.7 / 6.5,
+// 8 x 1024 x 4096 9.0 / 12.6 | 8.4 / 6.8, 8 x 640 x 8000 10.5 / 12.7 | 10.2 / 7.8 (not taken).
+bool own_codes(int M, int N, int K)
+{
+    if (M == 1) return K <= OWN_BYTES;
+    return (M <= 4 ? K <= 2048 : M <= OWN_ROWS && K <= 1024) && (long long)M * K * ((N + 4095) / 4096) <= OWN_BYTES;
+}
 
 size_t padded(int K) { return wm_align_up((size_t)K, 128); }
 
@@ -333,10 +348,11 @@ template <class E>
 int dense(const void *x, const int8_t *W, const float *wscale, const float *b, void *y, const int64_t *offsets, int G, int M, int N, int K, int relu,
           void *workspace, hipStream_t st)
 {
-    if (one_row(M, K)) {
-        hipLaunchKernelGGL(dense_i8_one_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, (const E *)x, W, wscale, b,
-                           (E *)y, (const long long *)offsets, G, N, K, relu);
-        WM_LAUNCH_CHECK("dense_i8_one_kernel");
+    if (own_codes(M, N, K)) {
+        const auto kernel = M == 1 ? dense_i8_own_kernel<E, true> : dense_i8_own_kernel<E, false>;
+        hipLaunchKernelGGL(kernel, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, (const E *)x, W, wscale, b, (E *)y,
+                           (const long long *)offsets, G, M, N, K, relu);
+        WM_LAUNCH_CHECK("dense_i8_own_kernel");
         return WM_OK;
     }
     float *scale = (float *)workspace;
@@ -375,9 +391,9 @@ extern "C" int wm_quantize_rows_i8(const void *x, int M, int K, int dtype, int8_
     }
 }
 
-extern "C" size_t wm_dense_i8_workspace_bytes(int M, int K)
+extern "C" size_t wm_dense_i8_workspace_bytes(int M, int N, int K)
 {
-    if (M <= 0 || K <= 0 || one_row(M, K)) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || own_codes(M, N, K)) return 0;
     return wm_align_up((size_t)M * sizeof(float), 256) + (size_t)M * padded(K);
 }
 
@@ -390,7 +406,7 @@ extern "C" int wm_dense_i8(const void *x, const int8_t *W, const float *wscale, 
     WM_REQUIRE(N <= 1 << 20 && G <= 4096, WM_ERR_UNSUPPORTED, "wm_dense_i8: N=%d groups=%d is beyond 2^20 columns or 4096 groups", N, G);
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && wscale && y, WM_ERR_INVALID, "wm_dense_i8: null pointer");
-    const size_t need = wm_dense_i8_workspace_bytes(M, K);
+    const size_t need = wm_dense_i8_workspace_bytes(M, N, K);
     WM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), WM_ERR_WORKSPACE, "wm_dense_i8: workspace of %zu bytes needed, %zu given", need,
                workspace_bytes);
     WM_REQUIRE(((uintptr_t)workspace & 15) == 0, WM_ERR_INVALID, "wm_dense_i8: workspace must be 16-byte aligned");

@@ -980,7 +980,7 @@ def _same_device(t, name, like):
 def _out_any(out, shape, like, name, *inputs):
     """``out`` checked, or a new tensor; it may not share memory with any of ``inputs``."""
     if out is None:
-        return torch.empty(shape, device=like.device, dtype=like.dtype)
+        return like.new_empty(*shape)             # 0.6 us less than torch.empty
     if tuple(out.shape) != tuple(shape) or out.dtype != like.dtype or out.device != like.device or \
             not out.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {like.dtype} {tuple(shape)} tensor on {like.device}")
@@ -1000,7 +1000,7 @@ def _call(device, fn, *args):
     """``fn(*args, stream)`` on the current stream of ``device``, which is made current for the call."""
     index = device.index
     stream = torch._C._cuda_getCurrentRawStream(index)       # 0.1 us; the Stream object costs 2.7
-    if torch.cuda.current_device() == index:
+    if torch._C._cuda_getDevice() == index:
         _lib.check(fn(*args, stream))
     else:
         with torch.cuda.device(device):
@@ -1012,12 +1012,12 @@ def _workspace_bytes(name, *sizes):
     return getattr(_lib.lib(), name + "_workspace_bytes")(*sizes)
 
 
-def _workspace(device, name, *sizes):
+def _workspace(like, name, *sizes):
     """(tensor, address, bytes) of the workspace of one call"""
     need = _workspace_bytes(name, *sizes)
     if need == 0:
         return None, 0, 0
-    ws = torch.empty((need,), device=device, dtype=torch.uint8)
+    ws = like.new_empty(need, dtype=torch.uint8)
     return ws, ws.data_ptr(), need
 
 
@@ -1058,7 +1058,7 @@ def dense_grouped_forward(x, weight, offsets, bias=None, relu=False, out=None):
             raise ValueError(f"bias must be {(G, N)}, got {tuple(bias.shape)}")
     y = _out_any(out, (M, N), x, "out", x, weight, bias, offsets)
     dt = _DTYPES[x.dtype]
-    ws, at, size = _workspace(x.device, "wm_dense_grouped_fwd", G, M, N, K, dt)
+    ws, at, size = _workspace(x, "wm_dense_grouped_fwd", G, M, N, K, dt)
     _call(x.device, _lib.lib().wm_dense_grouped_fwd, x.data_ptr(), weight.data_ptr(),
           0 if bias is None else bias.data_ptr(), y.data_ptr(), at, size, offsets.data_ptr(), G, M, N, K,
           dt, 1 if relu else 0)
@@ -1083,15 +1083,15 @@ def dense_grouped_backward(x, weight, offsets, gy, mask_below=None, need_gx=True
             mask_below = _req_any(mask_below, "mask", x)
             if tuple(mask_below.shape) != (M, K):
                 raise ValueError(f"mask must be {(M, K)}, got {tuple(mask_below.shape)}")
-        gx = torch.empty((M, K), device=x.device, dtype=x.dtype)
-        ws, at, size = _workspace(x.device, "wm_dense_grouped_bwd_data", G, M, N, K, dt)
+        gx = x.new_empty(M, K)
+        ws, at, size = _workspace(x, "wm_dense_grouped_bwd_data", G, M, N, K, dt)
         _call(x.device, L.wm_dense_grouped_bwd_data, gy.data_ptr(), weight.data_ptr(),
               0 if mask_below is None else mask_below.data_ptr(), gx.data_ptr(), at, size,
               offsets.data_ptr(), G, M, N, K, dt)
     if need_gw:
         gw = _out_any(out_w, (G, N, K), x, "out_w", x, gy, offsets)
         gb = _out_any(out_b, (G, N), x, "out_b", x, gy, gw, offsets) if need_bias else None
-        ws, at, size = _workspace(x.device, "wm_dense_grouped_bwd_wb", G, M, N, K, dt)
+        ws, at, size = _workspace(x, "wm_dense_grouped_bwd_wb", G, M, N, K, dt)
         _call(x.device, L.wm_dense_grouped_bwd_wb, x.data_ptr(), gy.data_ptr(), gw.data_ptr(),
               0 if gb is None else gb.data_ptr(), at, size, offsets.data_ptr(), G, M, N, K, dt)
     return gx, gw, gb
@@ -1214,8 +1214,8 @@ def quantize_rows(x):
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"quantize_rows expects (M, K) with K > 0, got {tuple(x.shape)}")
     M, K = x.shape
-    q = torch.empty((M, K), device=x.device, dtype=torch.int8)
-    scale = torch.empty((M,), device=x.device, dtype=torch.float32)
+    q = x.new_empty(M, K, dtype=torch.int8)
+    scale = x.new_empty(M, dtype=torch.float32)
     _call(x.device, _lib.lib().wm_quantize_rows_i8, x.data_ptr(), M, K, _DTYPES[x.dtype], q.data_ptr(),
           scale.data_ptr())
     return q, scale
@@ -1244,7 +1244,7 @@ def dense_i8(x, weight, scale, bias=None, relu=False, offsets=None, out=None):
         if bias.shape != scale.shape:
             raise ValueError(f"bias must be {tuple(scale.shape)}, got {tuple(bias.shape)}")
     y = _out_any(out, (M, N), x, "out", x, weight, scale, bias, offsets)
-    ws, at, size = _workspace(x.device, "wm_dense_i8", M, K)
+    ws, at, size = _workspace(x, "wm_dense_i8", M, N, K)
     _call(x.device, _lib.lib().wm_dense_i8, x.data_ptr(), weight.data_ptr(), scale.data_ptr(),
           0 if bias is None else bias.data_ptr(), y.data_ptr(), 0 if offsets is None else offsets.data_ptr(),
           G, M, N, K, _DTYPES[x.dtype], 1 if relu else 0, at, size)
