@@ -2,7 +2,12 @@
 // memory goes to LDS without passing through registers (buffer loads to LDS), which leaves the registers to two sets
 // of MFMA operands, so that the reads of one multiplication run under the one before.
 //
-// A stage is 64 bytes of the contraction (32 or 64 values), one MFMA deep; LDS holds a ring of them.  An operand lies as
+// Bound by the matrix unit: 16384 rows, 16 experts of 2048 -> 4096 bf16, evenly spread, 266 us = 1030 TFLOP/s, where a library product of
+// 8192^3 makes 1360; a stage in the loop runs at 1430.  What is lost is the ring's fill and the way out of each tile (5 and 6 us of
+// 27 a round) and, with uneven experts (300 us), their last rows.
+//
+// A stage is 64 bytes of the contraction (32 or 64 values), one MFMA deep; LDS holds a ring of them (256 x 256: of 5, 160 KB; of 4
+// 308 us instead of 299).  An operand lies as
 //   DirectRows  [row][c], c along memory: 4 chunks of 16 bytes a row, two rows a line, placed by lds_at<4> of tile_gemm.h
 //   DirectCols  [c][row], rows along memory (16-bit types): read transposed (ds_read_b64_tr_b16: 16 lanes give the
 //               addresses of a 4 x 16 block, 8 bytes each, and get a row of 4 values each); blocks of 32 bytes are

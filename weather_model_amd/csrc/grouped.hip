@@ -5,6 +5,9 @@
 //             gW[g][n][k] = sum_{r of g} gy[r][n] x[r][k],   gb[g][n] = sum_{r of g} gy[r][n]
 // The number of rows of an expert is only known on the device, so a launch has as many workgroups as any
 // partition of M rows can need tiles, and each finds its tile from the offsets (tile_gemm.h).
+// Bound by the matrix unit where the experts have hundreds of rows (direct_gemm.h has the figures of 16 bits; float32, 8191 rows, 8
+// experts of 1024 -> 1024: forward 104 us = 165 TFLOP/s, gx 124, gW 115, where a library float32 product of 8192^3 makes 155 and
+// six bf16 products could make 227: splitting and LDS reads share the issue slots), by reading the weights where they have a few.
 #include "direct_gemm.h"
 #include "few_rows.h"
 
@@ -419,6 +422,8 @@ int rows_parts(const void *x, const void *W, const void *bias, const void *mask,
     return WM_OK;
 }
 
+// 16-byte rows go from memory to LDS, others through registers: 16384 rows, 8 experts of 1024 -> 1024 bf16 in tiles of 128 x 128, us,
+// directly | through registers: forward 44 | 42, backward 43 | 79, gradients of weights 53 | 66.
 template <class T, bool BACKWARD>
 int rows_typed(const void *x, const void *W, const void *bias, const void *mask, void *out, void *workspace, const int64_t *offsets, int G, int M,
                int NO, int C, int relu, hipStream_t st)

@@ -799,7 +799,8 @@ inline long long row_tiles_most(int G, int M, int BM)
 }
 
 // Workgroups go round the eight XCDs in turn: logical tiles are dealt out so that an XCD works on a run of
-// them, and a run keeps to `band` row tiles and walks the columns, so that its operands stay in its L2.
+// them, and a run keeps to `band` row tiles and walks the columns, so that its operands stay in its L2 (us, row after row | so: 16384
+// rows, 16 experts, gradients 4096 -> 2048 bf16 312 | 306; 2999 rows, 33 experts, gradients 333 -> 515 float16 21.7 | 19.4).
 __device__ __forceinline__ void place_of_tile(int t, int row_tiles, int col_tiles, int band, int &rt, int &ct)
 {
     const int total = row_tiles * col_tiles, per = total / 8, extra = total % 8, xcd = t % 8;
@@ -811,8 +812,10 @@ __device__ __forceinline__ void place_of_tile(int t, int row_tiles, int col_tile
 
 // The work of a workgroup: a tile of S, or part of one.  `slots` workgroups run at once; the tiles that are left when they
 // have been filled a whole number of times are cut into tiles of Quarter or of Half where those find room at once, so that a
-// launch ends after a part of a tile's time instead of a whole one.  Halves only where a tile has a CU to itself: two tiles to a
-// CU leave one each for half of the slots, which is as fast (45001 x 216 x 432 float32 71 us whole, 76 in halves).
+// launch ends after a part of a tile's time instead of a whole one (us, whole | cut: 8191 rows, 8 experts of 1024 -> 1024 float32 130 | 104,
+// their gradients 159 | 124; 16384 rows, 16 experts, gradients 4096 -> 2048 bf16 344 | 306; int8 777 x 1283 -> 1001 23 | 15).  Halves
+// only where a tile has a CU to itself: two tiles to a CU leave one each for half of the slots, which is as fast (45001 x 216 x 432
+// float32 71 us whole, 76 in halves).
 template <class S, class Half, class Quarter> struct Cut {
     typedef typename std::conditional<S::ALONE, Half, S>::type H;
     static_assert(S::THREADS == H::THREADS && H::LDS <= S::LDS && (!S::ALONE || S::BM * S::BN == 2 * H::BM * H::BN), "one launch");
@@ -836,7 +839,8 @@ template <class S, class Half, class Quarter> struct Cut {
 
 // The order in which the groups' products over rows are taken up: the longest first, so that a launch does not end on one of
 // them; where two workgroups share a CU from the start (`first` groups are begun on empty CUs), the shortest are put beside the
-// longest.  More than 62 groups are taken as they come.  Gives the group and its rows.
+// longest (38115 rows in 16 uneven experts, us, in order | so: 512 x 512 bf16 57 | 54, float32 170 | 166).  More than 62 groups are
+// taken as they come.  Gives the group and its rows.
 __device__ __forceinline__ void group_in_turn(const long long *offsets, int G, int M, int turn, int first, int &g, int &row0, int &rows)
 {
     if (G > 62) {
