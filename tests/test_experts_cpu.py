@@ -75,3 +75,15 @@ def test_product_sizes_do_not_overflow_the_workspace_query():
     assert L.wm_dense_i8_workspace_bytes(4, 8, 2048) == 0 and L.wm_dense_i8_workspace_bytes(4, 8000, 2048) > 0
     assert L.wm_dense_i8_workspace_bytes(1 << 24, 8, 1 << 17) >= (1 << 24) * (1 << 17)
     assert L.wm_dense_grouped_bwd_wb_workspace_bytes(1, 1 << 30, 8, 8, 0) >= 8 * 8 * 4
+
+
+def test_group_offsets():
+    from weather_model_amd import ops
+    for dtype in (torch.int32, torch.int64):
+        off = ops.group_offsets(torch.tensor([3, 0, 5, 0], dtype=dtype))
+        assert off.dtype == torch.int64 and off.tolist() == [0, 3, 3, 8, 8]
+    assert ops.group_offsets(torch.zeros((0,), dtype=torch.int64)).tolist() == [0]
+    with pytest.raises(TypeError, match="int32 or int64"):
+        ops.group_offsets(torch.ones(3))
+    with pytest.raises(ValueError, match="counts must be"):
+        ops.group_offsets(torch.ones((2, 2), dtype=torch.int64))

@@ -284,7 +284,7 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const floa
 // Six waves a SIMD with four loads each of weights in flight: 48 rows over 12 of 16 experts of 2048 x 2048 bf16 in 22 us (4.6 TB/s);
 // 28 with eight loads and four waves.
 template <class T>
-__global__ __launch_bounds__(few::THREADS, 6) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
+__global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
                                                                    const typename T::elem *__restrict__ bias, typename T::elem *__restrict__ y,
                                                                    const long long *__restrict__ offsets, int G, int M, int N, int K, int relu)
 {

@@ -295,37 +295,26 @@ template <class T, int ROWS, int THREADS> struct Strided {
     }
     __device__ __forceinline__ void load_guarded(Regs &reg, int c0) const
     {
-        if (!slow) {                         // the last c again for those behind it
+        // the last c again for those behind it, and the last row
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int c = c0 + q * 8 + e;
-                const E *p = base + (long long)min(c, count - 1) * ld + r0;
-                if constexpr (WORDS == 1) {
-                    reg.v[e][0] = *reinterpret_cast<const u32u *>(p);
-                } else {
-                    const words v = *reinterpret_cast<const words *>(p);
+        for (int e = 0; e < 8; ++e) {
+            const E *p = base + (long long)min(c0 + q * 8 + e, count - 1) * ld;
+            if (slow) {
 #pragma unroll
-                    for (int w = 0; w < WORDS; ++w) reg.v[e][w] = v[w];
-                }
+                for (int w = 0; w < WORDS; ++w)
+                    if constexpr (PER_WORD == 1) reg.v[e][w] = __builtin_bit_cast(uint32_t, p[min(r0 + w, most - 1)]);
+                    else
+                        reg.v[e][w] = (uint32_t)__builtin_bit_cast(uint16_t, p[min(r0 + 2 * w, most - 1)]) |
+                                      (uint32_t)__builtin_bit_cast(uint16_t, p[min(r0 + 2 * w + 1, most - 1)]) << 16;
+            } else if constexpr (WORDS == 1) {
+                reg.v[e][0] = *reinterpret_cast<const u32u *>(p + r0);
+            } else {
+                const words v = *reinterpret_cast<const words *>(p + r0);
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w) reg.v[e][w] = v[w];
             }
-            trim(reg, c0);
-            return;
         }
-        const E *at = base + (long long)c0 * ld;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int w = 0; w < WORDS; ++w) {
-                uint32_t v = 0;
-#pragma unroll
-                for (int i = 0; i < PER_WORD; ++i)
-                    if (c0 + q * 8 + e < count && r0 + w * PER_WORD + i < most) {
-                        const E *p = at + (uint32_t)((q * 8 + e) * (int)ld + r0 + w * PER_WORD + i);
-                        if constexpr (PER_WORD == 1) v = __builtin_bit_cast(uint32_t, *p);
-                        else v |= (uint32_t)__builtin_bit_cast(uint16_t, *p) << (16 * i);
-                    }
-                reg.v[e][w] = v;
-            }
+        trim(reg, c0);
     }
     // adds what the registers hold to the sums of this thread's rows over c
     __device__ __forceinline__ void add_up(const Regs &reg)

@@ -1039,6 +1039,10 @@ def _group_offsets(offsets, groups, x):
 
 def group_offsets(counts):
     """Row offsets (G + 1,) int64 from the number of rows of each group (G,), on their device."""
+    if not isinstance(counts, torch.Tensor) or counts.dtype not in (torch.int32, torch.int64):
+        raise TypeError("counts must be an int32 or int64 tensor")
+    if counts.dim() != 1:
+        raise ValueError(f"counts must be (G,), got {tuple(counts.shape)}")
     out = torch.zeros((counts.numel() + 1,), device=counts.device, dtype=torch.int64)
     torch.cumsum(counts, 0, out=out[1:])
     return out
