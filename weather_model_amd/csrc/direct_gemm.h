@@ -35,7 +35,7 @@ __device__ __forceinline__ u32x4 descriptor(const char *p, long long bytes)
 // 16 bytes a lane to LDS at `to` + 16 lane.  No register is written; completion counts in vmcnt.
 __device__ __forceinline__ void load_to_lds(u32x4 desc, uint32_t voffset, uint32_t soffset, uint32_t to)
 {
-    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(desc), "s"(soffset), "s"(to));
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds" ::"v"(voffset), "s"(desc), "s"(soffset), "s"(to) : "m0");
 }
 template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
