@@ -175,6 +175,70 @@ def test_grouped_offsets_of_any_value_are_safe():
         close(y, ref, S, 8, off)
 
 
+def test_offsets_of_any_value_are_safe_in_every_path():
+    """Few and many rows, chunks of rows, parts of a contraction, 8 bits: offsets outside 0 .. M and falling ones."""
+    from weather_model_amd import ops
+    for M, N, K in ((3, 20, 40), (60, 24, 72), (200, 40, 1100), (3000, 24, 40)):
+        x, w, gy = rows(1, (M, K), torch.float32), rows(2, (4, N, K), torch.float32, K ** -0.5), rows(3, (M, N), torch.float32)
+        raw = [-5, M - 2, 1, M + 99, 7]
+        sizes = [M - 2, 0, 2, 0]
+        off = torch.tensor(raw, device="cuda")
+        y = ops.dense_grouped_forward(x.cuda(), w.cuda(), off)
+        ref, S = grouped_ref(x, w, None, sizes, 0, False)
+        close(y, ref, S, K, M)
+        gx, gw, gb = ops.dense_grouped_backward(x.cuda(), w.cuda(), off, gy.cuda())
+        rx, Sx = grouped_ref(gy, w.transpose(1, 2), None, sizes, 0, False)
+        close(gx, rx, Sx, N, M)
+        a, c = gy[:M - 2].double(), x[:M - 2].double()
+        close(gw[0], a.t() @ c, a.abs().t() @ c.abs(), M, M)
+        close(gb[0], a.sum(0), a.abs().sum(0), M, M, norm=False)
+        assert not bool(gw[1].any()) and not bool(gw[3].any()) and not bool(gb[1].any())
+        q, t = ops.quantize_rows(w.reshape(-1, K).cuda())
+        y8 = ops.dense_i8(x.cuda(), q.view(4, N, K), t.view(4, N), offsets=off).cpu().double()
+        xq, xs = codes_ref(x)
+        for g, p in ((0, slice(0, M - 2)), (2, slice(M - 2, M))):
+            e = (xq[p] @ q.view(4, N, K)[g].cpu().double().t()) * xs[p][:, None] * t.view(4, N)[g].cpu().double()
+            assert bool(((y8[p] - e).abs() <= 5 * U * e.abs()).all()), (M, g)
+
+
+def test_as_many_experts_as_there_may_be():
+    from weather_model_amd import ops
+    G, N, K = 4096, 12, 20
+    sizes = torch.randint(0, 4, (G,), generator=torch.Generator().manual_seed(1)).tolist()
+    sizes[77] = 600
+    M = sum(sizes)
+    x, w, gy = rows(1, (M, K), torch.bfloat16), rows(2, (G, N, K), torch.bfloat16, K ** -0.5), rows(3, (M, N), torch.bfloat16)
+    off = offsets_of(sizes)
+    y = ops.dense_grouped_forward(x.cuda(), w.cuda(), off)
+    ref, S = grouped_ref(x, w, None, sizes, 0, False)
+    close(y, ref, S, K, "y")
+    gx, gw, gb = ops.dense_grouped_backward(x.cuda(), w.cuda(), off, gy.cuda())
+    rx, Sx = grouped_ref(gy, w.transpose(1, 2), None, sizes, 0, False)
+    close(gx, rx, Sx, N, "gx")
+    at = np.cumsum([0] + sizes)
+    for g in (0, 1, 63, 64, 77, 78, 2047, 4094, 4095):
+        a, c = gy[at[g]:at[g + 1]].double(), x[at[g]:at[g + 1]].double()
+        close(gw[g], a.t() @ c, a.abs().t() @ c.abs(), sizes[g], g)
+        close(gb[g], a.sum(0), a.abs().sum(0), sizes[g], g, norm=False)
+
+
+def test_strided_inputs_are_taken_as_their_values():
+    from weather_model_amd import ops
+    sizes, N, K = [40, 61], 24, 36
+    off = offsets_of(sizes)
+    x, w, gy = (rows(k, s, torch.bfloat16).cuda() for k, s in ((1, (101, K)), (2, (2, N, K)), (3, (101, N))))
+    xs, ws, gs = x.t().contiguous().t(), w.transpose(0, 2).contiguous().transpose(0, 2), torch.cat([gy, gy], 1)[:, N:]
+    assert not xs.is_contiguous() and not ws.is_contiguous() and not gs.is_contiguous()
+    assert torch.equal(ops.dense_grouped_forward(x, w, off), ops.dense_grouped_forward(xs, ws, off))
+    for a, b in zip(ops.dense_grouped_backward(x, w, off, gy, mask_below=x), ops.dense_grouped_backward(xs, ws, off, gs, mask_below=xs)):
+        assert torch.equal(a, b)
+    assert torch.equal(ops.dropout_forward(x, 0.4, 3, residual=x), ops.dropout_forward(xs, 0.4, 3, residual=xs))
+    row = x[:1].expand(50, K)
+    assert torch.equal(ops.quantize_rows(row)[0], ops.quantize_rows(row.contiguous())[0])
+    bias = torch.ones((1, 1), dtype=torch.bfloat16, device="cuda").expand(2, N)
+    assert torch.equal(ops.dense_grouped_forward(x, w, off, bias), ops.dense_grouped_forward(x, w, off, bias.contiguous()))
+
+
 @pytest.mark.parametrize("more", [0, 230])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_grouped_infinities_and_nan_stay_in_their_rows(dtype, more):
