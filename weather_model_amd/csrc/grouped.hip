@@ -281,8 +281,8 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const floa
 
 // ---- few rows: y (M, N) for groups of a handful of rows.  One read of the weights is the cost, so a workgroup takes 16
 // outputs of one expert, its waves share the contraction, and the MFMA operands come straight from memory.
-// Six waves a SIMD with four loads each of weights in flight: 48 rows over 12 of 16 experts of 2048 x 2048 bf16 in 22 us (4.6 TB/s);
-// 28 with eight loads and four waves.
+// Six waves a SIMD with four loads each of weights in flight (five for float32, whose operands are wider): 48 rows over 8 experts of
+// 2048 x 2048 bf16 in 14.5 us (4.6 TB/s); over 16 of them 28 us with eight loads and four waves, 22 so.
 template <class T>
 __global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
                                                                    const typename T::elem *__restrict__ bias, typename T::elem *__restrict__ y,
@@ -443,9 +443,16 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows: it is for rows that are few even where one expert has
-// them all.  us, few rows | tiles, 1024 -> 1024: 1 expert bf16 32 rows 8.5 | 8.6, 64 rows 11 | 9.0, float32 32 rows 11 | 14, 64 rows
-// 21 | 14; 16 experts, 64 rows, bf16 9.0 | 12, float32 18 | 20; 128 rows, all in one of them, 20 | 9.1, 38 | 24.
-bool few_rows(int G, int M) { return M <= 32 || (M <= 64 && G >= 4); }
+// them all, and for weights that do not fill the CUs with tiles, which read them faster.  us, few rows | tiles: bf16 1 expert, 8
+// rows of 640 -> 8000 4.5 | 5.4, of 4096 -> 2048 12 | 9.3 (tiles in parts), of 3000 -> 1024 6.5 | 8.3, 32 rows of 4096 -> 4096 24 | 11; 8
+// experts, 48 rows of 2048 -> 2048 15 | 19, 16 experts 33 | 23; float32 1 expert, 8 rows of 640 -> 8000 6.7 | 13, 16 rows of 4096 ->
+// 4096 26 | 32, 32 rows 47 | 32, 16 experts, 40 rows of 2048 -> 2048 56 | 61.
+bool few_rows(int G, int M, int N, int K, int dtype)
+{
+    if (M > 16 && (M > 64 || G < 4)) return false;
+    if (dtype == WM_F32 || K % 8 != 0) return true;              // rows of other than 16 bytes take the slower way into LDS
+    return (long long)(G < M ? G : M) * N < 128 * 256 && rows_depth(G, M, N, K, dtype) == 0;
+}
 
 template <class T> int few_launch(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
                                   int relu, hipStream_t st)
@@ -534,7 +541,7 @@ int weights_typed(const void *x, const void *gy, void *gW, void *gb, void *works
 
 extern "C" size_t wm_dense_grouped_fwd_workspace_bytes(int G, int M, int N, int K, int dtype)
 {
-    return M > 0 && N > 0 && K > 0 && G > 0 && !few_rows(G, M) ? rows_bytes(G, M, N, K, dtype) : 0;
+    return M > 0 && N > 0 && K > 0 && G > 0 && !few_rows(G, M, N, K, dtype) ? rows_bytes(G, M, N, K, dtype) : 0;
 }
 
 extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b, void *y, void *workspace, size_t workspace_bytes,
@@ -544,7 +551,7 @@ extern "C" int wm_dense_grouped_fwd(const void *x, const void *W, const void *b,
     if (M == 0) return WM_OK;
     WM_REQUIRE(x && W && y && offsets, WM_ERR_INVALID, "wm_dense_grouped_fwd: null pointer");
     if (int rc = workspace_ok("wm_dense_grouped_fwd", wm_dense_grouped_fwd_workspace_bytes(G, M, N, K, dtype), workspace, workspace_bytes)) return rc;
-    if (few_rows(G, M)) {
+    if (few_rows(G, M, N, K, dtype)) {
         hipStream_t st = (hipStream_t)stream;
         switch (dtype) {
         case WM_F32: return few_launch<F32>(x, W, b, y, offsets, G, M, N, K, relu, st);

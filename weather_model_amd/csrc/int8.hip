@@ -344,6 +344,14 @@ int dense_tiles(const int8_t *q, long long ldq, const float *scale, const int8_t
     return WM_OK;
 }
 
+// As in grouped.hip.  us, few rows | tiles: 1 expert, 16 rows of 4096 -> 4096 10 | 15, 32 rows of 8192 -> 8192 36 | 24; 4 experts, 40 rows of
+// 4096 -> 2048 13 | 20, 16 experts of 2048 -> 2048 22 | 18.
+bool few_rows(int G, int M, int N, int K)
+{
+    if (M > 16 && (M > 64 || G < 4)) return false;
+    return G == 1 || K % 16 != 0 || (long long)(G < M ? G : M) * N < 128 * 256;
+}
+
 template <class E>
 int dense(const void *x, const int8_t *W, const float *wscale, const float *b, void *y, const int64_t *offsets, int G, int M, int N, int K, int relu,
           void *workspace, hipStream_t st)
@@ -359,7 +367,7 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     int8_t *q = (int8_t *)workspace + wm_align_up((size_t)M * sizeof(float), 256);
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
-    if (M <= 32 || (M <= 64 && G >= 4)) {        // as in grouped.hip (1024 -> 1024, 16 experts, 128 rows 15 us either way, 256 rows 16 | 15)
+    if (few_rows(G, M, N, K)) {
         hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, q, ldq, scale, W, wscale, b,
                            (E *)y, (const long long *)offsets, G, M, N, K, relu);
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
