@@ -62,7 +62,7 @@ def test_c_abi_refusals():
     refused(L.wm_dense_i8(p, p, p, 0, p, 0, 1, 4, 4, 4, 7, 0, p, 64, 0), -1, b"dtype")
     assert L.wm_dense_i8_workspace_bytes(0, 4, 4) == 0 and L.wm_dense_i8_workspace_bytes(3, 4, 0) == 0
     assert L.wm_dense_grouped_bwd_wb_workspace_bytes(0, 4, 4, 4, 0) == 0
-    assert L.wm_dense_grouped_fwd_workspace_bytes(1, 16, 64, 8192, 0) == 0          # few rows
+    assert L.wm_dense_grouped_fwd_workspace_bytes(1, 16, 8192, 8192, 0) == 0          # few rows
     assert L.wm_dense_grouped_fwd_workspace_bytes(1, 200, 64, 500, 0) == 0          # no long contraction
     assert L.wm_dense_grouped_fwd_workspace_bytes(1, 200, 64, 8192, 0) >= 200 * 64 * 4 * 2
     assert L.wm_dense_grouped_bwd_data_workspace_bytes(1, 16, 8192, 64, 2) >= 16 * 64 * 4 * 2

@@ -281,8 +281,8 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const floa
 
 // ---- few rows: y (M, N) for groups of a handful of rows.  One read of the weights is the cost, so a workgroup takes 16
 // outputs of one expert, its waves share the contraction, and the MFMA operands come straight from memory.
-// Six waves a SIMD with four loads each of weights in flight (five for float32, whose operands are wider): 48 rows over 8 experts of
-// 2048 x 2048 bf16 in 14.5 us (4.6 TB/s); over 16 of them 28 us with eight loads and four waves, 22 so.
+// Six waves a SIMD with four loads each of weights in flight (five for float32, whose operands are wider): 48 rows over 12 of 16
+// experts of 2048 x 2048 bf16 in 22 us (4.5 TB/s from HBM); 28 with eight loads and four waves.
 template <class T>
 __global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
                                                                    const typename T::elem *__restrict__ bias, typename T::elem *__restrict__ y,
@@ -443,15 +443,16 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows: it is for rows that are few even where one expert has
-// them all, and for weights that do not fill the CUs with tiles, which read them faster.  us, few rows | tiles: bf16 1 expert, 8
-// rows of 640 -> 8000 4.5 | 5.4, of 4096 -> 2048 12 | 9.3 (tiles in parts), of 3000 -> 1024 6.5 | 8.3, 32 rows of 4096 -> 4096 24 | 11; 8
-// experts, 48 rows of 2048 -> 2048 15 | 19, 16 experts 33 | 23; float32 1 expert, 8 rows of 640 -> 8000 6.7 | 13, 16 rows of 4096 ->
-// 4096 26 | 32, 32 rows 47 | 32, 16 experts, 40 rows of 2048 -> 2048 56 | 61.
+// them all, and not for long contractions that tiles take in parts: in 16 bits, and in float32 where its workgroups of 16 columns
+// would not fill the CUs.  us, few rows | tiles, weights from HBM: bf16 1 expert, 8 rows of 640 -> 8000 6.3 | 7.6, of 4096 -> 4096 17 | 13, 40 rows
+// 38 | 14; 8 experts, 40 rows of 2048 -> 2048 18 | 27, 16 experts 37 | 35, 16 experts, 8 rows of 4096 -> 1024 28 | 19; float32 1 expert, 8 rows
+// of 640 -> 8000 9.7 | 14, of 4096 -> 2048 30 | 22, of 4096 -> 4096 31 | 34, 40 rows 75 | 35; 16 experts of 1024 -> 4096 67 | 93.
 bool few_rows(int G, int M, int N, int K, int dtype)
 {
     if (M > 16 && (M > 64 || G < 4)) return false;
-    if (dtype == WM_F32 || K % 8 != 0) return true;              // rows of other than 16 bytes take the slower way into LDS
-    return (long long)(G < M ? G : M) * N < 128 * 256 && rows_depth(G, M, N, K, dtype) == 0;
+    const long long columns = (long long)(G < M ? G : M) * N;
+    if (dtype == WM_F32 ? columns >= 16 * 256 : K % 8 != 0) return true;       // rows of other than 16 bytes take the slower way into LDS
+    return rows_depth(G, M, N, K, dtype) == 0;
 }
 
 template <class T> int few_launch(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,

@@ -344,8 +344,8 @@ int dense_tiles(const int8_t *q, long long ldq, const float *scale, const int8_t
     return WM_OK;
 }
 
-// As in grouped.hip.  us, few rows | tiles: 1 expert, 16 rows of 4096 -> 4096 10 | 15, 32 rows of 8192 -> 8192 36 | 24; 4 experts, 40 rows of
-// 4096 -> 2048 13 | 20, 16 experts of 2048 -> 2048 22 | 18.
+// As in grouped.hip, but for experts that fill the card with tiles.  us, few rows | tiles, weights from HBM: 1 expert, 16 rows of 4096 -> 4096
+// 12 | 20, 40 rows of 8192 -> 8192 50 | 34; 8 experts, 40 rows of 2048 -> 2048 14 | 19, 16 experts 23 | 21, of 1024 -> 4096 39 | 22.
 bool few_rows(int G, int M, int N, int K)
 {
     if (M > 16 && (M > 64 || G < 4)) return false;
