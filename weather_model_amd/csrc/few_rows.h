@@ -12,8 +12,6 @@ namespace few {
 
 using namespace tile;
 
-constexpr int WAVES = 4, THREADS = 64 * WAVES;
-
 template <class T> __device__ __forceinline__ typename T::acc piece(u32x4 a, u32x4 b, typename T::acc c)
 {
     if constexpr (std::is_same<T, F32>::value) {     // float32 on its own MFMA: the weights' bytes are the bound here
@@ -29,9 +27,9 @@ template <class T> __device__ __forceinline__ typename T::acc piece(u32x4 a, u32
 // This wave's share of the products of matrix row w (i = lane & 15: four consecutive rows of the result per lane) with a row of x;
 // rows that do not exist are given as any that do.  x gives the pieces of its row: whole(c) from value c on, part(c, left) of which
 // only `left` values count.
-// UNROLL: rounds whose loads go out together.  EARLY: begin() is called long before multiply(), and the first loads of the weights
+// UNROLL: rounds whose loads go out together.  WAVES: of the workgroup.  EARLY: begin() is called long before multiply(), and the first loads of the weights
 // go out there.
-template <class T, int UNROLL, bool EARLY = false> struct Dot {
+template <class T, int UNROLL, int WAVES, bool EARLY = false> struct Dot {
     typedef typename T::elem E;
     static constexpr int ROUND = 128 / sizeof(E), PIECE = 16 / sizeof(E);
     typedef u32x4 Batch[UNROLL][2];

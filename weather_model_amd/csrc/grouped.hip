@@ -283,13 +283,15 @@ __global__ __launch_bounds__(THREADS) void grouped_weights_sum_kernel(const floa
 // outputs of one expert, its waves share the contraction, and the MFMA operands come straight from memory.
 // Six waves a SIMD with four loads each of weights in flight (five for float32, whose operands are wider): 48 rows over 12 of 16
 // experts of 2048 x 2048 bf16 in 22 us (4.5 TB/s from HBM); 28 with eight loads and four waves.
-template <class T>
-__global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
+// Four waves in 16 bits, eight in float32 (us, four | eight, 8 rows of 8192 -> 8192 float32 85 | 68, of 2048 -> 8192 24 | 19; bf16 13.2 | 11.7,
+// but 48 rows over the 12 experts 23 | 27).
+template <class T, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, T::PLANES == 3 ? 5 : 6) void grouped_few_kernel(const typename T::elem *__restrict__ x, const typename T::elem *__restrict__ W,
                                                                    const typename T::elem *__restrict__ bias, typename T::elem *__restrict__ y,
                                                                    const long long *__restrict__ offsets, int G, int M, int N, int K, int relu)
 {
     typedef typename T::elem E;
-    __shared__ f32x4 part[few::WAVES][64];
+    __shared__ f32x4 part[WAVES][64];
     const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int row0, rows;
     if (g == G) {                                    // rows of no expert: zeros
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_
         group_rows(offsets, G, M, G - 1, end, rows);
         end += rows;
         const int cols = min(16, N - n0);
-        for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += few::THREADS) {
+        for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += 64 * WAVES) {
             const int r = e / cols;
             y[(long long)(r < row0 ? r : r - row0 + end) * N + n0 + e % cols] = (E)0.0f;
         }
@@ -308,7 +310,7 @@ __global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_
     const E *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
     for (int r0 = 0; r0 < rows; r0 += 16) {
         const int r = min(r0 + (lane & 15), rows - 1);
-        few::Dot<T, 2> dot;
+        few::Dot<T, 2, WAVES> dot;
         dot.begin(wrow, W + (long long)G * N * K, K);
         const f32x4 acc = dot.multiply(few::RowOf<T>{x + (long long)(row0 + r) * K, x + (long long)M * K});
         if (wave > 0) part[wave][lane] = acc;
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(few::THREADS, T::PLANES == 3 ? 5 : 6) void grouped_
         if (wave == 0) {
             f32x4 v = acc;
 #pragma unroll
-            for (int w = 1; w < few::WAVES; ++w) v += part[w][lane];
+            for (int w = 1; w < WAVES; ++w) v += part[w][lane];
             const int n = n0 + 4 * (lane >> 4), have = min(4, N - n);
             if (r0 + (lane & 15) < rows && have > 0) {
                 E *at = y + (long long)(row0 + r) * N + n;
@@ -443,23 +445,23 @@ int rows_typed(const void *x, const void *W, const void *bias, const void *mask,
 }
 
 // The few-rows kernel reads an expert's weights once for every 16 of its rows: it is for rows that are few even where one expert has
-// them all, and not for long contractions that tiles take in parts: in 16 bits, and in float32 where its workgroups of 16 columns
-// would not fill the CUs.  us, few rows | tiles, weights from HBM: bf16 1 expert, 8 rows of 640 -> 8000 6.3 | 7.6, of 4096 -> 4096 17 | 13, 40 rows
-// 38 | 14; 8 experts, 40 rows of 2048 -> 2048 18 | 27, 16 experts 37 | 35, 16 experts, 8 rows of 4096 -> 1024 28 | 19; float32 1 expert, 8 rows
-// of 640 -> 8000 9.7 | 14, of 4096 -> 2048 30 | 22, of 4096 -> 4096 31 | 34, 40 rows 75 | 35; 16 experts of 1024 -> 4096 67 | 93.
+// them all, and in 16 bits not for long contractions, which tiles take in parts.  us, few rows | tiles, weights from HBM: bf16 1 expert, 8
+// rows of 640 -> 8000 6.3 | 7.6, of 4096 -> 4096 17 | 13, 40 rows 38 | 14; 8 experts, 40 rows of 2048 -> 2048 18 | 27, 16 experts 37 | 35, 16
+// experts, 8 rows of 4096 -> 1024 28 | 19; float32 1 expert, 8 rows of 640 -> 8000 8.7 | 14, of 4096 -> 4096 24 | 34, 16 experts, 40
+// rows of 2048 -> 2048 68 | 71.
 bool few_rows(int G, int M, int N, int K, int dtype)
 {
     if (M > 16 && (M > 64 || G < 4)) return false;
-    const long long columns = (long long)(G < M ? G : M) * N;
-    if (dtype == WM_F32 ? columns >= 16 * 256 : K % 8 != 0) return true;       // rows of other than 16 bytes take the slower way into LDS
-    return rows_depth(G, M, N, K, dtype) == 0;
+    // rows of other than 16 bytes take the slower way into LDS
+    return dtype == WM_F32 || K % 8 != 0 || rows_depth(G, M, N, K, dtype) == 0;
 }
 
 template <class T> int few_launch(const void *x, const void *W, const void *b, void *y, const int64_t *offsets, int G, int M, int N, int K,
                                   int relu, hipStream_t st)
 {
     typedef typename T::elem E;
-    hipLaunchKernelGGL(grouped_few_kernel<T>, dim3((N + 15) / 16, G + 1), dim3(few::THREADS), 0, st, (const E *)x, (const E *)W, (const E *)b,
+    constexpr int WAVES = T::PLANES == 3 ? 8 : 4;
+    hipLaunchKernelGGL((grouped_few_kernel<T, WAVES>), dim3((N + 15) / 16, G + 1), dim3(64 * WAVES), 0, st, (const E *)x, (const E *)W, (const E *)b,
                        (E *)y, (const long long *)offsets, G, M, N, K, relu);
     WM_LAUNCH_CHECK("grouped_few_kernel");
     return WM_OK;

@@ -185,8 +185,8 @@ __global__ __launch_bounds__(S::THREADS, 2) void dense_i8_kernel(const int8_t *_
 
 // ---- few rows: one read of the weights (few_rows.h)
 // joins the waves' sums; wave 0 scales and writes columns n0 .. n0 + 15 of row y (lane & 15), if `there`
-template <class E>
-__device__ __forceinline__ void few_out(i32x4 acc, i32x4 (&part)[few::WAVES][64], E *y, bool there, float qs, const float *wscale, const float *bias,
+template <int WAVES, class E>
+__device__ __forceinline__ void few_out(i32x4 acc, i32x4 (&part)[WAVES][64], E *y, bool there, float qs, const float *wscale, const float *bias,
                                         int n0, int N, int relu)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -194,7 +194,7 @@ __device__ __forceinline__ void few_out(i32x4 acc, i32x4 (&part)[few::WAVES][64]
     __syncthreads();
     if (wave == 0) {
 #pragma unroll
-        for (int w = 1; w < few::WAVES; ++w) acc += part[w][lane];
+        for (int w = 1; w < WAVES; ++w) acc += part[w][lane];
         const int n = n0 + 4 * (lane >> 4), have = min(4, N - n);
         if (there && have > 0) {
             f32x4 v;
@@ -220,19 +220,20 @@ template <class E> __device__ __forceinline__ void few_zeros(E *y, const long lo
     group_rows(offsets, G, M, G - 1, end, rows);
     end += rows;
     const int cols = min(16, N - n0);
-    for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += few::THREADS) {
+    for (int e = threadIdx.x; e < (row0 + M - end) * cols; e += blockDim.x) {
         const int r = e / cols;
         y[(long long)(r < row0 ? r : r - row0 + end) * N + n0 + e % cols] = (E)0.0f;
     }
 }
 
+constexpr int FEW_WAVES = 4;
 template <class E>
-__global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
+__global__ __launch_bounds__(64 * FEW_WAVES) void dense_i8_few_kernel(const int8_t *__restrict__ q, long long ldq, const float *__restrict__ qscale,
                                                                     const int8_t *__restrict__ W, const float *__restrict__ wscale,
                                                                     const float *__restrict__ bias, E *__restrict__ y,
                                                                     const long long *__restrict__ offsets, int G, int M, int N, int K, int relu)
 {
-    __shared__ i32x4 part[few::WAVES][64];
+    __shared__ i32x4 part[FEW_WAVES][64];
     const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63;
     if (g == G) return few_zeros(y, offsets, G, M, N, n0);
     int row0 = 0, rows = M;
@@ -240,7 +241,7 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
     const int8_t *wrow = W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K;
     for (int r0 = 0; r0 < rows; r0 += 16) {
         const int r = row0 + min(r0 + (lane & 15), rows - 1);
-        few::Dot<I8, 4> dot;
+        few::Dot<I8, 4, FEW_WAVES> dot;
         dot.begin(wrow, W + (long long)G * N * K, K);
         const i32x4 acc = dot.multiply(few::RowOf<I8>{q + r * ldq, q + M * ldq});
         few_out(acc, part, y + (long long)r * N, r0 + (lane & 15) < rows, qscale[r], wscale + (long long)g * N, bias ? bias + (long long)g * N : nullptr,
@@ -250,6 +251,8 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_few_kernel(const int8_t
 
 // A few short rows: every workgroup makes their codes itself, in LDS, while its first weights are on their way -- the same codes as
 // quantize_rows_kernel's, without its launch.  ONE: the whole workgroup takes the one row, K <= 8192; otherwise a wave takes a row.
+// Eight waves for one row (us in a captured graph, four | eight waves: 4096 x 4096 10.1 | 7.8) and for five to eight (8 x 1024 x 4096 8.4 |
+// 7.0), four for two to four (4 x 1024 x 4096 5.7 | 6.7).
 constexpr int OWN_ROWS = 8, OWN_BYTES = 8192, OWN_LDS = OWN_BYTES + OWN_ROWS * 144;
 struct Codes {                               // in LDS, zeros behind the row
     const int8_t *q;
@@ -257,13 +260,13 @@ struct Codes {                               // in LDS, zeros behind the row
     __device__ __forceinline__ u32x4 part(int c, int) const { return whole(c); }
 };
 
-template <class E, bool ONE>
-__global__ __launch_bounds__(few::THREADS) void dense_i8_own_kernel(const E *__restrict__ x, const int8_t *__restrict__ W,
+template <class E, bool ONE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void dense_i8_own_kernel(const E *__restrict__ x, const int8_t *__restrict__ W,
                                                                     const float *__restrict__ wscale, const float *__restrict__ bias,
                                                                     E *__restrict__ y, const long long *__restrict__ offsets, int G, int M, int N,
                                                                     int K, int relu)
 {
-    __shared__ i32x4 part[few::WAVES][64];
+    __shared__ i32x4 part[WAVES][64];
     __shared__ __attribute__((aligned(16))) int8_t codes[OWN_LDS];
     __shared__ float scales[OWN_ROWS];
     const int g = blockIdx.y, n0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -271,14 +274,14 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_own_kernel(const E *__r
     int row0 = 0, rows = M;
     if (offsets) group_rows(offsets, G, M, g, row0, rows);
     if (rows == 0) return;
-    few::Dot<I8, 4, true> dot;
+    few::Dot<I8, 4, WAVES, true> dot;
     dot.begin(W + ((long long)g * N + min(n0 + (lane & 15), N - 1)) * K, W + (long long)G * N * K, K);
     const int ldq = (K + 127) / 128 * 128, stride = ldq + 16;        // 16: the rows' chunks in different banks
     if constexpr (ONE) {
-        quantize_row<E, few::THREADS, OWN_BYTES / 8 / few::THREADS, few::THREADS>(x, K, codes, ldq, scales);
+        quantize_row<E, 64 * WAVES, OWN_BYTES / 8 / (64 * WAVES), 64 * WAVES>(x, K, codes, ldq, scales);
     } else {
-        for (int r = wave; r < rows; r += few::WAVES)
-            quantize_row<E, 64, 2048 / 8 / 64, few::THREADS>(x + (long long)(row0 + r) * K, K, codes + r * stride, ldq, scales + r);
+        for (int r = wave; r < rows; r += WAVES)
+            quantize_row<E, 64, 2048 / 8 / 64, 64 * WAVES>(x + (long long)(row0 + r) * K, K, codes + r * stride, ldq, scales + r);
     }
     __syncthreads();
     const int r = min(lane & 15, rows - 1);
@@ -288,8 +291,8 @@ __global__ __launch_bounds__(few::THREADS) void dense_i8_own_kernel(const E *__r
 }
 
 // Every 16 columns make the codes again: for rows whose codes take little more than the launch that this saves.  us a call | in a
-// captured graph, codes here / in a launch of their own: 1 x 640 x 8000 8.4 / 12.2 | 6.5 / 6.9, 4 x 1024 x 4096 8.3 / 12.3 | 5.7 / 6.5,
-// 8 x 1024 x 4096 9.0 / 12.6 | 8.4 / 6.8, 8 x 640 x 8000 10.5 / 12.7 | 10.2 / 7.8 (not taken).
+// captured graph, codes here / in a launch of their own: 1 x 640 x 8000 8.3 / 12.2 | 6.0 / 6.9, 4 x 1024 x 4096 8.3 / 12.3 | 5.7 / 6.5,
+// 8 x 1024 x 4096 8.5 / 12.6 | 7.0 / 6.8, 8 x 640 x 8000 (four waves) 10.5 / 12.7 | 10.2 / 7.8 (not taken).
 bool own_codes(int M, int N, int K)
 {
     if (M == 1) return K <= OWN_BYTES;
@@ -357,9 +360,9 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
           void *workspace, hipStream_t st)
 {
     if (own_codes(M, N, K)) {
-        const auto kernel = M == 1 ? dense_i8_own_kernel<E, true> : dense_i8_own_kernel<E, false>;
-        hipLaunchKernelGGL(kernel, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, (const E *)x, W, wscale, b, (E *)y,
-                           (const long long *)offsets, G, M, N, K, relu);
+        const auto kernel = M == 1 ? dense_i8_own_kernel<E, true, 8> : M <= 4 ? dense_i8_own_kernel<E, false, 4> : dense_i8_own_kernel<E, false, 8>;
+        hipLaunchKernelGGL(kernel, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(M > 1 && M <= 4 ? 256 : 512), 0, st, (const E *)x, W, wscale, b,
+                           (E *)y, (const long long *)offsets, G, M, N, K, relu);
         WM_LAUNCH_CHECK("dense_i8_own_kernel");
         return WM_OK;
     }
@@ -368,7 +371,7 @@ int dense(const void *x, const int8_t *W, const float *wscale, const float *b, v
     const long long ldq = (long long)padded(K);
     if (int rc = quantize<E>(x, M, K, q, ldq, scale, st)) return rc;
     if (few_rows(G, M, N, K)) {
-        hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(few::THREADS), 0, st, q, ldq, scale, W, wscale, b,
+        hipLaunchKernelGGL(dense_i8_few_kernel<E>, dim3((N + 15) / 16, offsets ? G + 1 : 1), dim3(64 * FEW_WAVES), 0, st, q, ldq, scale, W, wscale, b,
                            (E *)y, (const long long *)offsets, G, M, N, K, relu);
         WM_LAUNCH_CHECK("dense_i8_few_kernel");
         return WM_OK;
