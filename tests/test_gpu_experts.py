@@ -814,3 +814,48 @@ def test_expert_stack_trains_and_serves(dtype):
         a, err = z, e8
     assert bool(((y8 - a).abs() <= 1.01 * err).all())
     assert float((y8 - a).norm() / a.norm()) < 0.05
+
+
+def apart(spans):
+    """Whether no two of the (begin, length) share an element."""
+    spans = sorted(spans)
+    return all(a + n <= b for (a, n), (b, _) in zip(spans, spans[1:]))
+
+
+def test_expert_stack_draws_no_element_twice():
+    """Steps of unlike numbers of rows -- the last batch of an epoch is shorter --, eager ones and replays of a graph in
+    turn: each draws from where its `drawn` says, and no two from the same elements."""
+    from weather_model_amd.experts import ExpertStack
+    widths, p, seed = [20, 48, 33, 10], 0.25, 6
+    st = ExpertStack([rows(10 + l, (2, n, k), torch.float32, k ** -0.5).cuda() for l, (k, n) in enumerate(zip(widths, widths[1:]))],
+                     [rows(20 + l, (2, n), torch.float32, 0.1).cuda() for l, n in enumerate(widths[1:])], p=p, seed=seed)
+    spans = [[], []]
+
+    def seen(M):
+        for l, at in enumerate(st.drawn.tolist()):
+            n = M * widths[l + 1]
+            keep = kept(n, p, seed, at).view(M, widths[l + 1])
+            assert not bool(st.h[l + 1].cpu()[~keep].any()), (l, M)
+            spans[l].append((at, n))
+            assert apart(spans[l]), (l, M, spans[l])
+    def step(M):
+        off = torch.tensor([0, M // 3, M], device="cuda")
+        return st.step_grads(rows(M, (M, widths[0]), torch.float32).cuda(), off, rows(M + 1, (M, widths[-1]), torch.float32).cuda())
+    for M in (100, 7, 3, 64, 1, 1, 90):
+        step(M)
+        seen(M)
+    M = 40
+    sx, sg, off = rows(1, (M, widths[0]), torch.float32).cuda(), rows(2, (M, widths[-1]), torch.float32).cuda(), offsets_of([13, 27])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        st.step_grads(sx, off, sg)
+    captured = st.h
+    for other in (200, 5, 0, 1):
+        graph.replay()
+        torch.cuda.synchronize()
+        st.h = captured
+        seen(M)
+        if other:
+            step(other)
+            seen(other)

@@ -34,8 +34,11 @@ class ExpertStack:
                     (l and w.shape[2] != self.w[l - 1].shape[1]):
                 raise ValueError(f"layer {l}: weight {tuple(w.shape)} and bias {tuple(b.shape)} do not fit")
         self.p, self.seed = float(p), int(seed)
-        # where each layer's dropout last drew, on the device: the replays of a captured step move on as eager steps do
+        # where each layer's dropout last drew, on the device: the replays of a captured step move on as eager steps do.
+        # `span` is the most that any step has drawn from there, so that a step goes past what the one before it drew,
+        # however many rows that had; a graph replayed between eager steps finds it on the device too.
         self.drawn = torch.arange(len(weights) - 1, device=self.w[0].device, dtype=torch.int64) << 48
+        self.span = torch.zeros((1,), device=self.w[0].device, dtype=torch.int64)
         self.h = None
         sizes = [t.numel() for t in self.w + self.b]
         self.flat_grads = torch.zeros((sum(sizes),), device=self.w[0].device, dtype=self.w[0].dtype)
@@ -49,7 +52,8 @@ class ExpertStack:
         h, L = [x], len(self.w)
         drop = train and L > 1 and self.p > 0
         if drop:
-            self.drawn.add_(x.shape[0] * max(w.shape[1] for w in self.w[:-1]))
+            self.span.clamp_(min=x.shape[0] * max(w.shape[1] for w in self.w[:-1]))
+            self.drawn.add_(self.span)
         for l, (w, b) in enumerate(zip(self.w, self.b)):
             y = ops.dense_grouped_forward(h[-1], w, offsets, b, relu=l + 1 < L)
             if drop and l + 1 < L:
