@@ -859,3 +859,19 @@ def test_expert_stack_draws_no_element_twice():
         if other:
             step(other)
             seen(other)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_expert_stack_serves_the_weights_and_biases_it_quantised(dtype):
+    """Training that goes on in place does not reach what `predict` answers with."""
+    from weather_model_amd.experts import ExpertStack
+    widths = [24, 40, 9]
+    ws = [rows(10 + l, (2, n, k), dtype, k ** -0.5).cuda() for l, (k, n) in enumerate(zip(widths, widths[1:]))]
+    bs = [rows(20 + l, (2, n), dtype).cuda() for l, n in enumerate(widths[1:])]
+    x, off = rows(1, (50, widths[0]), dtype).cuda(), offsets_of([20, 30])
+    st = ExpertStack(ws, bs).quantize()
+    before = st.predict(x, off).clone()
+    for t in ws + bs:
+        t.add_(1.0)
+    assert torch.equal(st.predict(x, off), before)
+    assert not torch.equal(st.quantize().predict(x, off), before)

@@ -85,11 +85,12 @@ class ExpertStack:
         return self.flat_grads
 
     def quantize(self):
-        """Codes and scales of the present weights, for ``predict``."""
+        """Codes and scales of the present weights, and the present biases, for ``predict``; later changes in place do not
+        reach them."""
         self.codes = []
         for w, b in zip(self.w, self.b):
             q, s = ops.quantize_rows(w.reshape(-1, w.shape[2]))
-            self.codes.append((q.view(w.shape), s.view(w.shape[:2]), b.float()))
+            self.codes.append((q.view(w.shape), s.view(w.shape[:2]), b.to(torch.float32, copy=True)))
         return self
 
     def predict(self, x, offsets):
