@@ -87,3 +87,14 @@ def test_group_offsets():
         ops.group_offsets(torch.ones(3))
     with pytest.raises(ValueError, match="counts must be"):
         ops.group_offsets(torch.ones((2, 2), dtype=torch.int64))
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """Views of one element: nothing is allocated."""
+    from weather_model_amd import ops
+    n = 2 ** 32 + 4
+    for shape in ((n, 1), (1, n), (3, 2 ** 31), (1, n, 1), (n, 1, 2)):
+        with pytest.raises(ValueError, match="beyond 32 bits"):
+            ops._in_32_bits(torch.zeros((1,) * len(shape)).expand(shape), "input")
+    for shape in ((2 ** 31 - 1, 4), (2 ** 31 - 1,), (0, 5), (), (70000, 70000)):
+        ops._in_32_bits(torch.zeros((1,) * len(shape)).expand(shape) if shape else torch.zeros(()), "input")

@@ -875,3 +875,26 @@ def test_expert_stack_serves_the_weights_and_biases_it_quantised(dtype):
         t.add_(1.0)
     assert torch.equal(st.predict(x, off), before)
     assert not torch.equal(st.quantize().predict(x, off), before)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """A count that the C interface could only take modulo 2^32; the tensors are views of one element."""
+    from weather_model_amd import ops
+    n = 2 ** 32 + 4
+
+    def view(*shape, dtype=torch.bfloat16):
+        return torch.zeros((1,) * len(shape), dtype=dtype, device="cuda").expand(shape)
+    one, off = view(1, 1, 1), offsets_of([4])
+    calls = [lambda: ops.dense_grouped_forward(view(n, 1), one, off), lambda: ops.dense_grouped_forward(view(4, n), view(1, 1, n), off),
+             lambda: ops.dense_grouped_forward(view(4, 1), view(1, n, 1), off),
+             lambda: ops.dense_grouped_backward(view(n, 1), one, off, view(n, 1)), lambda: ops.quantize_rows(view(n, 1)),
+             lambda: ops.dense_i8(view(n, 1), view(1, 1, dtype=torch.int8), view(1, dtype=torch.float32)),
+             lambda: ops.dense_i8(view(4, 1), view(n, 1, dtype=torch.int8), view(n, dtype=torch.float32))]
+    for k, call in enumerate(calls):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        with pytest.raises(ValueError, match="beyond 32 bits"):
+            call()
+            raise AssertionError(f"call {k} was taken")
+        assert torch.cuda.max_memory_allocated() < before + (1 << 20), k          # nothing was copied first

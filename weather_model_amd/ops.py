@@ -956,7 +956,13 @@ def mse_metrics(pred, y, broadcast, eps=1e-7, want_grad=True):
 _DTYPES = {torch.float32: 0, torch.bfloat16: 2, torch.float16: 3}      # WM_F32, WM_BF16, WM_F16
 
 
-def _req_any(t, name, like=None):
+def _in_32_bits(t, name):
+    """The C interface takes sizes as 32-bit integers: larger ones are refused before anything is copied."""
+    if t.numel() > 0x7FFFFFFF and max(t.shape) > 0x7FFFFFFF:
+        raise ValueError(f"{name} {tuple(t.shape)} has a size beyond 32 bits")
+
+
+def _req_any(t, name, like=None, any_size=False):
     """``_req`` for the operators that also take bfloat16 and float16; ``like`` fixes type and device."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -968,6 +974,8 @@ def _req_any(t, name, like=None):
         if t.dtype != like.dtype:
             raise TypeError(f"{name} must be {like.dtype} like the rows, got {t.dtype}")
         _same_device(t, name, like)
+    if not any_size:
+        _in_32_bits(t, name)
     return t.contiguous()
 
 
@@ -1163,10 +1171,10 @@ def dropout_forward(x, p, seed, offset=0, residual=None, out=None):
     nowhere: the backward pass draws it again.  ``offset`` is an integer or one int64 on the GPU (read by
     the kernel, so that replays of a captured graph can move on); advance it by x.numel() from call to
     call.  float32, bfloat16 or float16; p is held to 2^-32; ``out`` may be x or residual."""
-    x = _req_any(x, "input")
+    x = _req_any(x, "input", any_size=True)
     p, seed, off, off_dev = _dropout_args(p, seed, offset, x)
     if residual is not None:
-        residual = _req_any(residual, "residual", x)
+        residual = _req_any(residual, "residual", x, any_size=True)
         if residual.shape != x.shape:
             raise ValueError(f"residual must be {tuple(x.shape)}, got {tuple(residual.shape)}")
     if out is None:
@@ -1231,6 +1239,8 @@ def dense_i8(x, weight, scale, bias=None, relu=False, offsets=None, out=None):
     both), bias (N,) float32.  Exact integer sums, output in the type of x.  With ``offsets`` (G + 1,) the
     rows are grouped as in ``dense_grouped_forward``: weight (G, N, K), scale and bias (G, N)."""
     x = _req_any(x, "input")
+    if isinstance(weight, torch.Tensor):
+        _in_32_bits(weight, "weight")
     weight = _same_device(_req(weight, "weight", torch.int8), "weight", x)
     scale = _same_device(_req(scale, "scale"), "scale", x)
     lead = 2 if offsets is None else 3
