@@ -464,7 +464,8 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
  * Rows that no expert owns (before offsets[0], behind offsets[G]) get zeros in y and gx and add nothing to gW and
  * gb.  Any values of offsets are safe: those outside 0 .. M count as the nearest inside, one below its
  * predecessor counts as that.  Results are bitwise reproducible.  float32 products are formed from three
- * bf16 pieces of each factor, with float32 accuracy; infinities and NaN come out as in float32 arithmetic.
+ * bf16 pieces of each factor, with float32 accuracy for factors of every size, subnormal ones included; infinities and
+ * NaN come out as in float32 arithmetic.
  * N, K <= 2^20, M <= 2^30, G <= 4096.  Outputs may not overlap inputs;
  * workspaces (0 bytes: none is needed) are 16-byte aligned. */
 size_t wm_dense_grouped_fwd_workspace_bytes(int G, int M, int N, int K, int dtype);

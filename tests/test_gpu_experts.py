@@ -898,3 +898,41 @@ def test_sizes_beyond_32_bits_are_refused():
             call()
             raise AssertionError(f"call {k} was taken")
         assert torch.cuda.max_memory_allocated() < before + (1 << 20), k          # nothing was copied first
+
+
+# (sizes, N, K): few rows, small tiles, a contraction in parts forward and backward, chunks of rows, whole tiles
+FAR = [([16], 24, 64), ([40], 24, 64), ([70, 0, 131], 40, 1100), ([70, 131], 1101, 41), ([2000, 0, 1501], 24, 40), ([300, 277], 260, 136)]
+
+
+@pytest.mark.parametrize("case", range(len(FAR)))
+@pytest.mark.parametrize("sx,sw,sy", [(-120, 100, -118), (100, -122, -119), (-124, 0, 60), (10, -118, -121), (-132, 90, -90), (90, 3, -133), (100, 3, 20), (112, -2, 10)])
+def test_grouped_float32_keeps_its_accuracy_for_small_and_large_values(case, sx, sw, sy):
+    """Rows, weights or gradients near and below the smallest normal float32, next to ones that bring the products back, and ones
+    next to the largest: the bound of every other float32 product (the module's tolerances), and the last step of a subnormal result."""
+    from weather_model_amd import ops
+    sizes, N, K = FAR[case]
+    M, G = sum(sizes), len(sizes)
+    x, w, gy = (rows(case + k, s, torch.float32) * 2.0 ** e for k, s, e in ((1, (M, K), sx), (2, (G, N, K), sw), (3, (M, N), sy)))
+    off = offsets_of(sizes)
+    y = ops.dense_grouped_forward(x.cuda(), w.cuda(), off)
+    gx, gw, _ = ops.dense_grouped_backward(x.cuda(), w.cuda(), off, gy.cuda(), need_bias=False)
+
+    def near(got, ref, S, n, what):
+        # a product or a partial sum below 2^-126 is rounded to 2^-149: half a step for each of n
+        acc = (5 * (1.5 * n + 16) ** 0.5 * U + 3 * 2.0 ** -26) * S + (1.5 * n + 16) * 2.0 ** -150
+        got, most = got.cpu().double(), torch.finfo(torch.float32).max
+        d = (got - ref).abs()
+        # past the largest float32 a sum is infinite; where S passes it, a partial sum may be, by the order of the sum
+        beyond = ref.abs() > most * (1 + U) + acc
+        assert not bool(got[beyond].isfinite().any()), what
+        fine = (d <= (1 + U) * acc + U * ref.abs()) | ((S > most) & ~got.isfinite())
+        assert bool(fine.all()), (what, float((d / S.clamp(min=1e-300)).max()))
+    ref, S = grouped_ref(x, w, None, sizes, 0, False)
+    near(y, ref, S, K, "y")
+    ref, S = grouped_ref(gy, w.transpose(1, 2), None, sizes, 0, False)
+    near(gx, ref, S, N, "gx")
+    at = 0
+    for g, n in enumerate(sizes):
+        a, c = gy[at:at + n].double(), x[at:at + n].double()
+        near(gw[g], a.t() @ c, a.abs().t() @ c.abs(), n, (g, "gw"))
+        at += n

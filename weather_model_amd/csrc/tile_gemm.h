@@ -8,12 +8,15 @@
 //   contiguous  c runs along memory: a chunk is one 16-byte load (two for float32)
 //   strided     i (or j) runs along memory: a thread loads 8 c of a few rows and transposes in registers
 //
-// float32 is split into three bf16 pieces, x = h + m + l (each the nearest to what is left: 24 bits), and a
+// float32 is split into three bf16 pieces, 2^16 x = h + m + l (each the nearest to what is left: 24 bits), and a
 // product is the six piece products that are not below 2^-24 of it: hh, hm, mh, hl, lh, mm, each exact in the
 // float32 accumulator.  That is float32 accuracy (what is left out is 3 2^-26 of |a||b| at most) at 2500 / 6
-// TFLOP/s of matrix rate where the float32 MFMA has 157.  An infinity, a NaN or a value that rounds up to
-// infinity in bf16 makes a NaN of its products, and a product next to the largest float32 may overflow in its first
-// piece; elements of C that are not finite are summed again in float32 (not_finite_again).
+// TFLOP/s of matrix rate where the float32 MFMA has 157.  The last bit of a subnormal x is 2^-149 and the last of bf16
+// 2^-133, hence the factor: without it the third piece of |x| < 2^-109 lost bits (5e-5 of 2^-120, all of 2^-133).  It costs
+// two multiplications a pair of values and the sums one by 2^-32 (8191 rows, 8 experts of 1024 -> 1024, forward and gradients
+// 326 | 335 us, 45001 rows of 432 -> 216 72.8 | 74.5).  An infinity, a NaN or a value that rounds up to infinity in bf16
+// (from 2^112 on) makes a NaN of its products, and a sum from 2^96 on may overflow in its first piece; elements of C that
+// are not finite are summed again in float32 (not_finite_again).
 #pragma once
 
 #include <type_traits>
@@ -136,9 +139,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b)
     typedef bf16_t b2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, b2));
 }
-// the three pieces of a pair of float32 values, packed
+// the three pieces of a pair of float32 values times SPLIT_SCALE, packed; a sum of products is then to be multiplied by SPLIT_UNSCALE
+constexpr float SPLIT_SCALE = 0x1p16f, SPLIT_UNSCALE = 0x1p-32f;
 __device__ __forceinline__ void split2(float a, float b, uint32_t out[3])
 {
+    a *= SPLIT_SCALE;
+    b *= SPLIT_SCALE;
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
         out[p] = pack_bf16(a, b);
@@ -578,6 +584,11 @@ __device__ __forceinline__ void product(LA &a, LB &b, int count, char *lds, type
         }
         __syncthreads();
     }
+    if constexpr (S::T::PLANES == 3)
+#pragma unroll
+        for (int m = 0; m < S::MI; ++m)
+#pragma unroll
+            for (int n = 0; n < S::NI; ++n) acc[m][n] *= SPLIT_UNSCALE;
 }
 
 // ---- the way out: a wave turns 16 rows of its results through LDS (its own piece: no barrier) so that a lane holds 16 bytes
