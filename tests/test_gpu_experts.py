@@ -936,3 +936,63 @@ def test_grouped_float32_keeps_its_accuracy_for_small_and_large_values(case, sx,
         a, c = gy[at:at + n].double(), x[at:at + n].double()
         near(gw[g], a.t() @ c, a.abs().t() @ c.abs(), n, (g, "gw"))
         at += n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes", [[9, 0, 4], [150, 0, 261], [1]])
+def test_grouped_autograd_with_the_relu_masks_of_neighbours(sizes, dtype):
+    """Two layers whose ReLU between them is masked by the upper one's gradient of rows (relu_bwd_fused below, relu_input above)
+    give the gradients of the layers by themselves, bit for bit, and those of the formula in float64."""
+    from weather_model_amd import ops
+    M, G, K, H, N = sum(sizes) + 2, len(sizes), 40, 72, 33
+    off = offsets_of(sizes)
+    host = [rows(k, s, dtype, c) for k, s, c in ((1, (M, K), 1.0), (2, (G, H, K), K ** -0.5), (3, (G, H), 0.3), (4, (G, N, H), H ** -0.5), (5, (G, N), 0.3))]
+    gout = rows(6, (M, N), dtype)
+
+    def grads(below, above):
+        x, w1, b1, w2, b2 = leaves = [t.cuda().requires_grad_() for t in host]
+        h = ops.dense_grouped(x, w1, off, b1, relu=True, relu_bwd_fused=below)
+        y = ops.dense_grouped(h, w2, off, b2, relu_input=above)
+        y.backward(gout.cuda())
+        return h.detach().cpu(), [t.grad for t in leaves]
+    h, alone = grads(False, False)
+    for below, above in ((True, True), (False, True)):       # masked twice is masked once
+        h2, fused = grads(below, above)
+        assert torch.equal(h, h2)
+        for k, (a, b) in enumerate(zip(alone, fused)):
+            assert torch.equal(a, b), (below, above, k)
+    _, unmasked = grads(True, False)
+    assert sum(sizes) < 2 or not torch.equal(unmasked[0], alone[0])
+    # gh is rounded to the type once; what it is off by goes on into the lower layer's gradients
+    half, tiny, at = half_step(dtype), torch.finfo(dtype).tiny, 0
+    for g, n in enumerate(sizes):
+        p = slice(at, at + n)
+        go, hd, xd, w1, w2 = (t.double() for t in (gout[p], h[p], host[0][p], host[1][g], host[3][g]))
+        mask = (hd > 0).double()
+        gh, Sh = go @ w2 * mask, go.abs() @ w2.abs() * mask
+        eh = 6 * (1.5 * N + 16) ** 0.5 * U * Sh + half * gh.abs() + tiny
+        for what, got, ref, S, e, terms in (
+                ("gw2", alone[3][g], go.t() @ hd, go.abs().t() @ hd, 0.0, n), ("gb2", alone[4][g], go.sum(0), go.abs().sum(0), 0.0, n),
+                ("gw1", alone[1][g], gh.t() @ xd, gh.abs().t() @ xd.abs(), eh.t() @ xd.abs(), n), ("gb1", alone[2][g], gh.sum(0), gh.abs().sum(0), eh.sum(0), n),
+                ("gx", alone[0][p], gh @ w1, gh.abs() @ w1.abs(), eh @ w1.abs(), H)):
+            tol = 1.01 * (6 * (1.5 * terms + 16) ** 0.5 * U * (S + e) + e + half * (ref.abs() + e) + tiny)
+            assert bool(((got.cpu().double() - ref).abs() <= tol).all()), (what, g)
+        at += n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,p,offset", [(1, 0.5, 0), (4099, 0.1, 1), (100003, 0.9, 2), (65536, 0.5, 2 ** 33 + 3), (262144, 2.0 ** -16, 8), (5000, 1.0, 0)])
+def test_dropout_zeros_are_the_dropped_elements_and_the_gradient_is_the_draws(n, p, offset, dtype):
+    """Every type: a result is zero where and only where the element is dropped or was zero (a kept value grows), and the backward
+    pass gives gy / (1 - p) of the same elements."""
+    from weather_model_amd import ops
+    x, gy = rows(n, (n,), dtype), rows(n + 1, (n,), dtype)
+    x[:: 97], gy[:: 89] = torch.finfo(dtype).smallest_normal, -torch.finfo(dtype).smallest_normal
+    keep = kept(n, p, 31, offset)
+    scale = 0.0 if p == 1.0 else 1.0 / (1.0 - round(p * 2 ** 32) / 2 ** 32)
+    for t, got in ((x, ops.dropout_forward(x.cuda(), p, 31, offset=offset)), (gy, ops.dropout_backward(gy.cuda(), p, 31, offset=offset))):
+        got, ref = got.cpu(), torch.where(keep, t.double() * scale, 0.0)
+        assert torch.equal(got == 0, ~keep | (t == 0))
+        # the scale and the product are rounded in float32, the result to its type (a subnormal one to its last step)
+        last = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+        assert bool(((got.double() - ref).abs() <= (2.1 * U + half_step(dtype)) * ref.abs() + last / 2).all())
