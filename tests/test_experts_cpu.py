@@ -98,3 +98,15 @@ def test_sizes_beyond_32_bits_are_refused():
             ops._in_32_bits(torch.zeros((1,) * len(shape)).expand(shape), "input")
     for shape in ((2 ** 31 - 1, 4), (2 ** 31 - 1,), (0, 5), (), (70000, 70000)):
         ops._in_32_bits(torch.zeros((1,) * len(shape)).expand(shape) if shape else torch.zeros(()), "input")
+
+
+def test_expert_stack_refuses_what_is_no_probability_and_no_seed():
+    """When it is made: a negative p or a NaN would train without dropout, and a seed would only be looked at by the first step."""
+    from weather_model_amd.experts import ExpertStack
+    w, b = [torch.zeros(2, 3, 4)], [torch.zeros(2, 3)]
+    for p in (-0.1, 1.5, float("nan")):
+        with pytest.raises(ValueError, match="probability"):
+            ExpertStack(w, b, p=p)
+    for seed in (-1, 1 << 32):
+        with pytest.raises(ValueError, match="seed"):
+            ExpertStack(w, b, seed=seed)

@@ -21,11 +21,13 @@ from . import dp, ops
 
 
 class ExpertStack:
-    """weights: (G, N_l, K_l) per layer, biases: (G, N_l); float32, bfloat16 or float16, all alike."""
+    """weights: (G, N_l, K_l) per layer, biases: (G, N_l); float32, bfloat16 or float16, all alike.  p and seed are
+    dropout's (``ops.dropout_forward``); ranks that train together take a seed each, as they draw by the row of their own batch."""
 
     def __init__(self, weights, biases, p=0.0, seed=0):
         if len(weights) != len(biases) or not weights:
             raise ValueError("one bias per weight, at least one layer")
+        self.p, self.seed = ops._dropout_args(p, seed, 0, None)[:2]
         self.w = [ops._req_any(weights[0], "weight")]
         self.w += [ops._req_any(w, "weight", self.w[0]) for w in weights[1:]]
         self.b = [ops._req_any(b, "bias", self.w[0]) for b in biases]
@@ -33,7 +35,6 @@ class ExpertStack:
             if w.dim() != 3 or w.shape[0] != self.w[0].shape[0] or tuple(b.shape) != tuple(w.shape[:2]) or \
                     (l and w.shape[2] != self.w[l - 1].shape[1]):
                 raise ValueError(f"layer {l}: weight {tuple(w.shape)} and bias {tuple(b.shape)} do not fit")
-        self.p, self.seed = float(p), int(seed)
         # where each layer's dropout last drew, on the device: the replays of a captured step move on as eager steps do.
         # `span` is the most that any step has drawn from there, so that a step goes past what the one before it drew,
         # however many rows that had; a graph replayed between eager steps finds it on the device too.
