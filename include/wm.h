@@ -457,8 +457,8 @@ int wm_linear_metrics_wide_f32(const float *X, const float *Y, const double *bet
  * linear map per WRF variable (multipleRegression.py:28-45,533-550).  x, W, b and y are all of `dtype`
  * (WM_F32, WM_BF16 or WM_F16); sums are held in float32.
  *   fwd       y[r] = act(W[g] x[r] + b[g]); b may be NULL; relu != 0 applies max(., 0)
- *   bwd_data  gx[r] = W[g]^T gy[r], zeroed where mask_below <= 0 when mask_below != NULL (the post-ReLU
- *             activation that fed this layer, shaped like gx); gy is the gradient of the pre-activation
+ *   bwd_data  gx[r] = W[g]^T gy[r], zero where mask_below is not > 0 (NaN among them) when mask_below != NULL (the
+ *             post-ReLU activation that fed this layer, shaped like gx); gy is the gradient of the pre-activation
  *   bwd_wb    gW[g] = sum_r gy[r] x[r]^T, gb[g] = sum_r gy[r] (gb may be NULL); zeros for an expert
  *             without rows; large sums are split over rows and joined in a fixed order through `workspace`
  * Rows that no expert owns (before offsets[0], behind offsets[G]) get zeros in y and gx and add nothing to gW and

@@ -48,7 +48,7 @@ __device__ __forceinline__ void draw(uint64_t seed, uint64_t e0, unsigned sub, u
 }
 
 // A thread takes UNROLL vectors of 16 bytes, BLOCK vectors apart: their loads go out before the first hash.
-// Bound by HBM: 32768 x 2048 bf16 with a residual 70 us = 5.7 TB/s, without 40 us = 6.7 (a copy of 512 MiB 5.3); small calls by the launch.
+// Bound by HBM: 32768 x 2048 bf16 with a residual 76 us = 5.3 TB/s, without 43 us = 6.2 (a copy of 512 MiB 5.3); small calls by the launch.
 template <class T, bool RES>
 __global__ __launch_bounds__(BLOCK) void dropout_kernel(const T *x, const T *res, T *y,
                                                         long long n, uint64_t seed, uint64_t offset,

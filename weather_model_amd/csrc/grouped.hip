@@ -6,7 +6,7 @@
 // The number of rows of an expert is only known on the device, so a launch has as many workgroups as any
 // partition of M rows can need tiles, and each finds its tile from the offsets (tile_gemm.h).
 // Bound by the matrix unit where the experts have hundreds of rows (direct_gemm.h has the figures of 16 bits; float32, 8191 rows, 8
-// experts of 1024 -> 1024: forward 104 us = 165 TFLOP/s, gx 124, gW 115, where a library float32 product of 8192^3 makes 155 and
+// experts of 1024 -> 1024: forward 107 us = 161 TFLOP/s, gx 132, gW 123, where a library float32 product of 8192^3 makes 155 and
 // six bf16 products could make 227: splitting and LDS reads share the issue slots), by reading the weights where they have a few.
 #include "direct_gemm.h"
 #include "few_rows.h"
@@ -485,7 +485,8 @@ int rows_any(int dtype, const void *x, const void *W, const void *bias, const vo
 // 98 84 98 126 (8); with at least 128, 256, 512, 1024 rows: bf16, 1 expert, 4096 rows 19 15 16 21 (taken: 256), 17112 rows of 16 x 73 -> 116
 // 15 15 20 28; float32 27 30 43 70 (128), 23 27 40 66.  Where the experts are enough, but one alone would be far from filling the card: 64
 // experts, 45000 rows in one of them 2500 us whole in float32, 570 in bf16; 101 and 52 in chunks; evenly spread it costs the launch that
-// finds nothing to add.
+// finds nothing to add.  Layers of more tiles stay whole, whose parts would be as large as the weights for each chunk (all rows in one of 8
+// experts of 1024 -> 1024 | evenly spread: 8192 rows float32 460 | 118, 16384 rows bf16 213 | 53; 16 experts of 2048 -> 4096 414 | 323).
 int weight_chunk(int M, int N, int K, int G, int dtype)
 {
     const int round = dtype == WM_F32 ? 512 : 256, least = dtype == WM_F32 ? 128 : 256;

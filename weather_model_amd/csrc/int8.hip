@@ -290,9 +290,11 @@ __global__ __launch_bounds__(64 * WAVES) void dense_i8_own_kernel(const E *__res
             bias ? bias + (long long)g * N : nullptr, n0, N, relu);
 }
 
-// Every 16 columns make the codes again: for rows whose codes take little more than the launch that this saves.  us a call | in a
-// captured graph, codes here / in a launch of their own: 1 x 640 x 8000 8.3 / 12.2 | 6.0 / 6.9, 4 x 1024 x 4096 8.3 / 12.3 | 5.7 / 6.5,
-// 8 x 1024 x 4096 8.5 / 12.6 | 7.0 / 6.8, 8 x 640 x 8000 (four waves) 10.5 / 12.7 | 10.2 / 7.8 (not taken).
+// Every 16 columns make the codes again: for rows whose codes take little more than the launch that this saves.  The choice is by the time
+// of a call; in a captured graph it is within 0.1 us of the other or better.  us a call | in a captured graph, float32, codes here /
+// in a launch of their own: 1 x 640 x 8000 8.3 / 12.7 | 6.3 / 6.7, 1 x 4096 x 4096 8.2 / 12.6 | 6.0 / 7.7, 2 x 2048 x 4096 8.3 / 12.5 | 6.1 /
+// 6.0, 3 and 4 x 2048 x 4096 8.3 / 12.6 | 6.3 / 6.2, 4 x 1024 x 4096 8.3 / 12.7 | 5.3 / 6.2, 8 x 1024 x 4096 8.4 / 12.9 | 6.6 / 6.5, 8 x 640 x
+// 8000 (four waves) 10.5 / 12.7 | 10.2 / 7.8 (not taken).
 bool own_codes(int M, int N, int K)
 {
     if (M == 1) return K <= OWN_BYTES;
